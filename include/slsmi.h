@@ -601,6 +601,84 @@ int slsmi_window_topk(float* enc, uint16_t* enc_bf16, void* scratch, size_t scra
                       int dict, int k, int window, int fmt, void* stream);
 size_t slsmi_window_topk_scratch_bytes(int B, int T, int dict, int window);
 
+/* ---- attention for recordings of any length and for live streams ------------
+ * No counterpart in the reference, whose encoder attends over a whole clip (wav2vec2.py:1046-1052) and was trained
+ * without a norm on queries and keys.  q, k, v: 16-bit (fmt), head widths 64 and 128, query head h reads key head
+ * h / (heads / kv_heads). */
+
+/* Norms of queries and keys for each head and the rotation by position, in one pass over the rows the QKV projection
+ * wrote.  x [rows][ldx]: heads query heads, then kv_heads key heads of head_dim channels (what follows them is left
+ * alone).  For each head x: n = x / sqrt(mean x^2 + eps) * w (wq [head_dim] or wk [head_dim], fp32), and the first
+ * rotary_dim channels of n as pairs turned by p * freqs[i] radians: (n_i, n_(i + rotary_dim / 2)), or with interleaved != 0
+ * (n_2i, n_(2i + 1)).  freqs [rotary_dim / 2] doubles; rotary_dim a multiple of 16 up to head_dim, or 0 with freqs NULL.
+ * p = positions[row % npos] (int64, device), or row % npos where positions is NULL: npos = rows, or frames per recording.
+ * Angles are formed in 64 bits.  y [rows][ldy] may be x itself.  ldx, ldy multiples of 8, pointers 16-byte aligned. */
+int slsmi_qk_norm_rope(const uint16_t* x, int64_t ldx, uint16_t* y, int64_t ldy, int64_t rows, int heads, int kv_heads,
+                       int head_dim, const float* wq, const float* wk, float eps, const double* freqs, int rotary_dim,
+                       int interleaved, const int64_t* positions, int64_t npos, int fmt, void* stream);
+
+/* Its gradient: dy at y, x as given to the forward (not its result) -> dx [rows][lddx] (may be dy itself; columns past the
+ * heads are left alone) and dwq, dwk [head_dim] fp32, written whole (rows == 0: zeros), summed in a fixed order.
+ * workspace: slsmi_qk_norm_rope_backward_workspace_bytes() bytes, 16-byte aligned, free again when the call's work is done. */
+int slsmi_qk_norm_rope_backward(const uint16_t* dy, int64_t lddy, const uint16_t* x, int64_t ldx, uint16_t* dx, int64_t lddx,
+                                int64_t rows, int heads, int kv_heads, int head_dim, const float* wq, const float* wk,
+                                float eps, const double* freqs, int rotary_dim, int interleaved, const int64_t* positions,
+                                int64_t npos, float* dwq, float* dwk, void* workspace, size_t workspace_bytes, int fmt,
+                                void* stream);
+size_t slsmi_qk_norm_rope_backward_workspace_bytes(int64_t rows, int head_dim);
+
+/* One of q, k, v, ... as [batch][frames][heads][head_dim] by element strides (host struct, device data): channels
+ * contiguous, data 16-byte aligned, strides multiples of 8, rows and heads disjoint. */
+typedef struct slsmi_heads {
+    uint16_t* data;
+    int64_t batch, row, head;
+} slsmi_heads;
+
+typedef struct slsmi_window_shape {
+    int32_t batch, frames;     /* frames: T, the padded length (at most 2^29) */
+    int32_t heads, kv_heads;   /* heads a multiple of kv_heads */
+    int32_t head_dim;          /* 64 or 128 */
+    int32_t left, right;       /* frames a query sees before and after itself; -1: no limit; right 0: causal */
+    int32_t sinks;             /* 0 .. 128: first frames that stay visible to every later query */
+    int32_t fmt;
+    float scale;               /* of the scores, > 0 */
+} slsmi_window_shape;
+
+/* Attention with a sliding window and sinks: query i of a recording of n frames (nframes [batch] int32 on the device,
+ * clamped to [0, frames]; NULL: frames) sees key j where j < n, j <= i + right and (j >= i - left or j < sinks).
+ * out rows of padded frames are written as zeros; what q, k, v hold there is never used.  lse: NULL or fp32
+ * [batch][heads][frames], the log of the sum of exponentials per row (-inf at padded frames): what the backward needs. */
+int slsmi_window_attention(const slsmi_window_shape* shape, const slsmi_heads* q, const slsmi_heads* k, const slsmi_heads* v,
+                           const slsmi_heads* out, float* lse, const int32_t* nframes, void* stream);
+
+/* Its gradient, from the forward's out and lse: dq, dk, dv written whole (zeros at padded frames), the same bits on every
+ * call.  workspace: slsmi_window_attention_backward_workspace_bytes() bytes, 16-byte aligned. */
+int slsmi_window_attention_backward(const slsmi_window_shape* shape, const slsmi_heads* dout, const slsmi_heads* q,
+                                    const slsmi_heads* k, const slsmi_heads* v, const slsmi_heads* out, const float* lse,
+                                    const int32_t* nframes, const slsmi_heads* dq, const slsmi_heads* dk,
+                                    const slsmi_heads* dv, void* workspace, size_t workspace_bytes, void* stream);
+size_t slsmi_window_attention_backward_workspace_bytes(const slsmi_window_shape* shape);
+
+/* A live stream: one new frame per sequence against a rolling cache k_cache, v_cache [batch][kv_heads][slots][head_dim]
+ * (slots > sinks; the window is slots - sinks frames, the new one among them; slots at most 2^24).  Position p lives in
+ * slot p for p < sinks, else in sinks + (p - sinks) mod (slots - sinks).  qkv [batch][ld]: the new frame's query, key and
+ * value heads; positions [batch] int64 on the device: its position in each sequence, negative for a sequence that has no
+ * frame now (its out rows become zeros, its cache is left alone).  With wq, wk (see slsmi_qk_norm_rope; NULL, NULL: q and
+ * k are taken as they are, rotary_dim 0) norm and rotation happen here.  The key and value are written to the cache and
+ * out [batch][heads][head_dim] = attention over the sinks and the window, as slsmi_window_attention with right = 0 and
+ * left = slots - sinks - 1 gives for that row.  Of `shape` frames, left and right are not read.
+ * workspace: slsmi_window_step_workspace_bytes() bytes (may be 0), 16-byte aligned. */
+int slsmi_window_step(const slsmi_window_shape* shape, int slots, const uint16_t* qkv, int64_t ld, uint16_t* k_cache,
+                      uint16_t* v_cache, const int64_t* positions, const float* wq, const float* wk, float eps,
+                      const double* freqs, int rotary_dim, int interleaved, uint16_t* out, void* workspace,
+                      size_t workspace_bytes, void* stream);
+size_t slsmi_window_step_workspace_bytes(const slsmi_window_shape* shape, int slots);
+
+/* Prefill: the keys (normalised and turned) and values of recordings that begin at position 0, nframes as above, into the
+ * slots their sinks and their last slots - sinks frames live in.  Slots no frame lives in are left alone. */
+int slsmi_window_cache_fill(const slsmi_window_shape* shape, int slots, const slsmi_heads* k, const slsmi_heads* v,
+                            uint16_t* k_cache, uint16_t* v_cache, const int32_t* nframes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

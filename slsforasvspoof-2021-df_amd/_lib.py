@@ -52,6 +52,18 @@ class Config(C.Structure):
     ]
 
 
+class Heads(C.Structure):
+    """slsmi_heads of include/slsmi.h: [batch][frames][heads][head_dim] by element strides."""
+    _fields_ = [("data", C.c_void_p), ("batch", C.c_int64), ("row", C.c_int64), ("head", C.c_int64)]
+
+
+class WindowShape(C.Structure):
+    """slsmi_window_shape of include/slsmi.h."""
+    _fields_ = [("batch", C.c_int32), ("frames", C.c_int32), ("heads", C.c_int32), ("kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("left", C.c_int32), ("right", C.c_int32), ("sinks", C.c_int32),
+                ("fmt", C.c_int32), ("scale", C.c_float)]
+
+
 _lib: Optional[C.CDLL] = None
 
 # name -> (restype, argtypes); every symbol include/slsmi.h declares
@@ -123,6 +135,21 @@ SIGNATURES = {
     "slsmi_ln1024_f32_bf16": (C.c_int, [_P, _P, C.c_int64, _P, _P, C.c_float, C.c_int, _P]),
     "slsmi_attention": (C.c_int, [_P, _P, C.c_int, C.c_int, C.c_int, _P]),
     "slsmi_attention_varlen": (C.c_int, [_P, _P, C.c_int, C.c_int, _P, C.c_int, _P]),
+    "slsmi_qk_norm_rope": (C.c_int, [_P, C.c_int64, _P, C.c_int64, C.c_int64, C.c_int, C.c_int, C.c_int, _P, _P, C.c_float, _P,
+                                     C.c_int, C.c_int, _P, C.c_int64, C.c_int, _P]),
+    "slsmi_qk_norm_rope_backward": (C.c_int, [_P, C.c_int64, _P, C.c_int64, _P, C.c_int64, C.c_int64, C.c_int, C.c_int,
+                                              C.c_int, _P, _P, C.c_float, _P, C.c_int, C.c_int, _P, C.c_int64, _P, _P, _P,
+                                              C.c_size_t, C.c_int, _P]),
+    "slsmi_qk_norm_rope_backward_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int]),
+    "slsmi_window_attention": (C.c_int, [C.POINTER(WindowShape)] + [C.POINTER(Heads)] * 4 + [_P, _P, _P]),
+    "slsmi_window_attention_backward": (C.c_int, [C.POINTER(WindowShape)] + [C.POINTER(Heads)] * 5 + [_P, _P] +
+                                        [C.POINTER(Heads)] * 3 + [_P, C.c_size_t, _P]),
+    "slsmi_window_attention_backward_workspace_bytes": (C.c_size_t, [C.POINTER(WindowShape)]),
+    "slsmi_window_step": (C.c_int, [C.POINTER(WindowShape), C.c_int, _P, C.c_int64, _P, _P, _P, _P, _P, C.c_float, _P,
+                                    C.c_int, C.c_int, _P, _P, C.c_size_t, _P]),
+    "slsmi_window_step_workspace_bytes": (C.c_size_t, [C.POINTER(WindowShape), C.c_int]),
+    "slsmi_window_cache_fill": (C.c_int, [C.POINTER(WindowShape), C.c_int, C.POINTER(Heads), C.POINTER(Heads), _P, _P, _P,
+                                          _P]),
     "slsmi_audio_info": (C.c_int, [C.c_char_p, C.POINTER(C.c_int), C.POINTER(C.c_int), C.POINTER(C.c_int64)]),
     "slsmi_audio_read": (C.c_int, [C.c_char_p, _P, C.c_int64, C.POINTER(C.c_int64), C.POINTER(C.c_int)]),
     "slsmi_audio_resample": (C.c_int, [_P, C.c_int64, C.c_int, C.c_int, _P, C.c_int64, _P]),

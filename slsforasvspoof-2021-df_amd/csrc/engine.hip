@@ -1265,4 +1265,114 @@ int slsmi_topk_rows(float* enc, uint16_t* enc_bf16, int64_t rows, int dict, int 
     return hip_rc(launch_topk_rows(enc, enc_bf16, rows, dict, k, fmt, reinterpret_cast<hipStream_t>(stream)));
 }
 
+static QkNormParams qk_norm_params(const uint16_t* x, int64_t ldx, uint16_t* y, int64_t ldy, int64_t rows, int heads,
+                                   int kv_heads, int head_dim, const float* wq, const float* wk, float eps,
+                                   const double* freqs, int rotary_dim, int interleaved, const int64_t* positions,
+                                   int64_t npos, int fmt) {
+    QkNormParams p;
+    p.x = x; p.ldx = ldx; p.y = y; p.ldy = ldy; p.rows = rows; p.npos = npos > 0x7fffffffL ? 0 : (int)npos;
+    p.positions = reinterpret_cast<const long long*>(positions);
+    p.freqs = freqs; p.half = rotary_dim % 16 ? -1 : rotary_dim / 2; p.wq = wq; p.wk = wk;
+    p.Hq = heads; p.Hk = kv_heads; p.D = head_dim; p.interleaved = interleaved != 0; p.eps = eps; p.fmt = fmt;
+    return p;
+}
+
+int slsmi_qk_norm_rope(const uint16_t* x, int64_t ldx, uint16_t* y, int64_t ldy, int64_t rows, int heads, int kv_heads,
+                       int head_dim, const float* wq, const float* wk, float eps, const double* freqs, int rotary_dim,
+                       int interleaved, const int64_t* positions, int64_t npos, int fmt, void* stream) {
+    if (fmt != SLSMI_FMT_BF16 && fmt != SLSMI_FMT_F16) return SLSMI_ERR_INVALID;
+    return hip_rc(launch_qk_norm_rope(qk_norm_params(x, ldx, y, ldy, rows, heads, kv_heads, head_dim, wq, wk, eps, freqs,
+                                                     rotary_dim, interleaved, positions, npos, fmt),
+                                      reinterpret_cast<hipStream_t>(stream)));
+}
+
+size_t slsmi_qk_norm_rope_backward_workspace_bytes(int64_t rows, int head_dim) {
+    return rows >= 0 && (head_dim == 64 || head_dim == 128) ? qk_norm_rope_bwd_workspace(rows, head_dim) : 0;
+}
+
+int slsmi_qk_norm_rope_backward(const uint16_t* dy, int64_t lddy, const uint16_t* x, int64_t ldx, uint16_t* dx, int64_t lddx,
+                                int64_t rows, int heads, int kv_heads, int head_dim, const float* wq, const float* wk,
+                                float eps, const double* freqs, int rotary_dim, int interleaved, const int64_t* positions,
+                                int64_t npos, float* dwq, float* dwk, void* workspace, size_t workspace_bytes, int fmt,
+                                void* stream) {
+    if (fmt != SLSMI_FMT_BF16 && fmt != SLSMI_FMT_F16) return SLSMI_ERR_INVALID;
+    const size_t need = slsmi_qk_norm_rope_backward_workspace_bytes(rows, head_dim);
+    if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)) return SLSMI_ERR_WORKSPACE;
+    return hip_rc(launch_qk_norm_rope_bwd(qk_norm_params(x, ldx, dx, lddx, rows, heads, kv_heads, head_dim, wq, wk, eps, freqs,
+                                                         rotary_dim, interleaved, positions, npos, fmt),
+                                          dy, lddy, dwq, dwk, reinterpret_cast<float*>(workspace),
+                                          reinterpret_cast<hipStream_t>(stream)));
+}
+
+static WindowHeads window_heads(const slsmi_heads& h) { return {h.data, (long)h.batch, (long)h.row, (long)h.head}; }
+
+static WindowParams window_params(const slsmi_window_shape* w) {
+    WindowParams p;
+    p.B = w->batch; p.T = w->frames; p.Hq = w->heads; p.Hk = w->kv_heads; p.D = w->head_dim;
+    p.left = w->left; p.right = w->right; p.sinks = w->sinks; p.scale = w->scale; p.fmt = w->fmt;
+    return p;
+}
+
+int slsmi_window_attention(const slsmi_window_shape* shape, const slsmi_heads* q, const slsmi_heads* k, const slsmi_heads* v,
+                           const slsmi_heads* out, float* lse, const int32_t* nframes, void* stream) {
+    if (!shape || !q || !k || !v || !out) return SLSMI_ERR_INVALID;
+    WindowParams p = window_params(shape);
+    p.q = window_heads(*q); p.k = window_heads(*k); p.v = window_heads(*v); p.o = window_heads(*out);
+    p.nframes = nframes;
+    return hip_rc(launch_window_attention(p, lse, reinterpret_cast<hipStream_t>(stream)));
+}
+
+size_t slsmi_window_attention_backward_workspace_bytes(const slsmi_window_shape* shape) {
+    return shape ? window_attention_bwd_workspace(window_params(shape)) : 0;
+}
+
+int slsmi_window_attention_backward(const slsmi_window_shape* shape, const slsmi_heads* dout, const slsmi_heads* q,
+                                    const slsmi_heads* k, const slsmi_heads* v, const slsmi_heads* out, const float* lse,
+                                    const int32_t* nframes, const slsmi_heads* dq, const slsmi_heads* dk,
+                                    const slsmi_heads* dv, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!shape || !dout || !q || !k || !v || !out || !dq || !dk || !dv) return SLSMI_ERR_INVALID;
+    WindowParams p = window_params(shape);
+    const size_t need = window_attention_bwd_workspace(p);
+    if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)) return SLSMI_ERR_WORKSPACE;
+    p.q = window_heads(*q); p.k = window_heads(*k); p.v = window_heads(*v); p.o = window_heads(*out);
+    p.nframes = nframes;
+    return hip_rc(launch_window_attention_bwd(p, lse, window_heads(*dout), window_heads(*dq), window_heads(*dk),
+                                              window_heads(*dv), workspace, workspace_bytes,
+                                              reinterpret_cast<hipStream_t>(stream)));
+}
+
+static WindowStepParams step_params(const slsmi_window_shape* w, int slots) {
+    WindowStepParams p;
+    p.B = w->batch; p.Hq = w->heads; p.Hk = w->kv_heads; p.D = w->head_dim; p.slots = slots; p.sinks = w->sinks;
+    p.scale = w->scale; p.fmt = w->fmt;
+    return p;
+}
+
+size_t slsmi_window_step_workspace_bytes(const slsmi_window_shape* shape, int slots) {
+    return shape ? window_step_workspace(step_params(shape, slots)) : 0;
+}
+
+int slsmi_window_step(const slsmi_window_shape* shape, int slots, const uint16_t* qkv, int64_t ld, uint16_t* k_cache,
+                      uint16_t* v_cache, const int64_t* positions, const float* wq, const float* wk, float eps,
+                      const double* freqs, int rotary_dim, int interleaved, uint16_t* out, void* workspace,
+                      size_t workspace_bytes, void* stream) {
+    if (!shape) return SLSMI_ERR_INVALID;
+    WindowStepParams p = step_params(shape, slots);
+    const size_t need = window_step_workspace(p);
+    if (need && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < need)) return SLSMI_ERR_WORKSPACE;
+    p.qkv = qkv; p.ld = ld; p.k_cache = k_cache; p.v_cache = v_cache;
+    p.positions = reinterpret_cast<const long long*>(positions);
+    p.wq = wq; p.wk = wk; p.eps = eps; p.freqs = freqs; p.half = rotary_dim % 16 ? -1 : rotary_dim / 2;
+    p.interleaved = interleaved != 0; p.out = out;
+    return hip_rc(launch_window_step(p, workspace, workspace_bytes, reinterpret_cast<hipStream_t>(stream)));
+}
+
+int slsmi_window_cache_fill(const slsmi_window_shape* shape, int slots, const slsmi_heads* k, const slsmi_heads* v,
+                            uint16_t* k_cache, uint16_t* v_cache, const int32_t* nframes, void* stream) {
+    if (!shape || !k || !v) return SLSMI_ERR_INVALID;
+    return hip_rc(launch_window_fill(window_heads(*k), window_heads(*v), k_cache, v_cache, nframes, shape->batch, shape->frames,
+                                     shape->kv_heads, shape->head_dim, slots, shape->sinks,
+                                     reinterpret_cast<hipStream_t>(stream)));
+}
+
 }  // extern "C"

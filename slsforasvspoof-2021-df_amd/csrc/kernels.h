@@ -213,6 +213,65 @@ hipError_t launch_attention(const bf16_t* qkv, bf16_t* out, int B, int T, int fm
 hipError_t launch_attention_dropout(const bf16_t* qkv, bf16_t* out, int B, int T, int fmt, const uint8_t* keep, int pitch,
                                     float drop_scale, hipStream_t s);
 
+// Norms of queries and keys with the position rotation (qknorm.hip) ---------
+// rows of Hq + Hk heads of D (64 or 128) channels; y may be x.  Position of a row: positions[row % npos], or row % npos
+// where positions is null; freqs [half] radians per position (null with half 0: no rotation), half a multiple of 8.
+struct QkNormParams {
+    const bf16_t* x = nullptr;
+    long ldx = 0;
+    bf16_t* y = nullptr;      // forward: the result; backward: the gradient at x
+    long ldy = 0;
+    long rows = 0;
+    int npos = 1;
+    const long long* positions = nullptr;
+    const double* freqs = nullptr;
+    int half = 0;
+    const float* wq = nullptr;   // [D]
+    const float* wk = nullptr;
+    int Hq = 0, Hk = 0, D = 64, interleaved = 0, fmt = 0;
+    float eps = 0.f;
+};
+hipError_t launch_qk_norm_rope(const QkNormParams& p, hipStream_t s);
+size_t qk_norm_rope_bwd_workspace(long rows, int D);
+hipError_t launch_qk_norm_rope_bwd(const QkNormParams& p, const bf16_t* dy, long lddy, float* dwq, float* dwk, float* ws,
+                                   hipStream_t s);
+
+// Windowed attention (window.hip) and its single-frame form (window_step.hip) --
+struct WindowHeads {          // [B][T][heads][D] by element strides, D contiguous; 16-byte aligned
+    const bf16_t* p = nullptr;
+    long batch = 0, row = 0, head = 0;
+};
+struct WindowParams {
+    WindowHeads q, k, v, o;   // o: the forward's result
+    const int* nframes = nullptr;
+    int B = 0, T = 0, Hq = 1, Hk = 1, D = 64;
+    int left = -1, right = -1, sinks = 0;   // -1: no limit
+    int fmt = 0;
+    float scale = 1.f;
+};
+hipError_t launch_window_attention(const WindowParams& p, float* lse, hipStream_t s);
+size_t window_attention_bwd_workspace(const WindowParams& p);
+hipError_t launch_window_attention_bwd(const WindowParams& p, const float* lse, const WindowHeads& dout, const WindowHeads& dq,
+                                       const WindowHeads& dk, const WindowHeads& dv, void* ws, size_t ws_bytes, hipStream_t s);
+struct WindowStepParams {
+    const bf16_t* qkv = nullptr;
+    long ld = 0;
+    bf16_t* k_cache = nullptr;   // [B][Hk][slots][D]
+    bf16_t* v_cache = nullptr;
+    const long long* positions = nullptr;
+    bf16_t* out = nullptr;       // [B][Hq][D]
+    const float* wq = nullptr;   // null: no norm, no rotation
+    const float* wk = nullptr;
+    const double* freqs = nullptr;
+    int half = 0, interleaved = 0;
+    float eps = 0.f, scale = 1.f;
+    int B = 0, Hq = 1, Hk = 1, D = 64, slots = 1, sinks = 0, fmt = 0;
+};
+size_t window_step_workspace(const WindowStepParams& p);
+hipError_t launch_window_step(const WindowStepParams& p, void* ws, size_t ws_bytes, hipStream_t s);
+hipError_t launch_window_fill(const WindowHeads& k, const WindowHeads& v, bf16_t* kc, bf16_t* vc, const int* nframes, int B, int T,
+                              int Hk, int D, int slots, int sinks, hipStream_t s);
+
 // SLS head -----------------------------------------------------------------
 // w[l][b] = sigmoid(fc0_b + mean_t sum_s dots_l[s][b T + t]), l < layers, from the row dots of launch_gemm
 // (dot_out); dots_l = dots + l * layer_stride is [slices][B T]; w is [layers][B]

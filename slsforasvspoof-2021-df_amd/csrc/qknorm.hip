@@ -1,0 +1,291 @@
+// Norms of queries and keys for each head with the position rotation in the same pass, and their gradient.
+//
+// A row of qkv holds Hq query heads, Hk key heads (and whatever follows: the value heads), D channels each.  For a head x
+// with weight w at position p:
+//   r = 1 / sqrt(mean x^2 + eps),  n = r x w,  y = n with the pairs (n_i, n_j) of the first R channels turned by p f_i.
+// Backward, with dn = dy turned back:
+//   dw = sum over rows and heads of dn r x,   dx = r (dn w - x r^2 mean(dn w x)).
+// Both are bound by HBM (a row read and written once, backward two rows read and one written).  A wave takes a whole row:
+// its angles (64-bit, one per lane) are computed once and serve all heads, D / 8 lanes hold a head, a lane eight channels
+// (16 bytes), so the mean square is a three- or four-step sum inside a row of lanes and the other half of a pair one lane
+// exchange away.
+#include "kernels.h"
+#include "window.h"
+
+namespace slsmi {
+
+namespace {
+
+constexpr int QN_WAVES = 4;
+
+struct QkNormArgs {
+    const bf16_t* x;
+    long ldx;
+    bf16_t* y;
+    long ldy;
+    const bf16_t* dy;     // backward: gradient at y
+    long lddy;
+    float* partial;       // backward: [workgroups][2][D]
+    const long long* positions;
+    const double* freqs;
+    const float* wq;
+    const float* wk;
+    long rows;
+    int npos;             // positions (or frame numbers) repeat with this period over the rows
+    int half;             // R / 2
+    int Hq, Hk;
+    int heads_per_wave;   // a multiple of the heads a wave holds at once
+    int interleaved;
+    float eps;
+};
+
+__device__ __forceinline__ long long row_position(const QkNormArgs& a, long row) {
+    const unsigned i = (unsigned)row % (unsigned)a.npos;
+    return a.positions ? a.positions[i] : (long long)i;
+}
+
+template <int D>
+__device__ __forceinline__ void lane_weights(const QkNormArgs& a, int c, int pc, float (&wq)[8], float (&wk)[8],
+                                             float (&pwq)[8], float (&pwk)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        wq[e] = a.wq[c * 8 + e];
+        wk[e] = a.wk[c * 8 + e];
+        pwq[e] = a.wq[pc * 8 + e];
+        pwk[e] = a.wk[pc * 8 + e];
+    }
+}
+
+template <int FMT, int D>
+__global__ __launch_bounds__(QN_WAVES * 64) void qk_norm_rope_kernel(QkNormArgs a) {
+    constexpr int GL = D / 8, HW = 64 / GL;   // lanes per head, heads a wave holds at once
+    __shared__ float2 tab[QN_WAVES][64];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long row = (long)blockIdx.x * QN_WAVES + wave;
+    if (row >= a.rows) return;   // no barrier below
+    const int g = lane / GL, c = lane & (GL - 1);
+    const int H = a.Hq + a.Hk;
+    const int h0 = blockIdx.y * a.heads_per_wave, h1 = min(h0 + a.heads_per_wave, H);
+    const bf16_t* x = a.x + row * a.ldx + c * 8;
+    bf16_t* y = a.y + row * a.ldy + c * 8;
+    const NormLane t = norm_lane<D>(lane, row_position(a, row), a.freqs, a.half, a.interleaved, tab[wave]);
+    float wq[8], wk[8], pwq[8], pwk[8];
+    lane_weights<D>(a, c, t.partner & (GL - 1), wq, wk, pwq, pwk);
+    constexpr int U = 4;   // heads in flight per lane
+    for (int h = h0 + g; h - g < h1; h += U * HW) {
+        u16x8 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const u16x8*>(x + (long)min(h + u * HW, H - 1) * D);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int hh = h + u * HW;
+            const bool isq = hh < a.Hq;
+            float w[8], pw[8], o[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                w[e] = isq ? wq[e] : wk[e];
+                pw[e] = isq ? pwq[e] : pwk[e];
+            }
+            norm_rope_lane<FMT, D>(v[u], w, pw, t, a.eps, o);
+            if (hh < h1) {
+                u32x4 r;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) r[i] = Op<FMT>::pack2(o[2 * i], o[2 * i + 1]);
+                *reinterpret_cast<u32x4*>(y + (long)hh * D) = r;
+            }
+        }
+    }
+}
+
+// dx of a wave's rows; the weights' gradients stay in registers over the rows of a wave and leave as one partial sum per
+// workgroup (summed in workgroup order by the kernel below: the result does not depend on timing).
+template <int FMT, int D>
+__global__ __launch_bounds__(QN_WAVES * 64) void qk_norm_rope_bwd_kernel(QkNormArgs a) {
+    constexpr int GL = D / 8, HW = 64 / GL;
+    __shared__ float2 tab[QN_WAVES][64];
+    __shared__ float red[QN_WAVES][2][D];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int g = lane / GL, c = lane & (GL - 1);
+    const int H = a.Hq + a.Hk;
+    float gq[8], gk[8], wq[8], wk[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        gq[e] = gk[e] = 0.f;
+        wq[e] = a.wq[c * 8 + e];
+        wk[e] = a.wk[c * 8 + e];
+    }
+    for (long row = (long)blockIdx.x * QN_WAVES + wave; row < a.rows; row += (long)gridDim.x * QN_WAVES) {
+        const NormLane t = norm_lane<D>(lane, row_position(a, row), a.freqs, a.half, a.interleaved, tab[wave]);
+        const bf16_t* x = a.x + row * a.ldx + c * 8;
+        const bf16_t* dy = a.dy + row * a.lddy + c * 8;
+        bf16_t* y = a.y + row * a.ldy + c * 8;
+        constexpr int U = 2;
+        for (int h = g; h - g < H; h += U * HW) {
+            u16x8 xv[U], dv[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const long at = (long)min(h + u * HW, H - 1) * D;
+                xv[u] = *reinterpret_cast<const u16x8*>(x + at);
+                dv[u] = *reinterpret_cast<const u16x8*>(dy + at);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int hh = h + u * HW;
+                const bool isq = hh < a.Hq, live = hh < H;
+                const float r = head_rstd<FMT, D>(xv[u], a.eps);
+                const u16x8 pd = lane_exchange(dv[u], t.partner);
+                float dn[8], xh[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    dn[e] = Op<FMT>::unpack(dv[u][e]);
+                    xh[e] = Op<FMT>::unpack(xv[u][e]) * r;
+                }
+                if (t.role == 3) {
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        const float p = dn[e], q = dn[e + 1];
+                        dn[e] = p * t.cs[e] + q * t.sn[e];
+                        dn[e + 1] = q * t.cs[e] - p * t.sn[e];
+                    }
+                } else if (t.role != 0) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float o = Op<FMT>::unpack(pd[e]);
+                        dn[e] = t.role == 1 ? dn[e] * t.cs[e] + o * t.sn[e] : dn[e] * t.cs[e] - o * t.sn[e];
+                    }
+                }
+                float dot = 0.f, gn[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    gn[e] = dn[e] * (isq ? wq[e] : wk[e]);
+                    dot = fmaf(gn[e], xh[e], dot);
+                    const float dw = dn[e] * xh[e];
+                    gq[e] += live && isq ? dw : 0.f;
+                    gk[e] += live && !isq ? dw : 0.f;
+                }
+                dot = lane_group_sum<GL>(dot) * (1.0f / D);
+                if (live) {
+                    u32x4 o;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        o[i] = Op<FMT>::pack2(r * (gn[2 * i] - xh[2 * i] * dot), r * (gn[2 * i + 1] - xh[2 * i + 1] * dot));
+                    *reinterpret_cast<u32x4*>(y + (long)hh * D) = o;
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+#pragma unroll
+        for (int o = GL; o < 64; o <<= 1) {
+            gq[e] += __shfl_xor(gq[e], o, 64);
+            gk[e] += __shfl_xor(gk[e], o, 64);
+        }
+        if (lane < GL) {
+            red[wave][0][c * 8 + e] = gq[e];
+            red[wave][1][c * 8 + e] = gk[e];
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * D; i += QN_WAVES * 64) {
+        float s = 0.f;
+#pragma unroll
+        for (int w = 0; w < QN_WAVES; ++w) s += red[w][i / D][i % D];
+        a.partial[(long)blockIdx.x * 2 * D + i] = s;
+    }
+}
+
+// dwq, dwk [D] = sums of the partials [n][2][D] in a fixed order: 16 columns per workgroup, 16 rows of threads
+__global__ __launch_bounds__(256) void qk_norm_dw_kernel(const float* __restrict__ partial, int n, int D, float* __restrict__ dwq,
+                                                         float* __restrict__ dwk) {
+    __shared__ float red[16][17];
+    const int col = blockIdx.x * 16 + (threadIdx.x & 15), rg = threadIdx.x >> 4;
+    float s = 0.f;
+    for (int i = rg; i < n; i += 16) s += partial[(long)i * 2 * D + col];
+    red[rg][threadIdx.x & 15] = s;
+    __syncthreads();
+    if (rg == 0) {
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) t += red[i][threadIdx.x & 15];
+        (col < D ? dwq : dwk)[col < D ? col : col - D] = t;
+    }
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+bool qk_norm_ok(const QkNormParams& p) {
+    if (p.rows < 0 || p.rows > 0x7fffffffL || p.Hq < 0 || p.Hk < 0 || p.Hq + p.Hk < 1 || p.Hq + p.Hk > 4096) return false;
+    if (p.D != 64 && p.D != 128) return false;
+    if (p.half < 0 || 2 * p.half > p.D || p.half % 8 != 0 || (p.half > 0 && !p.freqs)) return false;
+    const long width = (long)(p.Hq + p.Hk) * p.D;
+    if (p.rows == 0) return true;
+    if (!p.x || !p.y || !p.wq || !p.wk || p.npos < 1) return false;
+    if (!aligned16(p.x) || !aligned16(p.y) || p.ldx % 8 != 0 || p.ldy % 8 != 0) return false;
+    return p.rows == 1 || (p.ldx >= width && p.ldy >= width);
+}
+
+QkNormArgs qk_norm_args(const QkNormParams& p) {
+    QkNormArgs a{};
+    a.x = p.x; a.ldx = p.ldx; a.y = p.y; a.ldy = p.ldy; a.rows = p.rows; a.npos = p.npos;
+    a.positions = p.positions; a.freqs = p.freqs; a.half = p.half; a.wq = p.wq; a.wk = p.wk;
+    a.Hq = p.Hq; a.Hk = p.Hk; a.interleaved = p.interleaved; a.eps = p.eps;
+    return a;
+}
+
+// workgroups of the backward: up to four per CU, so that a wave's partial sums cover several rows of a large batch
+int qk_norm_bwd_blocks(long rows) {
+    const long b = (rows + QN_WAVES - 1) / QN_WAVES;
+    return (int)(b < 1024 ? b : 1024);
+}
+
+}  // namespace
+
+hipError_t launch_qk_norm_rope(const QkNormParams& p, hipStream_t s) {
+    if (!qk_norm_ok(p)) return hipErrorInvalidValue;
+    if (p.rows == 0) return hipSuccess;
+    QkNormArgs a = qk_norm_args(p);
+    const int H = p.Hq + p.Hk, hw = 512 / p.D;
+    // few rows: the heads of a row go to several waves (until about eight waves per CU have work)
+    int seg = 1;
+    while (seg * p.rows < 2048 && seg * hw < H) seg *= 2;
+    a.heads_per_wave = ((H + seg - 1) / seg + hw - 1) / hw * hw;
+    seg = (H + a.heads_per_wave - 1) / a.heads_per_wave;
+    const dim3 grid((unsigned)((p.rows + QN_WAVES - 1) / QN_WAVES), seg);
+    SLSMI_FMT_DISPATCH(p.fmt, {
+        if (p.D == 64) hipLaunchKernelGGL((qk_norm_rope_kernel<F, 64>), grid, dim3(QN_WAVES * 64), 0, s, a);
+        else hipLaunchKernelGGL((qk_norm_rope_kernel<F, 128>), grid, dim3(QN_WAVES * 64), 0, s, a);
+    });
+    return hipGetLastError();
+}
+
+size_t qk_norm_rope_bwd_workspace(long rows, int D) {
+    return rows > 0 ? (size_t)qk_norm_bwd_blocks(rows) * 2 * D * sizeof(float) : 0;
+}
+
+hipError_t launch_qk_norm_rope_bwd(const QkNormParams& p, const bf16_t* dy, long lddy, float* dwq, float* dwk, float* ws,
+                                   hipStream_t s) {
+    if (!qk_norm_ok(p) || !dwq || !dwk) return hipErrorInvalidValue;
+    QkNormArgs a = qk_norm_args(p);
+    int nb = 0;
+    if (p.rows > 0) {
+        if (!dy || !aligned16(dy) || lddy % 8 != 0 || (p.rows > 1 && lddy < (long)(p.Hq + p.Hk) * p.D) || !ws || !aligned16(ws))
+            return hipErrorInvalidValue;
+        a.dy = dy;
+        a.lddy = lddy;
+        a.partial = ws;
+        nb = qk_norm_bwd_blocks(p.rows);
+        SLSMI_FMT_DISPATCH(p.fmt, {
+            if (p.D == 64) hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<F, 64>), dim3(nb), dim3(QN_WAVES * 64), 0, s, a);
+            else hipLaunchKernelGGL((qk_norm_rope_bwd_kernel<F, 128>), dim3(nb), dim3(QN_WAVES * 64), 0, s, a);
+        });
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    hipLaunchKernelGGL(qk_norm_dw_kernel, dim3(2 * p.D / 16), dim3(256), 0, s, ws, nb, p.D, dwq, dwk);
+    return hipGetLastError();
+}
+
+}  // namespace slsmi

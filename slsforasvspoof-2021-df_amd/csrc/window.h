@@ -1,0 +1,150 @@
+// Device helpers shared by the windowed-attention kernels (window.hip, window_step.hip) and the query / key norm kernels
+// (qknorm.hip).
+#pragma once
+#include "common.h"
+
+namespace slsmi {
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4_ptr;
+
+template <int FMT>
+__device__ __forceinline__ f32x16 mfma32(u16x8 a, u16x8 b, f32x16 c) {
+    if constexpr (FMT == FMT_BF16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Lane j's value <- lane j's value of a neighbour inside its row of 16 lanes (no LDS): after the sums over 2, 4, 8, 16
+// lanes below every lane of the group holds the group's total.
+template <int CTRL>
+__device__ __forceinline__ float dpp_move(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+// sum over aligned groups of N lanes (8 or 16), the same total in every lane
+template <int N>
+__device__ __forceinline__ float lane_group_sum(float v) {
+    v += dpp_move<0xB1>(v);    // quad_perm [1, 0, 3, 2]
+    v += dpp_move<0x4E>(v);    // quad_perm [2, 3, 0, 1]
+    v += dpp_move<0x141>(v);   // row_half_mirror: the other quad of eight
+    if constexpr (N == 16) v += dpp_move<0x140>(v);   // row_mirror: the other eight of sixteen
+    return v;
+}
+
+// Norm of one head and its position rotation (slsmi_qk_norm_rope), the part of one lane.  D / 8 consecutive lanes hold a
+// head, eight channels each (chunk c = lane within the head).  x: the lane's raw channels; w: their weights; px, pw: the
+// same of the lane that holds the other members of the pairs (chunk c +- R / 16; not read where pairs are neighbours);
+// cs: (cos, sin) of the eight channels' pairs.  role: 0 not rotated, 1 first halves, 2 second halves of split pairs,
+// 3 neighbouring pairs.
+struct NormLane {
+    float cs[8], sn[8];
+    int role;
+    int partner;   // lane (of the wave) that holds the other members
+};
+
+template <int FMT, int D>
+__device__ __forceinline__ float head_rstd(u16x8 x, float eps) {
+    float ss = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float f = Op<FMT>::unpack(x[e]);
+        ss = fmaf(f, f, ss);
+    }
+    ss = lane_group_sum<D / 8>(ss);
+    return 1.0f / sqrtf(fmaf(ss, 1.0f / D, eps));
+}
+
+__device__ __forceinline__ u16x8 lane_exchange(u16x8 x, int src) {
+    const u32x4 v = __builtin_bit_cast(u32x4, x);
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = (uint32_t)__builtin_amdgcn_ds_bpermute(src << 2, (int)v[i]);
+    return __builtin_bit_cast(u16x8, r);
+}
+
+template <int FMT, int D>
+__device__ __forceinline__ void norm_rope_lane(u16x8 x, const float* w, const float* pw, const NormLane& t, float eps,
+                                               float* y) {
+    const float r = head_rstd<FMT, D>(x, eps);
+    const u16x8 px = lane_exchange(x, t.partner);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = Op<FMT>::unpack(x[e]) * r * w[e];
+    if (t.role == 3) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            const float a = y[e], b = y[e + 1];
+            y[e] = a * t.cs[e] - b * t.sn[e];
+            y[e + 1] = b * t.cs[e] + a * t.sn[e];
+        }
+    } else if (t.role != 0) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float o = Op<FMT>::unpack(px[e]) * r * pw[e];
+            y[e] = t.role == 1 ? y[e] * t.cs[e] - o * t.sn[e] : y[e] * t.cs[e] + o * t.sn[e];
+        }
+    }
+}
+
+// cos and sin of position p times `freq` radians: whole turns are taken off in 64 bits (a position of 10^6 is 1.6e5
+// turns of the fastest pair; 32 bits would leave 2^-7 of a turn there), the rest is exact enough in 32.
+__device__ __forceinline__ void angle_cos_sin(long long p, double freq, float& c, float& s) {
+    const double turns = (double)p * freq * 0.15915494309189533577;
+    const float t = (float)(turns - rint(turns));
+    sincospif(2.0f * t, &s, &c);
+}
+
+// What a lane of the norm has to know beside its data: which channels its pairs are and their angles.  tab: wave-private
+// LDS of 64 (cos, sin) pairs, written here (half = R / 2 <= 64 pairs).
+template <int D>
+__device__ __forceinline__ NormLane norm_lane(int lane, long long p, const double* __restrict__ freqs, int half,
+                                              int interleaved, float2* tab) {
+    constexpr int GL = D / 8;
+    const int c = lane & (GL - 1);
+    NormLane t;
+    t.role = 0;
+    t.partner = lane;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        t.cs[e] = 1.f;
+        t.sn[e] = 0.f;
+    }
+    if (half <= 0) return t;
+    if (lane < half) {
+        float cc, ss;
+        angle_cos_sin(p, freqs[lane], cc, ss);
+        tab[lane] = float2{cc, ss};
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    const int hc = half >> 3;   // chunks of a half (half is a multiple of 8)
+    if (c < 2 * hc) {
+        if (interleaved) {
+            t.role = 3;
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const float2 v = tab[c * 4 + (e >> 1)];
+                t.cs[e] = v.x;
+                t.sn[e] = v.y;
+            }
+        } else {
+            const bool first = c < hc;
+            t.role = first ? 1 : 2;
+            t.partner = first ? lane + hc : lane - hc;
+            const int at = (first ? c : c - hc) * 8;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float2 v = tab[at + e];
+                t.cs[e] = v.x;
+                t.sn[e] = v.y;
+            }
+        }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    return t;
+}
+
+}  // namespace slsmi

@@ -459,3 +459,298 @@ def window_topk(acts: torch.Tensor, k: int, window: int, want_16bit: bool = Fals
                                    _lib.FORMATS["f16" if dtype == torch.float16 else "bf16"], _s(acts.device))
     _lib.check(rc, None, "slsmi_window_topk")
     return (out, o16) if want_16bit else out
+
+
+# ---- attention for recordings of any length and for live streams -----------------------------------------------------
+
+def _require(ok: bool, what: str) -> None:
+    if not ok:
+        raise _lib.SlsmiError(what)
+
+
+def _same_device(first: torch.Tensor, *rest: Optional[torch.Tensor]) -> None:
+    _need_cuda(first, *rest)
+    for t in rest:
+        _require(t is None or t.device == first.device, f"tensors on {first.device} and {t.device if t is not None else ''}")
+
+
+def _window_side(n: Optional[int], name: str) -> int:
+    if n is None:
+        return -1
+    _require(int(n) == n and n >= 0, f"{name}: frames (0 or more), or None for no limit; got {n}")
+    return min(int(n), 0x7fffffff)
+
+
+def _distinct(t: torch.Tensor) -> bool:
+    """No two elements of t share memory (sufficient: each dimension steps past all smaller ones)."""
+    reach = 1
+    for size, stride in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n > 1), key=lambda d: d[1]):
+        if stride < reach:
+            return False
+        reach = stride * (size - 1) + reach
+    return True
+
+
+def _heads_arg(t: torch.Tensor, name: str, shape, dtype: torch.dtype, written: bool = False) -> _lib.Heads:
+    """[batch, frames, heads, head_dim] by its strides; a view of packed rows is taken as it is."""
+    _require(tuple(t.shape) == tuple(shape), f"{name}: shape {tuple(shape)} expected, got {tuple(t.shape)}")
+    _require(t.dtype == dtype, f"{name}: {dtype} expected, got {t.dtype}")
+    st = [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
+    _require(t.numel() == 0 or (t.stride(3) == 1 and all(s % 8 == 0 for s in st[:3]) and t.data_ptr() % 16 == 0),
+             f"{name}: channels must be contiguous, strides multiples of 8 and the data 16-byte aligned; got strides "
+             f"{t.stride()}")
+    _require(t.numel() == 0 or ((st[1] >= shape[3] or shape[1] == 1) and (st[2] >= shape[3] or shape[2] == 1)),
+             f"{name}: rows and heads must be distinct (an expanded tensor?); got strides {t.stride()}")
+    _require(not written or _distinct(t), f"{name}: its elements share memory; got strides {t.stride()}")
+    return _lib.Heads(t.data_ptr(), st[0], st[1], st[2])
+
+
+def _window_shape(q: torch.Tensor, kv_heads: int, left, right, sinks: int, scale: Optional[float]) -> _lib.WindowShape:
+    B, T, H, D = q.shape
+    _require(D in (64, 128), f"head width 64 or 128 expected, got {D}")
+    _require(kv_heads >= 1 and H >= 1 and H % kv_heads == 0, f"{H} query heads cannot share {kv_heads} key heads")
+    _require(0 <= sinks <= 128, f"sinks: 0 to 128 first frames, got {sinks}")
+    scale = D ** -0.5 if scale is None else float(scale)
+    _require(0.0 < scale < float("inf"), f"scale must be positive, got {scale}")
+    return _lib.WindowShape(B, T, H, kv_heads, D, _window_side(left, "left"), _window_side(right, "right"), int(sinks), _fmt(q),
+                            scale)
+
+
+def _nframes_arg(nframes: Optional[torch.Tensor], B: int) -> Optional[torch.Tensor]:
+    if nframes is not None:
+        _require(nframes.dtype == torch.int32 and tuple(nframes.shape) == (B,) and nframes.is_contiguous(),
+                 f"nframes: int32 [{B}] expected, got {nframes.dtype} {tuple(nframes.shape)}")
+    return nframes
+
+
+def _rows_arg(t: torch.Tensor, name: str, width: int, dtype: torch.dtype, lead=None, written: bool = False):
+    """(rows, row stride) of [rows, >= width] or [batch, frames, >= width] whose rows lie at one distance."""
+    _require(t.dtype == dtype, f"{name}: {dtype} expected, got {t.dtype}")
+    _require(t.dim() in (2, 3) and t.shape[-1] >= width, f"{name}: rows of at least {width} values expected, got {tuple(t.shape)}")
+    _require(lead is None or t.shape[:-1] == lead, f"{name}: leading shape {lead} expected, got {tuple(t.shape[:-1])}")
+    rows = t.numel() // t.shape[-1]
+    if rows == 0:
+        return 0, t.shape[-1]
+    ld = t.stride(-2) if t.shape[-2] > 1 else (t.stride(0) if t.dim() == 3 and t.shape[0] > 1 else t.shape[-1])
+    _require(t.dim() == 2 or t.shape[0] == 1 or t.shape[1] == 1 or t.stride(0) == t.shape[1] * t.stride(1),
+             f"{name}: all rows must lie at one distance; got strides {t.stride()}")
+    if rows == 1:
+        ld = (width + 7) // 8 * 8
+    _require(t.stride(-1) == 1 and ld % 8 == 0 and ld >= width and t.data_ptr() % 16 == 0,
+             f"{name}: contiguous channels, a row stride that is a multiple of 8 and 16-byte alignment needed; got strides "
+             f"{t.stride()}")
+    return rows, ld
+
+
+def _norm_args(x: torch.Tensor, q_weight, k_weight, freqs, positions, lead):
+    D = q_weight.numel()
+    _require(D in (64, 128), f"head width 64 or 128 expected, got {D} norm weights")
+    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        _require(w.dtype == torch.float32 and tuple(w.shape) == (D,) and w.is_contiguous(),
+                 f"{name}: contiguous float32 [{D}] expected, got {w.dtype} {tuple(w.shape)}")
+    R = 0
+    if freqs is not None:
+        _require(freqs.dtype == torch.float64 and freqs.dim() == 1 and freqs.is_contiguous(),
+                 f"freqs: contiguous float64 [rotary_dim / 2] expected, got {freqs.dtype} {tuple(freqs.shape)}")
+        R = 2 * freqs.numel()
+        _require(R % 16 == 0 and R <= D, f"the rotated width must be a multiple of 16 up to {D}, got {R}")
+    rows = 1
+    for n in lead:
+        rows *= n
+    T = lead[-1]
+    npos = max(1, T)
+    if positions is not None:
+        _require(positions.dtype == torch.int64 and positions.is_contiguous() and
+                 (tuple(positions.shape) == tuple(lead) or tuple(positions.shape) == (T,)),
+                 f"positions: contiguous int64 {tuple(lead)} or {(T,)} expected, got {positions.dtype} {tuple(positions.shape)}")
+        npos = max(1, positions.numel())
+    _same_device(x, q_weight, k_weight, freqs, positions)
+    return D, R, rows, npos
+
+
+def qk_norm_rope(qkv: torch.Tensor, heads: int, kv_heads: int, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                 freqs: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                 interleaved: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Root-mean-square norms of query and key heads and their rotation by position in one pass (slsmi_qk_norm_rope).
+
+    qkv [rows, width] or [batch, frames, width], 16 bits: heads query heads, kv_heads key heads of D = q_weight.numel()
+    channels, then anything (the value heads).  q_weight, k_weight fp32 [D].  freqs float64 [R / 2] radians per position
+    (None: no rotation): pairs (i, i + R / 2), or neighbours with interleaved.  positions int64, one per row or one per
+    frame; None counts frames (or rows) from 0.  Returns [..., (heads + kv_heads) * D]; out (may be qkv itself) receives
+    the heads in its first columns instead, the rest of its rows is left alone."""
+    _need_cuda(qkv, out)
+    lead = qkv.shape[:-1]
+    D, R, rows, npos = _norm_args(qkv, q_weight, k_weight, freqs, positions, lead)
+    _require(heads >= 0 and kv_heads >= 0 and heads + kv_heads >= 1, f"{heads} query and {kv_heads} key heads")
+    width = (heads + kv_heads) * D
+    fmt = _fmt(qkv)
+    _, ldx = _rows_arg(qkv, "qkv", width, qkv.dtype)
+    if out is None:
+        out = torch.empty(*lead, width, dtype=qkv.dtype, device=qkv.device)
+    _same_device(qkv, out)
+    _, ldy = _rows_arg(out, "out", width, qkv.dtype, lead)
+    with torch.cuda.device(qkv.device):
+        rc = _lib.load().slsmi_qk_norm_rope(_p(qkv), ldx, _p(out), ldy, rows, heads, kv_heads, D, _p(q_weight), _p(k_weight),
+                                            float(eps), _p(freqs), R, int(interleaved), _p(positions), npos, fmt,
+                                            _s(qkv.device))
+    _lib.check(rc, None, "slsmi_qk_norm_rope")
+    return out
+
+
+def qk_norm_rope_backward(dout: torch.Tensor, qkv: torch.Tensor, heads: int, kv_heads: int, q_weight: torch.Tensor,
+                          k_weight: torch.Tensor, freqs: Optional[torch.Tensor] = None,
+                          positions: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False,
+                          out: Optional[torch.Tensor] = None):
+    """Gradient of qk_norm_rope: dout at its result, qkv as it was given -> (dqkv [..., (heads + kv_heads) * D],
+    dq_weight, dk_weight).  out: where dqkv goes (dout itself, or the packed gradient whose value columns
+    window_attention_backward wrote)."""
+    _need_cuda(dout, qkv, out)
+    lead = qkv.shape[:-1]
+    D, R, rows, npos = _norm_args(qkv, q_weight, k_weight, freqs, positions, lead)
+    _require(heads >= 0 and kv_heads >= 0 and heads + kv_heads >= 1, f"{heads} query and {kv_heads} key heads")
+    width = (heads + kv_heads) * D
+    fmt = _fmt(qkv)
+    _, ldx = _rows_arg(qkv, "qkv", width, qkv.dtype)
+    _, lddy = _rows_arg(dout, "dout", width, qkv.dtype, lead)
+    if out is None:
+        out = torch.empty(*lead, width, dtype=qkv.dtype, device=qkv.device)
+    _same_device(qkv, dout, out)
+    _, lddx = _rows_arg(out, "out", width, qkv.dtype, lead)
+    dwq, dwk = torch.empty_like(q_weight), torch.empty_like(k_weight)
+    lib = _lib.load()
+    n = lib.slsmi_qk_norm_rope_backward_workspace_bytes(rows, D)
+    ws = torch.empty(n, dtype=torch.uint8, device=qkv.device)
+    with torch.cuda.device(qkv.device):
+        rc = lib.slsmi_qk_norm_rope_backward(_p(dout), lddy, _p(qkv), ldx, _p(out), lddx, rows, heads, kv_heads, D, _p(q_weight),
+                                             _p(k_weight), float(eps), _p(freqs), R, int(interleaved), _p(positions), npos,
+                                             _p(dwq), _p(dwk), _p(ws), n, fmt, _s(qkv.device))
+    _lib.check(rc, None, "slsmi_qk_norm_rope_backward")
+    return out, dwq, dwk
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: Optional[int], right: Optional[int] = 0,
+                     sinks: int = 0, nframes: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                     return_lse: bool = False, out: Optional[torch.Tensor] = None):
+    """Attention with a sliding window over recordings of any length (slsmi_window_attention).
+
+    q [batch, frames, heads, D], k, v [batch, frames, kv_heads, D], 16 bits, D 64 or 128, any strides with contiguous
+    channels (views of packed rows).  Query i sees key j where j <= i + right and (j >= i - left or j < sinks), up to its
+    recording's nframes (int32 [batch] on the device; None: all).  None for left or right: no limit.  scale: 1 / sqrt(D)
+    unless given.  Returns [batch, frames, heads, D], zeros at padded frames; with return_lse also the rows'
+    log-sum-exp, fp32 [batch, heads, frames], for window_attention_backward."""
+    _same_device(q, k, v, nframes, out)
+    _require(q.dim() == 4 and k.dim() == 4, f"q, k, v [batch, frames, heads, D] expected, got {tuple(q.shape)}, {tuple(k.shape)}")
+    B, T, H, D = q.shape
+    shape = _window_shape(q, k.shape[2], left, right, sinks, scale)
+    kv = (B, T, k.shape[2], D)
+    out = torch.empty(B, T, H, D, dtype=q.dtype, device=q.device) if out is None else out
+    args = [_heads_arg(q, "q", q.shape, q.dtype), _heads_arg(k, "k", kv, q.dtype), _heads_arg(v, "v", kv, q.dtype),
+            _heads_arg(out, "out", q.shape, q.dtype, written=True)]
+    lse = torch.empty(B, H, T, dtype=torch.float32, device=q.device) if return_lse else None
+    with torch.cuda.device(q.device):
+        rc = _lib.load().slsmi_window_attention(C.byref(shape), *(C.byref(x) for x in args), _p(lse),
+                                                _p(_nframes_arg(nframes, B)), _s(q.device))
+    _lib.check(rc, None, "slsmi_window_attention")
+    return (out, lse) if return_lse else out
+
+
+def window_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                              lse: torch.Tensor, left: Optional[int], right: Optional[int] = 0, sinks: int = 0,
+                              nframes: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                              dq: Optional[torch.Tensor] = None, dk: Optional[torch.Tensor] = None,
+                              dv: Optional[torch.Tensor] = None):
+    """Gradient of window_attention at q, k, v from its out and lse, the other arguments as given to it
+    (slsmi_window_attention_backward).  dq, dk, dv: where the gradients go (views of packed rows, say); new tensors unless
+    given.  Gradients at padded frames are zeros.  Returns (dq, dk, dv)."""
+    _same_device(q, dout, k, v, out, lse, nframes, dq, dk, dv)
+    _require(q.dim() == 4 and k.dim() == 4, f"q, k, v [batch, frames, heads, D] expected, got {tuple(q.shape)}, {tuple(k.shape)}")
+    B, T, H, D = q.shape
+    shape = _window_shape(q, k.shape[2], left, right, sinks, scale)
+    kv = (B, T, k.shape[2], D)
+    _require(lse.dtype == torch.float32 and tuple(lse.shape) == (B, H, T) and lse.is_contiguous(),
+             f"lse: contiguous float32 {(B, H, T)} expected, got {lse.dtype} {tuple(lse.shape)}")
+    dq = torch.empty(B, T, H, D, dtype=q.dtype, device=q.device) if dq is None else dq
+    dk = torch.empty(kv, dtype=q.dtype, device=q.device) if dk is None else dk
+    dv = torch.empty(kv, dtype=q.dtype, device=q.device) if dv is None else dv
+    ins = [_heads_arg(t, n, s, q.dtype) for t, n, s in ((dout, "dout", q.shape), (q, "q", q.shape), (k, "k", kv), (v, "v", kv),
+                                                       (out, "out", q.shape))]
+    outs = [_heads_arg(t, n, s, q.dtype, written=True) for t, n, s in ((dq, "dq", q.shape), (dk, "dk", kv), (dv, "dv", kv))]
+    lib = _lib.load()
+    n = lib.slsmi_window_attention_backward_workspace_bytes(C.byref(shape))
+    ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+    with torch.cuda.device(q.device):
+        rc = lib.slsmi_window_attention_backward(C.byref(shape), *(C.byref(x) for x in ins), _p(lse),
+                                                 _p(_nframes_arg(nframes, B)), *(C.byref(x) for x in outs), _p(ws), n,
+                                                 _s(q.device))
+    _lib.check(rc, None, "slsmi_window_attention_backward")
+    return dq, dk, dv
+
+
+def _cache_args(k_cache: torch.Tensor, v_cache: torch.Tensor, sinks: int):
+    _require(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.dtype == v_cache.dtype and
+             k_cache.is_contiguous() and v_cache.is_contiguous(),
+             f"k_cache, v_cache: contiguous [batch, kv_heads, slots, D] of one type expected, got {tuple(k_cache.shape)}, "
+             f"{tuple(v_cache.shape)}")
+    slots = k_cache.shape[2]
+    _require(0 <= sinks < slots <= 1 << 24, f"sinks + window slots (window at least 1, at most 2^24 in all) expected, got {slots} "
+             f"slots for {sinks} sinks")
+    return slots
+
+
+def window_cache_fill(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, sinks: int,
+                      nframes: Optional[torch.Tensor] = None) -> None:
+    """Prefill of a rolling cache (slsmi_window_cache_fill): the keys and values [batch, frames, kv_heads, D] of
+    recordings that begin at position 0 go to the slots their first `sinks` and their last (slots - sinks) frames live in.
+    k_cache, v_cache [batch, kv_heads, slots, D]."""
+    _same_device(k, v, k_cache, v_cache, nframes)
+    slots = _cache_args(k_cache, v_cache, sinks)
+    _require(k.dim() == 4, f"k, v [batch, frames, kv_heads, D] expected, got {tuple(k.shape)}")
+    B, T, H, D = k.shape
+    _require(tuple(k_cache.shape) == (B, H, slots, D) and D in (64, 128) and H >= 1,
+             f"a cache {(B, H, slots, D)} with D 64 or 128 expected, got {tuple(k_cache.shape)}")
+    _require(k_cache.dtype == k.dtype, f"cache of {k_cache.dtype}, keys of {k.dtype}")
+    shape = _lib.WindowShape(B, T, H, H, D, -1, 0, int(sinks), _fmt(k), 1.0)
+    args = [_heads_arg(k, "k", k.shape, k.dtype), _heads_arg(v, "v", k.shape, k.dtype)]
+    with torch.cuda.device(k.device):
+        rc = _lib.load().slsmi_window_cache_fill(C.byref(shape), slots, C.byref(args[0]), C.byref(args[1]), _p(k_cache),
+                                                 _p(v_cache), _p(_nframes_arg(nframes, B)), _s(k.device))
+    _lib.check(rc, None, "slsmi_window_cache_fill")
+
+
+def window_attention_step(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, positions: torch.Tensor, heads: int,
+                          sinks: int, q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                          freqs: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False,
+                          scale: Optional[float] = None) -> torch.Tensor:
+    """One new frame per live stream (slsmi_window_step): qkv [batch, (heads + 2 kv_heads) * D], the frame's query, key
+    and value heads; positions int64 [batch] on the device, its position in each stream (negative: this stream has no
+    frame now).  The key and value go to the rolling cache k_cache, v_cache [batch, kv_heads, slots, D] and the result
+    [batch, heads, D] is what window_attention(left=slots - sinks - 1, right=0, sinks=sinks) gives for that frame.  With
+    q_weight and k_weight the norms and the rotation of qk_norm_rope happen inside.  The caller advances positions."""
+    _same_device(qkv, k_cache, v_cache, positions, q_weight, k_weight, freqs)
+    slots = _cache_args(k_cache, v_cache, sinks)
+    B, Hk, _, D = k_cache.shape
+    _require(D in (64, 128), f"head width 64 or 128 expected, got {D}")
+    _require(Hk >= 1 and heads >= 1 and heads % Hk == 0, f"{heads} query heads cannot share {Hk} key heads")
+    _require(qkv.dim() == 2 and tuple(qkv.shape) == (B, (heads + 2 * Hk) * D) and qkv.dtype == k_cache.dtype,
+             f"qkv: {k_cache.dtype} {(B, (heads + 2 * Hk) * D)} expected, got {qkv.dtype} {tuple(qkv.shape)}")
+    _require(positions.dtype == torch.int64 and tuple(positions.shape) == (B,) and positions.is_contiguous(),
+             f"positions: contiguous int64 [{B}] expected, got {positions.dtype} {tuple(positions.shape)}")
+    _require((q_weight is None) == (k_weight is None) and (q_weight is not None or freqs is None),
+             "the rotation needs both norm weights")
+    R = 0
+    if q_weight is not None:
+        n, R, _, _ = _norm_args(qkv, q_weight, k_weight, freqs, None, qkv.shape[:-1])
+        _require(n == D, f"norm weights of {D} channels expected, got {n}")
+    scale = D ** -0.5 if scale is None else float(scale)
+    _require(0.0 < scale < float("inf"), f"scale must be positive, got {scale}")
+    _, ld = _rows_arg(qkv, "qkv", qkv.shape[1], qkv.dtype)
+    shape = _lib.WindowShape(B, 1, heads, Hk, D, -1, 0, int(sinks), _fmt(qkv), scale)
+    out = torch.empty(B, heads, D, dtype=qkv.dtype, device=qkv.device)
+    lib = _lib.load()
+    n = lib.slsmi_window_step_workspace_bytes(C.byref(shape), slots)
+    ws = torch.empty(n, dtype=torch.uint8, device=qkv.device) if n else None
+    with torch.cuda.device(qkv.device):
+        rc = lib.slsmi_window_step(C.byref(shape), slots, _p(qkv), ld, _p(k_cache), _p(v_cache), _p(positions), _p(q_weight),
+                                   _p(k_weight), float(eps), _p(freqs), R, int(interleaved), _p(out), _p(ws), n, _s(qkv.device))
+    _lib.check(rc, None, "slsmi_window_step")
+    return out
