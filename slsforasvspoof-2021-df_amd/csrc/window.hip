@@ -21,6 +21,10 @@ namespace {
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float LN2 = 0.6931471805599453f;
 
+// Waves per SIMD the kernels are built for: the most that registers allow without spilling (128 / 168 / 256 per wave).
+constexpr int fwd_waves(int D) { return D == 64 ? 4 : 3; }
+constexpr int bwd_waves(int D) { return D == 64 ? 3 : 2; }
+
 struct HeadPtr {
     const bf16_t* p;
     long b, r, h;   // element strides of batch, row, head
@@ -45,55 +49,85 @@ struct WinArgs {
 };
 
 constexpr int SINK_MAX = 128;
+constexpr long ROW_MAX = 1L << 23;   // row stride: 64 rows of a tile are reached by 32-bit offsets
+
+// rows of a staged tile: 8 KiB either way, so that the two buffers of two tiles of several workgroups fit a CU
+constexpr int tile_rows(int D) { return D == 64 ? 64 : 32; }
 
 // LDS image of a tile of rows of D 16-bit values, without padding: 16-byte chunks of a row permuted by its row number so
 // that 16 consecutive rows read at one chunk (ds_read_b128 of the row operand) and four consecutive rows read at four
-// neighbouring chunks (ds_read_b64_tr_b16 of the transposed operand) both touch every bank once.
+// neighbouring chunks (ds_read_b64_tr_b16 of the transposed operand) both touch every bank once (no conflict cycles
+// measured).  The permutation repeats every 16 rows.
+template <int D>
+__device__ __forceinline__ int chunk_turn(int row) {
+    return D == 64 ? (((row >> 1) & 1) << 2) | ((row >> 2) & 3) : ((row & 3) << 2) | ((row >> 2) & 3);
+}
 template <int D>
 __device__ __forceinline__ int tile_at(int row, int chunk) {
-    if constexpr (D == 64) return row * 128 + ((chunk ^ ((((row >> 1) & 1) << 2) | ((row >> 2) & 3))) << 4);
-    else return row * 256 + ((chunk ^ (((row & 3) << 2) | ((row >> 2) & 3))) << 4);
+    return row * D * 2 + ((chunk ^ chunk_turn<D>(row)) << 4);
 }
 
+// Byte offsets inside a tile of what a lane reads: the row operand of rows 0 .. 31 per 16 columns, and the transposed
+// operand (rows as columns' neighbours) of rows 0 .. 15 per 32 columns; other rows of a tile lie a constant further.
 template <int D>
-__device__ __forceinline__ u16x8 row_frag(const char* tile, int row, int chunk) {
-    return *reinterpret_cast<const u16x8*>(tile + tile_at<D>(row, chunk));
-}
-
-// A operand of the transposed product for column block dt (32 columns) and the 16 rows row0 ..: rows enumerated as above
-template <int D>
-__device__ __forceinline__ u16x8 tr_frag(const char* tile, int row0, int dt, int lane) {
-    const int row = row0 + ((lane >> 5) << 2) + ((lane & 15) >> 2);
-    const int col = dt * 32 + (lane & 16) + (lane & 3) * 4;
-    const int in = (col & 4) * 2;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(tile + tile_at<D>(row, col >> 3) + in));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(tile + tile_at<D>(row + 8, col >> 3) + in));
-    return __builtin_bit_cast(u16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-}
-
-// Rows row0 .. row0 + ROWS - 1 of a head on their way to LDS: requested early, written when the tile before is used up.
-// Rows at or past `len` become zeros (what lies there may be anything, NaN among it).
-template <int D, int ROWS>
-struct Stage {
-    static constexpr int CH = D / 8;
-    static constexpr int N = ROWS * CH / 256;
-    u16x8 v[N];
-    __device__ __forceinline__ void load(const bf16_t* head, long rs, int row0, int len, int tid) {
+struct LaneAt {
+    int row[D / 16], tr[D / 32][2];
+    __device__ __forceinline__ explicit LaneAt(int lane) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = tid + i * 256, row = row0 + c / CH;
-            v[i] = *reinterpret_cast<const u16x8*>(head + (long)min(row, len - 1) * rs + (c & (CH - 1)) * 8);
-            if (row >= len) v[i] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
-        }
-    }
-    __device__ __forceinline__ void store(char* tile, int tid) const {
+        for (int e = 0; e < D / 16; ++e) row[e] = tile_at<D>(lane & 31, 2 * e + (lane >> 5));
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int c = tid + i * 256;
-            *reinterpret_cast<u16x8*>(tile + tile_at<D>(c / CH, c & (CH - 1))) = v[i];
+        for (int dt = 0; dt < D / 32; ++dt) {
+            const int r = ((lane >> 5) << 2) + ((lane & 15) >> 2), c = dt * 32 + (lane & 16) + (lane & 3) * 4;
+            tr[dt][0] = tile_at<D>(r, c >> 3) + (c & 4) * 2;
+            tr[dt][1] = tile_at<D>(r + 8, c >> 3) + (c & 4) * 2;
         }
     }
 };
+
+template <int D>
+__device__ __forceinline__ u16x8 row_frag(const char* tile, int row0, const LaneAt<D>& at, int e) {
+    return *reinterpret_cast<const u16x8*>(tile + row0 * D * 2 + at.row[e]);
+}
+// A operand of the transposed product for column block dt (32 columns) and the 16 rows row0 ..: rows enumerated as above
+template <int D>
+__device__ __forceinline__ u16x8 tr_frag(const char* tile, int row0, const LaneAt<D>& at, int dt) {
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(tile + row0 * D * 2 + at.tr[dt][0]));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(tile + row0 * D * 2 + at.tr[dt][1]));
+    return __builtin_bit_cast(u16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+typedef __attribute__((address_space(3))) void* lds_ptr;
+
+// Rows row0 .. row0 + ROWS - 1 of a head straight into an LDS tile (16 bytes per lane; a wave fills 1 KiB pieces; the
+// permutation is applied to the source addresses).  The buffer descriptor ends behind row len - 1: later rows arrive as
+// zeros, whatever lies there.  The caller waits (vmcnt) and synchronizes before the tile is read.
+template <int D, int ROWS>
+struct TileLoad {
+    static constexpr int CH = D / 8, PER = 64 / CH, N = ROWS / PER / 4;   // chunks of a row, rows of a piece, pieces of a wave
+    int off[N];
+    __device__ __forceinline__ TileLoad(long rs, int lane, int wave) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int row = (wave + 4 * i) * PER + lane / CH;
+            off[i] = row * (int)rs * 2 + (((lane & (CH - 1)) ^ chunk_turn<D>(row)) << 4);
+        }
+    }
+    __device__ __forceinline__ void issue(const bf16_t* head, long rs, int row0, int len, char* tile, int wave) const {
+#ifdef __HIP_DEVICE_COMPILE__   // (the descriptor type does not exist in the host pass)
+        const int rows = min(max(len - row0, 0), ROWS);
+        const int bytes = rows > 0 ? (rows - 1) * (int)rs * 2 + D * 2 : 0;
+        const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)(head + (long)row0 * rs), 0, bytes, 0x00027000);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(tile + (wave + 4 * i) * 1024), 16, off[i], 0, 0, 0);
+#endif
+    }
+};
+// every load of this wave has landed, and every wave's has
+__device__ __forceinline__ void tiles_landed() {
+    __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0)
+    __syncthreads();
+}
 
 // Workgroup number -> (batch x head, tile): consecutive workgroups go to the 8 XCDs in turn, and each XCD gets a
 // contiguous share of the work, so that the tiles of a head -- which read the same keys -- meet in one L2.
@@ -102,14 +136,14 @@ __device__ __forceinline__ unsigned xcd_order(unsigned n, unsigned total) {
     return x * q + (x < r ? x : r) + i;
 }
 
-// Whether the 32 keys k0 .. and the 32 queries q0 .. have visible pairs, and whether all pairs are.
+// Whether the 32 keys k0 .. and the nq queries q0 .. have visible pairs, and whether all pairs are.
 struct Vis {
     bool any, all;
 };
-__device__ __forceinline__ Vis block_visibility(int q0, int k0, int len, int left, int right, int sinks) {
+__device__ __forceinline__ Vis block_visibility(int q0, int nq, int k0, int len, int left, int right, int sinks) {
     Vis r;
-    r.any = k0 < len && q0 < len && k0 <= q0 + 31 + right && (k0 + 31 >= q0 - left || k0 < sinks);
-    r.all = k0 + 31 < len && k0 + 31 <= q0 + right && (k0 >= q0 + 31 - left || k0 + 31 < sinks);
+    r.any = k0 < len && q0 < len && k0 <= q0 + nq - 1 + right && (k0 + 31 >= q0 - left || k0 < sinks);
+    r.all = k0 + 31 < len && k0 + 31 <= q0 + right && (k0 >= q0 + nq - 1 - left || k0 + 31 < sinks);
     return r;
 }
 
@@ -159,17 +193,54 @@ __device__ __forceinline__ u16x8 pack_step_unit(const f32x16& p, int s) {
 __device__ __forceinline__ f32x16 zero16() {
     return f32x16{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 }
-__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
+// one value of each half of the wave (lane i and lane i ^ 32), the same pair in both
+__device__ __forceinline__ f32x2 both_halves(float v) {
+    const uint32_t x = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return f32x2{__builtin_bit_cast(float, (uint32_t)r[0]), __builtin_bit_cast(float, (uint32_t)r[1])};
+}
+__device__ __forceinline__ float halves_sum(float v) {
+    const f32x2 p = both_halves(v);
+    return p[0] + p[1];
+}
 
 __device__ __forceinline__ int frames_of(const WinArgs& a, int b) { return a.nframes ? min(max(a.nframes[b], 0), a.T) : a.T; }
 
-// ---- forward: 128 queries per workgroup, 32 per wave; 64-key tiles
+// Bounds of a query's keys relative to itself, for the masked blocks: key - q in [-left, right] and below len.
+struct KeyRange {
+    int left;
+    unsigned span;   // left + min(right, len - 1 - q)
+    __device__ __forceinline__ KeyRange(int q, int len, int l, int right) : left(l), span((unsigned)(l + min(right, len - 1 - q))) {}
+    __device__ __forceinline__ bool has(int rel) const { return (unsigned)(rel + left) <= span; }
+};
+
+// Scores of the 32 keys kb' .. of one lane's query that it does not see become -inf.  kb: key of register 0 of this lane.
+__device__ __forceinline__ void hide_keys(f32x16& s, int k0, int kb, int q, int len, int left, int right, int sinks) {
+    const KeyRange in(q, len, left, right);
+    if (k0 < sinks) {
+        const int last = min(min(sinks, len) - 1, q + right);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int key = kb + 8 * (r >> 2) + (r & 3);
+            s[r] = (in.has(key - q) | (key <= last)) ? s[r] : -INFINITY;
+        }
+    } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = in.has(kb - q + 8 * (r >> 2) + (r & 3)) ? s[r] : -INFINITY;
+    }
+}
+
+// ---- forward: 128 queries per workgroup, 32 per wave; key tiles in two LDS buffers (one barrier per tile).
+//
+// The running maximum `m` of a query is only a reference for the exponent: it is moved (and the sums rescaled) when a
+// tile's scores pass it by more than 2^RISE, so almost never after the first tile; probabilities stay below 2^RISE times
+// the row's largest, well inside both formats.
+constexpr float RISE = 8.f;
+
 template <int FMT, int D>
-__global__ __launch_bounds__(256) void window_fwd_kernel(WinArgs a) {
-    constexpr int BN = 64, NS = D / 16, DT = D / 32;
-    __shared__ __attribute__((aligned(16))) char lds[2 * BN * D * 2];
-    char* const Ks = lds;
-    char* const Vs = lds + BN * D * 2;
+__global__ __launch_bounds__(256, fwd_waves(D)) void window_fwd_kernel(WinArgs a) {
+    constexpr int BN = tile_rows(D), NS = D / 16, DT = D / 32, TILE = BN * D * 2;
+    extern __shared__ __attribute__((aligned(16))) char lds[];   // two buffers of a K and a V tile
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, hi = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const unsigned w = xcd_order(blockIdx.x, gridDim.x);
@@ -189,101 +260,91 @@ __global__ __launch_bounds__(256) void window_fwd_kernel(WinArgs a) {
     }
     const bf16_t* kh = a.k.p + b * a.k.b + hk * a.k.h;
     const bf16_t* vh = a.v.p + b * a.v.b + hk * a.v.h;
+    const KeyTiles kt = key_tiles(q0, min(q0 + 127, len - 1), len, a.left, a.right, a.sinks, BN);
+    const LaneAt<D> at(lane);
+    const TileLoad<D, BN> lk(a.k.r, lane, wave), lv(a.v.r, lane, wave);
+    lk.issue(kh, a.k.r, kt.tile(0) * BN, len, lds, wave);
+    lv.issue(vh, a.v.r, kt.tile(0) * BN, len, lds + TILE, wave);
     u16x8 qf[NS];
     {
         const bf16_t* qr = a.q.p + b * a.q.b + h * a.q.h + (long)min(q, len - 1) * a.q.r + hi * 8;
 #pragma unroll
         for (int s = 0; s < NS; ++s) qf[s] = *reinterpret_cast<const u16x8*>(qr + s * 16);
     }
-    const KeyTiles kt = key_tiles(q0, min(q0 + 127, len - 1), len, a.left, a.right, a.sinks, BN);
     const float sc = a.scale * LOG2E;
     float m = -INFINITY, l = 0.f;
     f32x16 o[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] = zero16();
-    Stage<D, BN> sk, sv;
-    sk.load(kh, a.k.r, kt.tile(0) * BN, len, tid);
-    sv.load(vh, a.v.r, kt.tile(0) * BN, len, tid);
+    tiles_landed();
     for (int it = 0; it < kt.n; ++it) {
         const int k0 = kt.tile(it) * BN;
-        __syncthreads();
-        sk.store(Ks, tid);
-        sv.store(Vs, tid);
-        __syncthreads();
-        if (it + 1 < kt.n) {
-            sk.load(kh, a.k.r, kt.tile(it + 1) * BN, len, tid);
-            sv.load(vh, a.v.r, kt.tile(it + 1) * BN, len, tid);
+        char* const Ks = lds + (it & 1) * 2 * TILE;
+        char* const Vs = Ks + TILE;
+        const bool more = it + 1 < kt.n;
+        if (more) {
+            char* const next = lds + ((it + 1) & 1) * 2 * TILE;
+            lk.issue(kh, a.k.r, kt.tile(it + 1) * BN, len, next, wave);
+            lv.issue(vh, a.v.r, kt.tile(it + 1) * BN, len, next + TILE, wave);
         }
-        Vis vis[2];
-        f32x16 s[2];
-        float mx = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            vis[u] = block_visibility(qw, k0 + 32 * u, len, a.left, a.right, a.sinks);
-            if (!vis[u].any) continue;
-            s[u] = zero16();
+        for (int u = 0; u < BN / 32; ++u) {
+            const int kb = k0 + 32 * u;
+            const Vis vis = block_visibility(qw, 32, kb, len, a.left, a.right, a.sinks);
+            if (!vis.any) continue;
+            f32x16 s = zero16();
 #pragma unroll
-            for (int e = 0; e < NS; ++e) s[u] = mfma32<FMT>(row_frag<D>(Ks, 32 * u + col, 2 * e + hi), qf[e], s[u]);
-            if (!vis[u].all) {
+            for (int e = 0; e < NS; ++e) s = mfma32<FMT>(row_frag<D>(Ks, 32 * u, at, e), qf[e], s);
+            if (!vis.all) hide_keys(s, kb, kb + 4 * hi, q, len, a.left, a.right, a.sinks);
+            float mx = s[0];
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int key = k0 + 32 * u + 8 * (r >> 2) + 4 * hi + (r & 3);
-                    const bool ok = key < len && key <= q + a.right && (key >= q - a.left || key < a.sinks);
-                    s[u][r] = ok ? s[u][r] : -INFINITY;
-                }
+            for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+            const f32x2 two = both_halves(mx);
+            mx = fmaxf(two[0], two[1]) * sc;
+            if (__builtin_amdgcn_ballot_w64(mx > m + RISE) != 0) {   // (m starts at -inf)
+                const float mn = fmaxf(m, mx);
+                const float corr = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+                m = mn;
+                l *= corr;
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) o[dt] *= corr;
             }
-#pragma unroll
-            for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[u][r]);
-        }
-        if (!vis[0].any && !vis[1].any) continue;
-        mx = fmaxf(mx, other_half(mx)) * sc;
-        const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.f : mn;
-        const float corr = __builtin_amdgcn_exp2f(m - ref);
-        m = mn;
-        float sum = 0.f;
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            if (!vis[u].any) continue;
+            const float ref = m == -INFINITY ? 0.f : m;
+            float sum = 0.f;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], sc, -ref));
-                sum += s[u][r];
+                s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], sc, -ref));
+                sum += s[r];
             }
-        }
-        l = l * corr + sum;
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) o[dt] *= corr;
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            if (!vis[u].any) continue;
+            l += sum;
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
-                const u16x8 p = pack_step_unit<FMT>(s[u], st);
+                const u16x8 p = pack_step_unit<FMT>(s, st);
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) o[dt] = mfma32<FMT>(tr_frag<D>(Vs, 32 * u + 16 * st, dt, lane), p, o[dt]);
+                for (int dt = 0; dt < DT; ++dt) o[dt] = mfma32<FMT>(tr_frag<D>(Vs, 32 * u + 16 * st, at, dt), p, o[dt]);
             }
         }
+        if (more) tiles_landed();
     }
-    l += other_half(l);
+    l = halves_sum(l);
     const bool live = q < len;
     const float inv = live ? 1.0f / l : 0.f;
     if (q < a.T) {
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-            f32x16 v = live ? o[dt] * inv : zero16();
+            const f32x16 v = live ? o[dt] * inv : zero16();
             store_column<FMT, true>(orow, dt, v, hi);
         }
         if (lse && hi == 0) *lse = live ? (m + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
     }
 }
 
-// ---- backward, queries: dQ and delta = rowsum(dO o O); the forward's loop with P recomputed from lse
+// ---- backward, queries: dQ and delta = rowsum(dO o O); the forward's loop with P recomputed from lse.  The product
+// dO V^T starts from -delta, so dP - delta leaves the matrix units.
 template <int FMT, int D>
-__global__ __launch_bounds__(256) void window_dq_kernel(WinArgs a) {
-    constexpr int BN = 64, NS = D / 16, DT = D / 32;
-    __shared__ __attribute__((aligned(16))) char lds[2 * BN * D * 2];
-    char* const Ks = lds;
-    char* const Vs = lds + BN * D * 2;
+__global__ __launch_bounds__(256, bwd_waves(D)) void window_dq_kernel(WinArgs a) {
+    constexpr int BN = tile_rows(D), NS = D / 16, DT = D / 32, TILE = BN * D * 2;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, hi = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const unsigned w = xcd_order(blockIdx.x, gridDim.x);
@@ -297,12 +358,16 @@ __global__ __launch_bounds__(256) void window_dq_kernel(WinArgs a) {
         if (q < a.T) {
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) store_column<FMT, true>(dqrow, dt, zero16(), hi);
-            if (hi == 0) *drow = 0.f;
         }
         return;
     }
     const bf16_t* kh = a.k.p + b * a.k.b + hk * a.k.h;
     const bf16_t* vh = a.v.p + b * a.v.b + hk * a.v.h;
+    const KeyTiles kt = key_tiles(q0, min(q0 + 127, len - 1), len, a.left, a.right, a.sinks, BN);
+    const LaneAt<D> at(lane);
+    const TileLoad<D, BN> lk(a.k.r, lane, wave), lv(a.v.r, lane, wave);
+    lk.issue(kh, a.k.r, kt.tile(0) * BN, len, lds, wave);
+    lv.issue(vh, a.v.r, kt.tile(0) * BN, len, lds + TILE, wave);
     u16x8 qf[NS], df[NS];
     float delta = 0.f;
     {
@@ -318,53 +383,50 @@ __global__ __launch_bounds__(256) void window_dq_kernel(WinArgs a) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) delta = fmaf(Op<FMT>::unpack(df[s][e]), Op<FMT>::unpack(of[e]), delta);
         }
-        delta += other_half(delta);
+        delta = halves_sum(delta);
     }
     const bool live = q < len;
-    if (q < a.T && hi == 0) *drow = live ? delta : 0.f;
+    if (live && hi == 0) *drow = delta;
     const float sc = a.scale * LOG2E;
     const float ls = a.lse[(long)bh * a.T + min(q, len - 1)] * LOG2E;
-    const KeyTiles kt = key_tiles(q0, min(q0 + 127, len - 1), len, a.left, a.right, a.sinks, BN);
-    f32x16 acc[DT];
+    f32x16 acc[DT], start;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt] = zero16();
-    Stage<D, BN> sk, sv;
-    sk.load(kh, a.k.r, kt.tile(0) * BN, len, tid);
-    sv.load(vh, a.v.r, kt.tile(0) * BN, len, tid);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) start[r] = -delta;
+    tiles_landed();
     for (int it = 0; it < kt.n; ++it) {
         const int k0 = kt.tile(it) * BN;
-        __syncthreads();
-        sk.store(Ks, tid);
-        sv.store(Vs, tid);
-        __syncthreads();
-        if (it + 1 < kt.n) {
-            sk.load(kh, a.k.r, kt.tile(it + 1) * BN, len, tid);
-            sv.load(vh, a.v.r, kt.tile(it + 1) * BN, len, tid);
+        char* const Ks = lds + (it & 1) * 2 * TILE;
+        char* const Vs = Ks + TILE;
+        const bool more = it + 1 < kt.n;
+        if (more) {
+            char* const next = lds + ((it + 1) & 1) * 2 * TILE;
+            lk.issue(kh, a.k.r, kt.tile(it + 1) * BN, len, next, wave);
+            lv.issue(vh, a.v.r, kt.tile(it + 1) * BN, len, next + TILE, wave);
         }
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const Vis vis = block_visibility(qw, k0 + 32 * u, len, a.left, a.right, a.sinks);
+        for (int u = 0; u < BN / 32; ++u) {
+            const int kb = k0 + 32 * u;
+            const Vis vis = block_visibility(qw, 32, kb, len, a.left, a.right, a.sinks);
             if (!vis.any) continue;
-            f32x16 s = zero16(), dp = zero16();
+            f32x16 s = zero16(), dp = start;
 #pragma unroll
             for (int e = 0; e < NS; ++e) {
-                s = mfma32<FMT>(row_frag<D>(Ks, 32 * u + col, 2 * e + hi), qf[e], s);
-                dp = mfma32<FMT>(row_frag<D>(Vs, 32 * u + col, 2 * e + hi), df[e], dp);
+                s = mfma32<FMT>(row_frag<D>(Ks, 32 * u, at, e), qf[e], s);
+                dp = mfma32<FMT>(row_frag<D>(Vs, 32 * u, at, e), df[e], dp);
             }
+            if (!vis.all) hide_keys(s, kb, kb + 4 * hi, q, len, a.left, a.right, a.sinks);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(s[r], sc, -ls));
-                const int key = k0 + 32 * u + 8 * (r >> 2) + 4 * hi + (r & 3);
-                const bool ok = vis.all || (key < len && key <= q + a.right && (key >= q - a.left || key < a.sinks));
-                s[r] = ok ? p * (dp[r] - delta) : 0.f;
-            }
+            for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], sc, -ls)) * dp[r];
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
                 const u16x8 e = pack_step<FMT>(s, st);
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) acc[dt] = mfma32<FMT>(tr_frag<D>(Ks, 32 * u + 16 * st, dt, lane), e, acc[dt]);
+                for (int dt = 0; dt < DT; ++dt) acc[dt] = mfma32<FMT>(tr_frag<D>(Ks, 32 * u + 16 * st, at, dt), e, acc[dt]);
             }
         }
+        if (more) tiles_landed();
     }
     if (q < a.T) {
 #pragma unroll
@@ -377,19 +439,17 @@ __global__ __launch_bounds__(256) void window_dq_kernel(WinArgs a) {
 
 // ---- backward, keys: dK and dV.  A workgroup owns 128 keys (32 per wave) and goes through the 64-query tiles of every
 // query head of the group that see them; S = Q K^T this time (queries on the row index), so P and dS are the B operands
-// of dV^T = dO^T P and dK^T = Q^T dS.
+// of dV^T = dO^T P and dK^T = Q^T dS.  The products start from -lse / scale and -delta of their rows (LDS), which also
+// takes rows out: a row with lse = +inf has P = 0.
 //
 // The sinks' keys are seen by every later query: the queries past the near ones of a sink block (32 keys) are cut into
 // chunks of far_chunk, one workgroup each, whose four waves share the block's keys and take 32 of 128 queries in turn.
 // Those sums, and the near workgroup's for sink rows, go as fp32 to `part` [B][Hk][sink block][1 + 4 far_blocks][dK, dV]
 // [32 keys][D] and are added in that order by window_sink_kernel.
 template <int FMT, int D>
-__global__ __launch_bounds__(256, 1) void window_dkv_kernel(WinArgs a) {
-    constexpr int NS = D / 16, DT = D / 32, BQ = 128;
-    __shared__ __attribute__((aligned(16))) char lds[2 * BQ * D * 2];
-    __shared__ __attribute__((aligned(16))) float st_l[BQ], st_d[BQ];
-    char* const Qs = lds;
-    char* const Ds = lds + BQ * D * 2;
+__global__ __launch_bounds__(256, bwd_waves(D)) void window_dkv_kernel(WinArgs a) {
+    constexpr int NS = D / 16, DT = D / 32, BQ = tile_rows(D), TILE = BQ * D * 2, BUF = 2 * TILE + 2 * BQ * 4;
+    extern __shared__ __attribute__((aligned(16))) char lds[];   // two buffers of Q, dO, -lse / scale, -delta
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, hi = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int sink_blocks = (a.sinks + 31) / 32;
@@ -405,7 +465,7 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(WinArgs a) {
         const int k0 = item * 128;
         k0w = k0 + wave * 32;
         qa = max(k0 - a.right, 0);
-        qb = min(k0 + 127 + a.left, len - 1);
+        qb = k0 < len ? min(k0 + 127 + a.left, len - 1) : -1;
     } else {
         block = (item - a.tiles) / a.far_blocks;
         chunk = (item - a.tiles) % a.far_blocks;
@@ -430,71 +490,92 @@ __global__ __launch_bounds__(256, 1) void window_dkv_kernel(WinArgs a) {
     f32x16 ak[DT], av[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) ak[dt] = av[dt] = zero16();
-    const float sc = a.scale * LOG2E;
-    const int t0 = qa / BQ, nt = (!far && item * 128 >= len) || qb < qa ? 0 : qb / BQ - t0 + 1;
+    const float sc = a.scale * LOG2E, lsc = 1.0f / a.scale;
+    const int t0 = qa / BQ, nt = qb < qa ? 0 : qb / BQ - t0 + 1;
     const int total = nt * grp;
-    Stage<D, BQ> sq, sd;
-    float l1 = 0.f, d1 = 0.f;
-    auto request = [&](int it) {
-        const int h = hk * grp + it / nt, q0 = (t0 + it % nt) * BQ;
-        sq.load(a.q.p + b * a.q.b + h * a.q.h, a.q.r, q0, len, tid);
-        sd.load(a.d.p + b * a.d.b + h * a.d.h, a.d.r, q0, len, tid);
-        if (tid < BQ) {
-            const long at = ((long)b * a.Hq + h) * a.T + min(q0 + tid, len - 1);
-            l1 = a.lse[at] * LOG2E;
-            d1 = a.delta[at];
+    const LaneAt<D> at(lane);
+    const TileLoad<D, BQ> lq(a.q.r, lane, wave), ld(a.d.r, lane, wave);
+    float stat = 0.f;   // thread t: -lse / scale of row t of the tile for t < BQ, then -delta of row t - BQ
+    int rt = t0, rh = hk * grp;   // tile and head of the next request
+    auto request = [&](char* buf) {
+        const int q0 = rt * BQ;
+        lq.issue(a.q.p + b * a.q.b + rh * a.q.h, a.q.r, q0, len, buf, wave);
+        ld.issue(a.d.p + b * a.d.b + rh * a.d.h, a.d.r, q0, len, buf + TILE, wave);
+        if (tid < 2 * BQ) {
+            const int q = q0 + (tid & (BQ - 1));
+            const long at = ((long)b * a.Hq + rh) * a.T + min(q, len - 1);
+            const bool in = q >= qa && q <= qb;
+            stat = tid < BQ ? (in ? -a.lse[at] * lsc : -INFINITY) : (in ? -a.delta[at] : 0.f);
+        }
+        if (++rt == t0 + nt) {
+            rt = t0;
+            ++rh;
         }
     };
-    if (total > 0) request(0);
+    auto landed = [&](char* buf) {
+        if (tid < 2 * BQ) reinterpret_cast<float*>(buf + 2 * TILE)[tid] = stat;
+        tiles_landed();
+    };
+    if (total > 0) {
+        request(lds);
+        landed(lds);
+    }
+    int qt = t0;
     for (int it = 0; it < total; ++it) {
-        const int q0 = (t0 + it % nt) * BQ;
-        __syncthreads();
-        sq.store(Qs, tid);
-        sd.store(Ds, tid);
-        if (tid < BQ) {
-            st_l[tid] = l1;
-            st_d[tid] = d1;
-        }
-        __syncthreads();
-        if (it + 1 < total) request(it + 1);
-#pragma unroll 1
-        for (int u = 0; u < BQ / 32; ++u) {
-            if (far && u != wave) continue;
-            const int qs = q0 + 32 * u;
-            Vis vis = block_visibility(qs, k0w, len, a.left, a.right, a.sinks);
-            if (qs > qb || qs + 31 < qa) vis.any = false;
-            if (!vis.any) continue;
-            const bool whole = vis.all && qs + 31 < len && qs >= qa && qs + 31 <= qb;
-            f32x16 s = zero16(), dp = zero16();
+        const int q0 = qt * BQ;
+        char* const Qs = lds + (it & 1) * BUF;
+        char* const Ds = Qs + TILE;
+        const float* const st_l = reinterpret_cast<const float*>(Qs + 2 * TILE) + 4 * hi;
+        const float* const st_d = st_l + BQ;
+        const bool more = it + 1 < total;
+        char* const next = lds + ((it + 1) & 1) * BUF;
+        if (more) request(next);
+        if (++qt == t0 + nt) qt = t0;
 #pragma unroll
-            for (int e = 0; e < NS; ++e) {
-                s = mfma32<FMT>(row_frag<D>(Qs, 32 * u + col, 2 * e + hi), kf[e], s);
-                dp = mfma32<FMT>(row_frag<D>(Ds, 32 * u + col, 2 * e + hi), vf[e], dp);
-            }
+        for (int u = 0; u < BQ / 32; ++u) {
+            if (far && (BQ == 64 ? 2 * (it & 1) + u : it & 3) != wave) continue;
+            const int qs = q0 + 32 * u;
+            const Vis vis = block_visibility(qs, 32, k0w, len, a.left, a.right, a.sinks);
+            if (!vis.any) continue;
+            f32x16 s, dp;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const f32x4 l4 = *reinterpret_cast<const f32x4*>(st_l + 32 * u + 8 * g + 4 * hi);
-                const f32x4 d4 = *reinterpret_cast<const f32x4*>(st_d + 32 * u + 8 * g + 4 * hi);
+                const f32x4 l4 = *reinterpret_cast<const f32x4*>(st_l + 32 * u + 8 * g);
+                const f32x4 d4 = *reinterpret_cast<const f32x4*>(st_d + 32 * u + 8 * g);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int r = 4 * g + j, q = qs + 8 * g + 4 * hi + j;
-                    const bool ok = whole || (q >= qa && q <= qb && key < len && key <= q + a.right &&
-                                              (key >= q - a.left || key < a.sinks));
-                    const float p = ok ? __builtin_amdgcn_exp2f(fmaf(s[r], sc, -l4[j])) : 0.f;
-                    s[r] = p;
-                    dp[r] = ok ? p * (dp[r] - d4[j]) : 0.f;
+                    s[4 * g + j] = l4[j];
+                    dp[4 * g + j] = d4[j];
                 }
+            }
+#pragma unroll
+            for (int e = 0; e < NS; ++e) {
+                s = mfma32<FMT>(row_frag<D>(Qs, 32 * u, at, e), kf[e], s);
+                dp = mfma32<FMT>(row_frag<D>(Ds, 32 * u, at, e), vf[e], dp);
+            }
+            if (!vis.all) {
+                // q - key of register r is base + 8 (r / 4) + r % 4: seen from -right to left, and any later query by a sink
+                const int base = qs + 4 * hi - key;
+                const unsigned span = (unsigned)(a.right + (key < a.sinks ? 2 * a.T : a.left));
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = (unsigned)(base + 8 * (r >> 2) + (r & 3) + a.right) <= span ? s[r] : -INFINITY;
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[r] = __builtin_amdgcn_exp2f(s[r] * sc);
+                dp[r] *= s[r];
             }
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
                 const u16x8 pf = pack_step_unit<FMT>(s, st), ef = pack_step<FMT>(dp, st);
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
-                    av[dt] = mfma32<FMT>(tr_frag<D>(Ds, 32 * u + 16 * st, dt, lane), pf, av[dt]);
-                    ak[dt] = mfma32<FMT>(tr_frag<D>(Qs, 32 * u + 16 * st, dt, lane), ef, ak[dt]);
+                    av[dt] = mfma32<FMT>(tr_frag<D>(Ds, 32 * u + 16 * st, at, dt), pf, av[dt]);
+                    ak[dt] = mfma32<FMT>(tr_frag<D>(Qs, 32 * u + 16 * st, at, dt), ef, ak[dt]);
                 }
             }
         }
+        if (more) landed(next);
     }
     if (far || (k0w < a.sinks && a.far_blocks > 0)) {
         const int blk = far ? block : k0w / 32, slot = far ? 1 + chunk * 4 + wave : 0;
@@ -558,7 +639,7 @@ int far_blocks_of(int T, int left, int sinks) {
 
 bool head_ok(const WindowHeads& x, int heads, int T, int D) {
     if (!x.p || ((uintptr_t)x.p & 15) || x.batch % 8 || x.row % 8 || x.head % 8) return false;
-    if (x.batch < 0 || x.row < 0 || x.head < 0 || x.row > (1L << 31) || x.head > (1L << 40) || x.batch > (1L << 50)) return false;
+    if (x.batch < 0 || x.row < 0 || x.head < 0 || x.row > ROW_MAX || x.head > (1L << 40) || x.batch > (1L << 50)) return false;
     // rows and heads are distinct pieces of D values
     if (T > 1 && x.row < D) return false;
     if (heads > 1 && x.head < D) return false;
@@ -589,6 +670,34 @@ size_t delta_bytes(const WinArgs& a) { return ((size_t)a.B * a.Hq * a.T * sizeof
 
 }  // namespace
 
+// launches a kernel whose LDS size may pass the default limit of a launch
+template <typename K>
+hipError_t launch_lds(K* kernel, LdsAttrState& attr, unsigned blocks, int lds, const WinArgs& a, hipStream_t s) {
+    const hipError_t e = ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), lds, attr);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), lds, s, a);
+    return hipGetLastError();
+}
+
+template <int FMT, int D>
+hipError_t launch_fwd(const WinArgs& a, hipStream_t s) {
+    static LdsAttrState attr;
+    return launch_lds(&window_fwd_kernel<FMT, D>, attr, (unsigned)(a.B * a.Hq * a.tiles), 4 * 8192, a, s);
+}
+
+template <int FMT, int D>
+hipError_t launch_bwd(const WinArgs& a, hipStream_t s) {
+    static LdsAttrState at_q, at_k;
+    const int sb = (a.sinks + 31) / 32;
+    hipError_t e = launch_lds(&window_dq_kernel<FMT, D>, at_q, (unsigned)(a.B * a.Hq * a.tiles), 4 * 8192, a, s);
+    if (e != hipSuccess) return e;
+    e = launch_lds(&window_dkv_kernel<FMT, D>, at_k, (unsigned)(a.B * a.Hk * (a.tiles + sb * a.far_blocks)), 2 * (2 * 8192 + 2 * tile_rows(D) * 4),
+                   a, s);
+    if (e != hipSuccess || a.far_blocks == 0) return e;
+    hipLaunchKernelGGL((window_sink_kernel<FMT, D>), dim3(a.B * a.Hk * sb * 4), dim3(256), 0, s, a);
+    return hipGetLastError();
+}
+
 hipError_t launch_window_attention(const WindowParams& p, float* lse, hipStream_t s) {
     WinArgs a{};
     if (!window_args(p, a)) return hipErrorInvalidValue;
@@ -598,12 +707,9 @@ hipError_t launch_window_attention(const WindowParams& p, float* lse, hipStream_
         return hipErrorInvalidValue;
     a.q = in_head(p.q); a.k = in_head(p.k); a.v = in_head(p.v); a.out = out_head(p.o);
     a.lse = lse;
-    const dim3 grid((unsigned)(p.B * p.Hq * a.tiles));
-    SLSMI_FMT_DISPATCH(p.fmt, {
-        if (p.D == 64) hipLaunchKernelGGL((window_fwd_kernel<F, 64>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((window_fwd_kernel<F, 128>), grid, dim3(256), 0, s, a);
-    });
-    return hipGetLastError();
+    hipError_t rc = hipSuccess;
+    SLSMI_FMT_DISPATCH(p.fmt, rc = p.D == 64 ? (launch_fwd<F, 64>(a, s)) : (launch_fwd<F, 128>(a, s)));
+    return rc;
 }
 
 size_t window_attention_bwd_workspace(const WindowParams& p) {
@@ -630,22 +736,9 @@ hipError_t launch_window_attention_bwd(const WindowParams& p, const float* lse, 
     a.part = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + delta_bytes(a));
     a.far_chunk = FAR_CHUNK;
     a.far_blocks = far_blocks_of(p.T, a.left, a.sinks);
-    const int sb = (a.sinks + 31) / 32;
-    const dim3 gq((unsigned)(p.B * p.Hq * a.tiles)), gk((unsigned)(p.B * p.Hk * (a.tiles + sb * a.far_blocks)));
-    SLSMI_FMT_DISPATCH(p.fmt, {
-        if (p.D == 64) {
-            hipLaunchKernelGGL((window_dq_kernel<F, 64>), gq, dim3(256), 0, s, a);
-            hipLaunchKernelGGL((window_dkv_kernel<F, 64>), gk, dim3(256), 0, s, a);
-        } else {
-            hipLaunchKernelGGL((window_dq_kernel<F, 128>), gq, dim3(256), 0, s, a);
-            hipLaunchKernelGGL((window_dkv_kernel<F, 128>), gk, dim3(256), 0, s, a);
-        }
-        if (a.far_blocks > 0) {
-            if (p.D == 64) hipLaunchKernelGGL((window_sink_kernel<F, 64>), dim3(p.B * p.Hk * sb * 4), dim3(256), 0, s, a);
-            else hipLaunchKernelGGL((window_sink_kernel<F, 128>), dim3(p.B * p.Hk * sb * 4), dim3(256), 0, s, a);
-        }
-    });
-    return hipGetLastError();
+    hipError_t rc = hipSuccess;
+    SLSMI_FMT_DISPATCH(p.fmt, rc = p.D == 64 ? (launch_bwd<F, 64>(a, s)) : (launch_bwd<F, 128>(a, s)));
+    return rc;
 }
 
 }  // namespace slsmi
