@@ -141,14 +141,14 @@ SIGNATURES = {
                                               C.c_int, _P, _P, C.c_float, _P, C.c_int, C.c_int, _P, C.c_int64, _P, _P, _P,
                                               C.c_size_t, C.c_int, _P]),
     "slsmi_qk_norm_rope_backward_workspace_bytes": (C.c_size_t, [C.c_int64, C.c_int]),
-    "slsmi_window_attention": (C.c_int, [C.POINTER(WindowShape)] + [C.POINTER(Heads)] * 4 + [_P, _P, _P]),
-    "slsmi_window_attention_backward": (C.c_int, [C.POINTER(WindowShape)] + [C.POINTER(Heads)] * 5 + [_P, _P] +
-                                        [C.POINTER(Heads)] * 3 + [_P, C.c_size_t, _P]),
-    "slsmi_window_attention_backward_workspace_bytes": (C.c_size_t, [C.POINTER(WindowShape)]),
-    "slsmi_window_step": (C.c_int, [C.POINTER(WindowShape), C.c_int, _P, C.c_int64, _P, _P, _P, _P, _P, C.c_float, _P,
+    "slsmi_window_attention": (C.c_int, [_P] + [_P] * 4 + [_P, _P, _P]),
+    "slsmi_window_attention_backward": (C.c_int, [_P] + [_P] * 5 + [_P, _P] +
+                                        [_P] * 3 + [_P, C.c_size_t, _P]),
+    "slsmi_window_attention_backward_workspace_bytes": (C.c_size_t, [_P]),
+    "slsmi_window_step": (C.c_int, [_P, C.c_int, _P, C.c_int64, _P, _P, _P, _P, _P, C.c_float, _P,
                                     C.c_int, C.c_int, _P, _P, C.c_size_t, _P]),
-    "slsmi_window_step_workspace_bytes": (C.c_size_t, [C.POINTER(WindowShape), C.c_int]),
-    "slsmi_window_cache_fill": (C.c_int, [C.POINTER(WindowShape), C.c_int, C.POINTER(Heads), C.POINTER(Heads), _P, _P, _P,
+    "slsmi_window_step_workspace_bytes": (C.c_size_t, [_P, C.c_int]),
+    "slsmi_window_cache_fill": (C.c_int, [_P, C.c_int, _P, _P, _P, _P, _P,
                                           _P]),
     "slsmi_audio_info": (C.c_int, [C.c_char_p, C.POINTER(C.c_int), C.POINTER(C.c_int), C.POINTER(C.c_int64)]),
     "slsmi_audio_read": (C.c_int, [C.c_char_p, _P, C.c_int64, C.POINTER(C.c_int64), C.POINTER(C.c_int)]),

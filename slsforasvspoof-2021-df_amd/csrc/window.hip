@@ -14,6 +14,8 @@
 #include "kernels.h"
 #include "window.h"
 
+#include <type_traits>
+
 namespace slsmi {
 
 namespace {
@@ -88,12 +90,57 @@ template <int D>
 __device__ __forceinline__ u16x8 row_frag(const char* tile, int row0, const LaneAt<D>& at, int e) {
     return *reinterpret_cast<const u16x8*>(tile + row0 * D * 2 + at.row[e]);
 }
-// A operand of the transposed product for column block dt (32 columns) and the 16 rows row0 ..: rows enumerated as above
-template <int D>
-__device__ __forceinline__ u16x8 tr_frag(const char* tile, int row0, const LaneAt<D>& at, int dt) {
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(tile + row0 * D * 2 + at.tr[dt][0]));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(tile + row0 * D * 2 + at.tr[dt][1]));
+__device__ __forceinline__ uint32_t lds_offset(const char* p) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
+}
+__device__ __forceinline__ u16x8 tr_pair(s16x4 lo, s16x4 hi) {
     return __builtin_bit_cast(u16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// A operands of a transposed product for all column blocks (32 columns each) of the 16 rows that lie `OFF` bytes past
+// `tile`, rows enumerated as above.  The transposed read's builtin makes the compiler wait for every load into LDS that is
+// under way (the next tile's), so the reads are written out, with their wait in the same block.
+template <int D, int OFF>
+__device__ __forceinline__ void tr_frags(uint32_t tile, const LaneAt<D>& at, u16x8 (&f)[D / 32]) {
+#pragma unroll
+    for (int d = 0; d < D / 32; d += 2) {
+        s16x4 r0, r1, r2, r3;
+        asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%8\n\t"
+                     "ds_read_b64_tr_b16 %1, %5 offset:%8\n\t"
+                     "ds_read_b64_tr_b16 %2, %6 offset:%8\n\t"
+                     "ds_read_b64_tr_b16 %3, %7 offset:%8\n\t"
+                     "s_waitcnt lgkmcnt(0)"
+                     : "=&v"(r0), "=&v"(r1), "=&v"(r2), "=&v"(r3)
+                     : "v"(tile + at.tr[d][0]), "v"(tile + at.tr[d][1]), "v"(tile + at.tr[d + 1][0]), "v"(tile + at.tr[d + 1][1]), "n"(OFF)
+                     : "memory");
+        f[d] = tr_pair(r0, r1);
+        f[d + 1] = tr_pair(r2, r3);
+    }
+}
+// the same for two 16-row steps, OFF and OFF + 32 D bytes
+template <int D, int OFF>
+__device__ __forceinline__ void tr_frags2(uint32_t tile, const LaneAt<D>& at, u16x8 (&f)[2][D / 32]) {
+#pragma unroll
+    for (int d = 0; d < D / 32; d += 2) {
+        s16x4 r0, r1, r2, r3, r4, r5, r6, r7;
+        asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n\t"
+                     "ds_read_b64_tr_b16 %1, %9 offset:%12\n\t"
+                     "ds_read_b64_tr_b16 %2, %10 offset:%12\n\t"
+                     "ds_read_b64_tr_b16 %3, %11 offset:%12\n\t"
+                     "ds_read_b64_tr_b16 %4, %8 offset:%13\n\t"
+                     "ds_read_b64_tr_b16 %5, %9 offset:%13\n\t"
+                     "ds_read_b64_tr_b16 %6, %10 offset:%13\n\t"
+                     "ds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+                     "s_waitcnt lgkmcnt(0)"
+                     : "=&v"(r0), "=&v"(r1), "=&v"(r2), "=&v"(r3), "=&v"(r4), "=&v"(r5), "=&v"(r6), "=&v"(r7)
+                     : "v"(tile + at.tr[d][0]), "v"(tile + at.tr[d][1]), "v"(tile + at.tr[d + 1][0]), "v"(tile + at.tr[d + 1][1]), "n"(OFF),
+                       "n"(OFF + 32 * D)
+                     : "memory");
+        f[0][d] = tr_pair(r0, r1);
+        f[0][d + 1] = tr_pair(r2, r3);
+        f[1][d] = tr_pair(r4, r5);
+        f[1][d + 1] = tr_pair(r6, r7);
+    }
 }
 
 typedef __attribute__((address_space(3))) void* lds_ptr;
@@ -136,16 +183,24 @@ __device__ __forceinline__ unsigned xcd_order(unsigned n, unsigned total) {
     return x * q + (x < r ? x : r) + i;
 }
 
-// Whether the 32 keys k0 .. and the nq queries q0 .. have visible pairs, and whether all pairs are.
-struct Vis {
-    bool any, all;
+// Which blocks of 32 keys a block of 32 queries sees at all, and sees whole, as bounds on the block's first key.
+struct BlockVis {
+    int any0, any1, all0, all1, sink, sink_all;
+    __device__ __forceinline__ BlockVis(int q0, int len, int left, int right, int sinks)
+        : any0(q0 - left - 31), any1(q0 < len ? min(q0 + 31 + right, len - 1) : -1), all0(q0 + 31 - left),
+          all1(min(q0 + right, len - 1) - 31), sink(sinks), sink_all(sinks - 31) {}
+    __device__ __forceinline__ bool any(int k0) const { return k0 <= any1 && (k0 >= any0 || k0 < sink); }
+    __device__ __forceinline__ bool all(int k0) const { return k0 <= all1 && (k0 >= all0 || k0 < sink_all); }
 };
-__device__ __forceinline__ Vis block_visibility(int q0, int nq, int k0, int len, int left, int right, int sinks) {
-    Vis r;
-    r.any = k0 < len && q0 < len && k0 <= q0 + nq - 1 + right && (k0 + 31 >= q0 - left || k0 < sinks);
-    r.all = k0 + 31 < len && k0 + 31 <= q0 + right && (k0 >= q0 + nq - 1 - left || k0 + 31 < sinks);
-    return r;
-}
+
+// The same for the query blocks that a block of 32 keys is seen by (lengths are taken care of elsewhere).
+struct QueryVis {
+    int any0, any1, all0, all1;
+    __device__ __forceinline__ QueryVis(int k0, int len, int left, int right, int sinks)
+        : any0(k0 - right - 31), any1(k0 < sinks ? len : k0 + 31 + left), all0(k0 + 31 - right), all1((k0 + 31 < sinks ? len : k0 + left) - 31) {}
+    __device__ __forceinline__ bool any(int q0) const { return q0 >= any0 && q0 <= any1; }
+    __device__ __forceinline__ bool all(int q0) const { return q0 >= all0 && q0 <= all1; }
+};
 
 // The key tiles (of BN) that queries qa .. qb see: [0, st) of the sinks, then [w0, w0 + n - st)
 struct KeyTiles {
@@ -277,6 +332,7 @@ __global__ __launch_bounds__(256, fwd_waves(D)) void window_fwd_kernel(WinArgs a
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] = zero16();
     tiles_landed();
+    const BlockVis vis(qw, len, a.left, a.right, a.sinks);
     for (int it = 0; it < kt.n; ++it) {
         const int k0 = kt.tile(it) * BN;
         char* const Ks = lds + (it & 1) * 2 * TILE;
@@ -290,12 +346,17 @@ __global__ __launch_bounds__(256, fwd_waves(D)) void window_fwd_kernel(WinArgs a
 #pragma unroll
         for (int u = 0; u < BN / 32; ++u) {
             const int kb = k0 + 32 * u;
-            const Vis vis = block_visibility(qw, 32, kb, len, a.left, a.right, a.sinks);
-            if (!vis.any) continue;
+            if (!vis.any(kb)) continue;
             f32x16 s = zero16();
 #pragma unroll
             for (int e = 0; e < NS; ++e) s = mfma32<FMT>(row_frag<D>(Ks, 32 * u, at, e), qf[e], s);
-            if (!vis.all) hide_keys(s, kb, kb + 4 * hi, q, len, a.left, a.right, a.sinks);
+            const uint32_t v_at = lds_offset(Vs) + 64 * D * u;
+            u16x8 vt[2][DT];
+            if constexpr (D == 64) {   // (wide heads have no registers to spare for this)
+                __builtin_amdgcn_sched_barrier(0);   // the value fragments are read while the scores are multiplied
+                tr_frags2<D, 0>(v_at, at, vt);
+            }
+            if (!vis.all(kb)) hide_keys(s, kb, kb + 4 * hi, q, len, a.left, a.right, a.sinks);
             float mx = s[0];
 #pragma unroll
             for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
@@ -320,8 +381,12 @@ __global__ __launch_bounds__(256, fwd_waves(D)) void window_fwd_kernel(WinArgs a
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
                 const u16x8 p = pack_step_unit<FMT>(s, st);
+                if constexpr (D != 64) {
+                    if (st == 0) tr_frags<D, 0>(v_at, at, vt[0]);
+                    else tr_frags<D, 32 * D>(v_at, at, vt[1]);
+                }
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) o[dt] = mfma32<FMT>(tr_frag<D>(Vs, 32 * u + 16 * st, at, dt), p, o[dt]);
+                for (int dt = 0; dt < DT; ++dt) o[dt] = mfma32<FMT>(vt[st][dt], p, o[dt]);
             }
         }
         if (more) tiles_landed();
@@ -395,6 +460,7 @@ __global__ __launch_bounds__(256, bwd_waves(D)) void window_dq_kernel(WinArgs a)
 #pragma unroll
     for (int r = 0; r < 16; ++r) start[r] = -delta;
     tiles_landed();
+    const BlockVis vis(qw, len, a.left, a.right, a.sinks);
     for (int it = 0; it < kt.n; ++it) {
         const int k0 = kt.tile(it) * BN;
         char* const Ks = lds + (it & 1) * 2 * TILE;
@@ -408,22 +474,24 @@ __global__ __launch_bounds__(256, bwd_waves(D)) void window_dq_kernel(WinArgs a)
 #pragma unroll
         for (int u = 0; u < BN / 32; ++u) {
             const int kb = k0 + 32 * u;
-            const Vis vis = block_visibility(qw, 32, kb, len, a.left, a.right, a.sinks);
-            if (!vis.any) continue;
+            if (!vis.any(kb)) continue;
             f32x16 s = zero16(), dp = start;
 #pragma unroll
             for (int e = 0; e < NS; ++e) {
                 s = mfma32<FMT>(row_frag<D>(Ks, 32 * u, at, e), qf[e], s);
                 dp = mfma32<FMT>(row_frag<D>(Vs, 32 * u, at, e), df[e], dp);
             }
-            if (!vis.all) hide_keys(s, kb, kb + 4 * hi, q, len, a.left, a.right, a.sinks);
+            __builtin_amdgcn_sched_barrier(0);
+            u16x8 kt2[2][DT];
+            tr_frags2<D, 0>(lds_offset(Ks) + 64 * D * u, at, kt2);
+            if (!vis.all(kb)) hide_keys(s, kb, kb + 4 * hi, q, len, a.left, a.right, a.sinks);
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], sc, -ls)) * dp[r];
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
                 const u16x8 e = pack_step<FMT>(s, st);
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) acc[dt] = mfma32<FMT>(tr_frag<D>(Ks, 32 * u + 16 * st, at, dt), e, acc[dt]);
+                for (int dt = 0; dt < DT; ++dt) acc[dt] = mfma32<FMT>(kt2[st][dt], e, acc[dt]);
             }
         }
         if (more) tiles_landed();
@@ -520,6 +588,7 @@ __global__ __launch_bounds__(256, bwd_waves(D)) void window_dkv_kernel(WinArgs a
         request(lds);
         landed(lds);
     }
+    const QueryVis vis(k0w, len, a.left, a.right, a.sinks);
     int qt = t0;
     for (int it = 0; it < total; ++it) {
         const int q0 = qt * BQ;
@@ -535,8 +604,7 @@ __global__ __launch_bounds__(256, bwd_waves(D)) void window_dkv_kernel(WinArgs a
         for (int u = 0; u < BQ / 32; ++u) {
             if (far && (BQ == 64 ? 2 * (it & 1) + u : it & 3) != wave) continue;
             const int qs = q0 + 32 * u;
-            const Vis vis = block_visibility(qs, 32, k0w, len, a.left, a.right, a.sinks);
-            if (!vis.any) continue;
+            if (!vis.any(qs)) continue;
             f32x16 s, dp;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
@@ -553,7 +621,7 @@ __global__ __launch_bounds__(256, bwd_waves(D)) void window_dkv_kernel(WinArgs a
                 s = mfma32<FMT>(row_frag<D>(Qs, 32 * u, at, e), kf[e], s);
                 dp = mfma32<FMT>(row_frag<D>(Ds, 32 * u, at, e), vf[e], dp);
             }
-            if (!vis.all) {
+            if (!vis.all(qs)) {
                 // q - key of register r is base + 8 (r / 4) + r % 4: seen from -right to left, and any later query by a sink
                 const int base = qs + 4 * hi - key;
                 const unsigned span = (unsigned)(a.right + (key < a.sinks ? 2 * a.T : a.left));
@@ -565,15 +633,20 @@ __global__ __launch_bounds__(256, bwd_waves(D)) void window_dkv_kernel(WinArgs a
                 s[r] = __builtin_amdgcn_exp2f(s[r] * sc);
                 dp[r] *= s[r];
             }
-#pragma unroll
-            for (int st = 0; st < 2; ++st) {
+            const uint32_t q_at = lds_offset(Qs) + 64 * D * u;
+            auto step = [&](auto off, int st) {
+                constexpr int OFF = decltype(off)::value;
+                u16x8 t[DT];
+                tr_frags<D, OFF>(q_at + TILE, at, t);
                 const u16x8 pf = pack_step_unit<FMT>(s, st), ef = pack_step<FMT>(dp, st);
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) {
-                    av[dt] = mfma32<FMT>(tr_frag<D>(Ds, 32 * u + 16 * st, at, dt), pf, av[dt]);
-                    ak[dt] = mfma32<FMT>(tr_frag<D>(Qs, 32 * u + 16 * st, at, dt), ef, ak[dt]);
-                }
-            }
+                for (int dt = 0; dt < DT; ++dt) av[dt] = mfma32<FMT>(t[dt], pf, av[dt]);
+                tr_frags<D, OFF>(q_at, at, t);
+#pragma unroll
+                for (int dt = 0; dt < DT; ++dt) ak[dt] = mfma32<FMT>(t[dt], ef, ak[dt]);
+            };
+            step(std::integral_constant<int, 0>{}, 0);
+            step(std::integral_constant<int, 32 * D>{}, 1);
         }
         if (more) landed(next);
     }
@@ -670,31 +743,19 @@ size_t delta_bytes(const WinArgs& a) { return ((size_t)a.B * a.Hq * a.T * sizeof
 
 }  // namespace
 
-// launches a kernel whose LDS size may pass the default limit of a launch
-template <typename K>
-hipError_t launch_lds(K* kernel, LdsAttrState& attr, unsigned blocks, int lds, const WinArgs& a, hipStream_t s) {
-    const hipError_t e = ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), lds, attr);
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), lds, s, a);
+template <int FMT, int D>
+hipError_t launch_fwd(const WinArgs& a, hipStream_t s) {
+    hipLaunchKernelGGL((window_fwd_kernel<FMT, D>), dim3((unsigned)(a.B * a.Hq * a.tiles)), dim3(256), 4 * 8192, s, a);
     return hipGetLastError();
 }
 
 template <int FMT, int D>
-hipError_t launch_fwd(const WinArgs& a, hipStream_t s) {
-    static LdsAttrState attr;
-    return launch_lds(&window_fwd_kernel<FMT, D>, attr, (unsigned)(a.B * a.Hq * a.tiles), 4 * 8192, a, s);
-}
-
-template <int FMT, int D>
 hipError_t launch_bwd(const WinArgs& a, hipStream_t s) {
-    static LdsAttrState at_q, at_k;
     const int sb = (a.sinks + 31) / 32;
-    hipError_t e = launch_lds(&window_dq_kernel<FMT, D>, at_q, (unsigned)(a.B * a.Hq * a.tiles), 4 * 8192, a, s);
-    if (e != hipSuccess) return e;
-    e = launch_lds(&window_dkv_kernel<FMT, D>, at_k, (unsigned)(a.B * a.Hk * (a.tiles + sb * a.far_blocks)), 2 * (2 * 8192 + 2 * tile_rows(D) * 4),
-                   a, s);
-    if (e != hipSuccess || a.far_blocks == 0) return e;
-    hipLaunchKernelGGL((window_sink_kernel<FMT, D>), dim3(a.B * a.Hk * sb * 4), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((window_dq_kernel<FMT, D>), dim3((unsigned)(a.B * a.Hq * a.tiles)), dim3(256), 4 * 8192, s, a);
+    hipLaunchKernelGGL((window_dkv_kernel<FMT, D>), dim3((unsigned)(a.B * a.Hk * (a.tiles + sb * a.far_blocks))), dim3(256),
+                       2 * (2 * 8192 + 2 * tile_rows(D) * 4), s, a);
+    if (a.far_blocks > 0) hipLaunchKernelGGL((window_sink_kernel<FMT, D>), dim3(a.B * a.Hk * sb * 4), dim3(256), 0, s, a);
     return hipGetLastError();
 }
 

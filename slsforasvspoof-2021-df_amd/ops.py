@@ -8,6 +8,7 @@ here computes on the host.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from typing import Optional
 
 import torch
@@ -462,110 +463,162 @@ def window_topk(acts: torch.Tensor, k: int, window: int, want_16bit: bool = Fals
 
 
 # ---- attention for recordings of any length and for live streams -----------------------------------------------------
+# A call on one frame or one clip is bound by what happens here on the host, so the checks below read each tensor's
+# metadata once, describe tensors to the library in packed words, and form messages only when something is wrong.
 
-def _require(ok: bool, what: str) -> None:
-    if not ok:
-        raise _lib.SlsmiError(what)
+_HEADS = struct.Struct("Pqqq")              # slsmi_heads
+_SHAPE = struct.Struct("9if")               # slsmi_window_shape
+_DTYPE_FMT = {torch.bfloat16: _lib.FMT_BF16, torch.float16: _lib.FMT_F16}
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
+    lambda index: torch.cuda.current_stream(index).cuda_stream
 
 
-def _same_device(first: torch.Tensor, *rest: Optional[torch.Tensor]) -> None:
-    _need_cuda(first, *rest)
-    for t in rest:
-        _require(t is None or t.device == first.device, f"tensors on {first.device} and {t.device if t is not None else ''}")
+def _refuse(what: str):
+    raise _lib.SlsmiError(what)
+
+
+def _on_device(index: int, fn, *args) -> None:
+    """fn(*args, stream) on the device's current stream, which becomes the current device for the call."""
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc, None, fn.__name__)
+
+
+def _device_of(t: torch.Tensor) -> int:
+    i = t.get_device()
+    if i < 0:
+        _refuse("slsmi ops need ROCm tensors; there is no CPU path")
+    return i
+
+
+def _vector(t: Optional[torch.Tensor], name: str, dtype: torch.dtype, shape, index: int) -> Optional[int]:
+    """Address of a contiguous tensor of the given type and shape on device `index`; None stays None."""
+    if t is None:
+        return None
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != index:
+        _refuse(f"{name}: contiguous {dtype} {tuple(shape)} on device {index} expected, got {t.dtype} {tuple(t.shape)}, strides "
+                f"{t.stride()}, on {t.device}")
+    return t.data_ptr()
 
 
 def _window_side(n: Optional[int], name: str) -> int:
     if n is None:
         return -1
-    _require(int(n) == n and n >= 0, f"{name}: frames (0 or more), or None for no limit; got {n}")
+    if n < 0 or n != int(n):
+        _refuse(f"{name}: frames (0 or more), or None for no limit; got {n}")
     return min(int(n), 0x7fffffff)
 
 
 def _distinct(t: torch.Tensor) -> bool:
     """No two elements of t share memory (sufficient: each dimension steps past all smaller ones)."""
+    if t.is_contiguous():
+        return True
     reach = 1
     for size, stride in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n > 1), key=lambda d: d[1]):
         if stride < reach:
             return False
-        reach = stride * (size - 1) + reach
+        reach += stride * (size - 1)
     return True
 
 
-def _heads_arg(t: torch.Tensor, name: str, shape, dtype: torch.dtype, written: bool = False) -> _lib.Heads:
+def _heads_arg(t: torch.Tensor, name: str, shape, dtype: torch.dtype, index: int, written: bool = False) -> bytes:
     """[batch, frames, heads, head_dim] by its strides; a view of packed rows is taken as it is."""
-    _require(tuple(t.shape) == tuple(shape), f"{name}: shape {tuple(shape)} expected, got {tuple(t.shape)}")
-    _require(t.dtype == dtype, f"{name}: {dtype} expected, got {t.dtype}")
-    st = [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
-    _require(t.numel() == 0 or (t.stride(3) == 1 and all(s % 8 == 0 for s in st[:3]) and t.data_ptr() % 16 == 0),
-             f"{name}: channels must be contiguous, strides multiples of 8 and the data 16-byte aligned; got strides "
-             f"{t.stride()}")
-    _require(t.numel() == 0 or ((st[1] >= shape[3] or shape[1] == 1) and (st[2] >= shape[3] or shape[2] == 1)),
-             f"{name}: rows and heads must be distinct (an expanded tensor?); got strides {t.stride()}")
-    _require(not written or _distinct(t), f"{name}: its elements share memory; got strides {t.stride()}")
-    return _lib.Heads(t.data_ptr(), st[0], st[1], st[2])
+    if t.shape != shape or t.dtype != dtype or t.get_device() != index:
+        _refuse(f"{name}: {dtype} {tuple(shape)} on device {index} expected, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    b, r, h, c = t.stride()
+    p = t.data_ptr()
+    D = shape[3]
+    if c != 1 or (b | r | h) & 7 or p & 15 or r < D or h < D:
+        if t.numel() == 0:
+            return _HEADS.pack(0, 0, 0, 0)
+        b, r, h = (s if n > 1 else D for s, n in zip((b, r, h), shape))   # the step of a single entry means nothing
+        if c != 1 or (b | r | h) & 7 or p & 15 or b < 0:
+            _refuse(f"{name}: channels must be contiguous, strides multiples of 8 and the data 16-byte aligned; got strides "
+                    f"{t.stride()}")
+        if r < D or h < D:
+            _refuse(f"{name}: rows and heads must be distinct (an expanded tensor?); got strides {t.stride()}")
+    if written and not _distinct(t):
+        _refuse(f"{name}: its elements share memory; got strides {t.stride()}")
+    return _HEADS.pack(p, b, r, h)
 
 
-def _window_shape(q: torch.Tensor, kv_heads: int, left, right, sinks: int, scale: Optional[float]) -> _lib.WindowShape:
-    B, T, H, D = q.shape
-    _require(D in (64, 128), f"head width 64 or 128 expected, got {D}")
-    _require(kv_heads >= 1 and H >= 1 and H % kv_heads == 0, f"{H} query heads cannot share {kv_heads} key heads")
-    _require(0 <= sinks <= 128, f"sinks: 0 to 128 first frames, got {sinks}")
+def _group(heads: int, kv_heads: int, D: int, dtype: torch.dtype) -> int:
+    """Checks a head layout; the operand format."""
+    if D != 64 and D != 128:
+        _refuse(f"head width 64 or 128 expected, got {D}")
+    if kv_heads < 1 or heads < 1 or heads % kv_heads:
+        _refuse(f"{heads} query heads cannot share {kv_heads} key heads")
+    fmt = _DTYPE_FMT.get(dtype)
+    if fmt is None:
+        _refuse(f"16-bit operand expected, got {dtype}")
+    return fmt
+
+
+def _window_shape(q: torch.Tensor, k: torch.Tensor, left, right, sinks: int, scale: Optional[float]):
+    """(q's shape, k's shape, packed slsmi_window_shape)"""
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4:
+        _refuse(f"q, k, v [batch, frames, heads, D] expected, got {tuple(qs)}, {tuple(ks)}")
+    B, T, H, D = qs
+    kv = ks[2]
+    fmt = _group(H, kv, D, q.dtype)
+    if not 0 <= sinks <= 128:
+        _refuse(f"sinks: 0 to 128 first frames, got {sinks}")
     scale = D ** -0.5 if scale is None else float(scale)
-    _require(0.0 < scale < float("inf"), f"scale must be positive, got {scale}")
-    return _lib.WindowShape(B, T, H, kv_heads, D, _window_side(left, "left"), _window_side(right, "right"), int(sinks), _fmt(q),
-                            scale)
+    if not 0.0 < scale < float("inf"):
+        _refuse(f"scale must be positive, got {scale}")
+    return qs, (B, T, kv, D), _SHAPE.pack(B, T, H, kv, D, _window_side(left, "left"), _window_side(right, "right"), sinks, fmt, scale)
 
 
-def _nframes_arg(nframes: Optional[torch.Tensor], B: int) -> Optional[torch.Tensor]:
-    if nframes is not None:
-        _require(nframes.dtype == torch.int32 and tuple(nframes.shape) == (B,) and nframes.is_contiguous(),
-                 f"nframes: int32 [{B}] expected, got {nframes.dtype} {tuple(nframes.shape)}")
-    return nframes
-
-
-def _rows_arg(t: torch.Tensor, name: str, width: int, dtype: torch.dtype, lead=None, written: bool = False):
-    """(rows, row stride) of [rows, >= width] or [batch, frames, >= width] whose rows lie at one distance."""
-    _require(t.dtype == dtype, f"{name}: {dtype} expected, got {t.dtype}")
-    _require(t.dim() in (2, 3) and t.shape[-1] >= width, f"{name}: rows of at least {width} values expected, got {tuple(t.shape)}")
-    _require(lead is None or t.shape[:-1] == lead, f"{name}: leading shape {lead} expected, got {tuple(t.shape[:-1])}")
-    rows = t.numel() // t.shape[-1]
-    if rows == 0:
-        return 0, t.shape[-1]
-    ld = t.stride(-2) if t.shape[-2] > 1 else (t.stride(0) if t.dim() == 3 and t.shape[0] > 1 else t.shape[-1])
-    _require(t.dim() == 2 or t.shape[0] == 1 or t.shape[1] == 1 or t.stride(0) == t.shape[1] * t.stride(1),
-             f"{name}: all rows must lie at one distance; got strides {t.stride()}")
-    if rows == 1:
+def _rows_arg(t: torch.Tensor, name: str, width: int, dtype: torch.dtype, index: int, lead=None, written: bool = False) -> int:
+    """Row stride of [rows, >= width] or [batch, frames, >= width] whose rows lie at one distance."""
+    shape = t.shape
+    if t.dtype != dtype or len(shape) not in (2, 3) or shape[-1] < width or t.get_device() != index or \
+            (lead is not None and shape[:-1] != lead):
+        _refuse(f"{name}: {dtype} {'rows' if lead is None else tuple(lead)} of at least {width} values on device {index} expected, "
+                f"got {t.dtype} {tuple(shape)} on {t.device}")
+    st = t.stride()
+    rows = shape[0] if len(shape) == 2 else shape[0] * shape[1]
+    if rows <= 1:
         ld = (width + 7) // 8 * 8
-    _require(t.stride(-1) == 1 and ld % 8 == 0 and ld >= width and t.data_ptr() % 16 == 0,
-             f"{name}: contiguous channels, a row stride that is a multiple of 8 and 16-byte alignment needed; got strides "
-             f"{t.stride()}")
-    return rows, ld
+    elif len(shape) == 2 or shape[0] == 1:
+        ld = st[-2]
+    elif shape[1] == 1:
+        ld = st[0]
+    else:
+        ld = st[1]
+        if st[0] != shape[1] * ld:
+            _refuse(f"{name}: all rows must lie at one distance; got strides {st}")
+    if rows and (st[-1] != 1 or ld & 7 or ld < width or t.data_ptr() & 15):
+        _refuse(f"{name}: contiguous channels, a row stride that is a multiple of 8 and 16-byte alignment needed; got strides {st}")
+    return ld
 
 
-def _norm_args(x: torch.Tensor, q_weight, k_weight, freqs, positions, lead):
+def _norm_args(q_weight, k_weight, freqs, positions, lead, index: int):
+    """(D, rotary_dim, rows, npos, addresses of q_weight, k_weight, freqs, positions)"""
     D = q_weight.numel()
-    _require(D in (64, 128), f"head width 64 or 128 expected, got {D} norm weights")
-    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        _require(w.dtype == torch.float32 and tuple(w.shape) == (D,) and w.is_contiguous(),
-                 f"{name}: contiguous float32 [{D}] expected, got {w.dtype} {tuple(w.shape)}")
-    R = 0
+    if D != 64 and D != 128:
+        _refuse(f"head width 64 or 128 expected, got {D} norm weights")
+    wq = _vector(q_weight, "q_weight", torch.float32, (D,), index)
+    wk = _vector(k_weight, "k_weight", torch.float32, (D,), index)
+    R, fr = 0, None
     if freqs is not None:
-        _require(freqs.dtype == torch.float64 and freqs.dim() == 1 and freqs.is_contiguous(),
-                 f"freqs: contiguous float64 [rotary_dim / 2] expected, got {freqs.dtype} {tuple(freqs.shape)}")
         R = 2 * freqs.numel()
-        _require(R % 16 == 0 and R <= D, f"the rotated width must be a multiple of 16 up to {D}, got {R}")
-    rows = 1
+        if R % 16 or R > D:
+            _refuse(f"the rotated width must be a multiple of 16 up to {D}, got {R}")
+        fr = _vector(freqs, "freqs", torch.float64, (R // 2,), index) if R else None
+    rows, T = 1, lead[-1]
     for n in lead:
         rows *= n
-    T = lead[-1]
-    npos = max(1, T)
+    npos, pos = T, None
     if positions is not None:
-        _require(positions.dtype == torch.int64 and positions.is_contiguous() and
-                 (tuple(positions.shape) == tuple(lead) or tuple(positions.shape) == (T,)),
-                 f"positions: contiguous int64 {tuple(lead)} or {(T,)} expected, got {positions.dtype} {tuple(positions.shape)}")
-        npos = max(1, positions.numel())
-    _same_device(x, q_weight, k_weight, freqs, positions)
-    return D, R, rows, npos
+        npos = positions.numel()
+        pos = _vector(positions, "positions", torch.int64, lead if positions.dim() == len(lead) else (T,), index)
+    return D, R, rows, max(1, npos), wq, wk, fr, pos
 
 
 def qk_norm_rope(qkv: torch.Tensor, heads: int, kv_heads: int, q_weight: torch.Tensor, k_weight: torch.Tensor,
@@ -578,22 +631,21 @@ def qk_norm_rope(qkv: torch.Tensor, heads: int, kv_heads: int, q_weight: torch.T
     (None: no rotation): pairs (i, i + R / 2), or neighbours with interleaved.  positions int64, one per row or one per
     frame; None counts frames (or rows) from 0.  Returns [..., (heads + kv_heads) * D]; out (may be qkv itself) receives
     the heads in its first columns instead, the rest of its rows is left alone."""
-    _need_cuda(qkv, out)
+    index = _device_of(qkv)
     lead = qkv.shape[:-1]
-    D, R, rows, npos = _norm_args(qkv, q_weight, k_weight, freqs, positions, lead)
-    _require(heads >= 0 and kv_heads >= 0 and heads + kv_heads >= 1, f"{heads} query and {kv_heads} key heads")
+    D, R, rows, npos, wq, wk, fr, pos = _norm_args(q_weight, k_weight, freqs, positions, lead, index)
+    if heads < 0 or kv_heads < 0 or heads + kv_heads < 1:
+        _refuse(f"{heads} query and {kv_heads} key heads")
     width = (heads + kv_heads) * D
-    fmt = _fmt(qkv)
-    _, ldx = _rows_arg(qkv, "qkv", width, qkv.dtype)
+    dtype = qkv.dtype
+    fmt = _group(1, 1, D, dtype)
+    ldx = _rows_arg(qkv, "qkv", width, dtype, index)
     if out is None:
-        out = torch.empty(*lead, width, dtype=qkv.dtype, device=qkv.device)
-    _same_device(qkv, out)
-    _, ldy = _rows_arg(out, "out", width, qkv.dtype, lead)
-    with torch.cuda.device(qkv.device):
-        rc = _lib.load().slsmi_qk_norm_rope(_p(qkv), ldx, _p(out), ldy, rows, heads, kv_heads, D, _p(q_weight), _p(k_weight),
-                                            float(eps), _p(freqs), R, int(interleaved), _p(positions), npos, fmt,
-                                            _s(qkv.device))
-    _lib.check(rc, None, "slsmi_qk_norm_rope")
+        out, ldy = qkv.new_empty(lead + (width,)), width
+    else:
+        ldy = _rows_arg(out, "out", width, dtype, index, lead)
+    _on_device(index, _lib.load().slsmi_qk_norm_rope, qkv.data_ptr(), ldx, out.data_ptr(), ldy, rows, heads, kv_heads, D, wq, wk,
+               eps, fr, R, interleaved, pos, npos, fmt)
     return out
 
 
@@ -604,27 +656,28 @@ def qk_norm_rope_backward(dout: torch.Tensor, qkv: torch.Tensor, heads: int, kv_
     """Gradient of qk_norm_rope: dout at its result, qkv as it was given -> (dqkv [..., (heads + kv_heads) * D],
     dq_weight, dk_weight).  out: where dqkv goes (dout itself, or the packed gradient whose value columns
     window_attention_backward wrote)."""
-    _need_cuda(dout, qkv, out)
+    index = _device_of(qkv)
     lead = qkv.shape[:-1]
-    D, R, rows, npos = _norm_args(qkv, q_weight, k_weight, freqs, positions, lead)
-    _require(heads >= 0 and kv_heads >= 0 and heads + kv_heads >= 1, f"{heads} query and {kv_heads} key heads")
+    D, R, rows, npos, wq, wk, fr, pos = _norm_args(q_weight, k_weight, freqs, positions, lead, index)
+    if heads < 0 or kv_heads < 0 or heads + kv_heads < 1:
+        _refuse(f"{heads} query and {kv_heads} key heads")
     width = (heads + kv_heads) * D
-    fmt = _fmt(qkv)
-    _, ldx = _rows_arg(qkv, "qkv", width, qkv.dtype)
-    _, lddy = _rows_arg(dout, "dout", width, qkv.dtype, lead)
+    dtype = qkv.dtype
+    fmt = _group(1, 1, D, dtype)
+    ldx = _rows_arg(qkv, "qkv", width, dtype, index)
+    lddy = _rows_arg(dout, "dout", width, dtype, index, lead)
     if out is None:
-        out = torch.empty(*lead, width, dtype=qkv.dtype, device=qkv.device)
-    _same_device(qkv, dout, out)
-    _, lddx = _rows_arg(out, "out", width, qkv.dtype, lead)
-    dwq, dwk = torch.empty_like(q_weight), torch.empty_like(k_weight)
+        out, lddx = qkv.new_empty(lead + (width,)), width
+    else:
+        lddx = _rows_arg(out, "out", width, dtype, index, lead)
+    dw = torch.empty(2, D, dtype=torch.float32, device=qkv.device)
+    dwq, dwk = dw[0], dw[1]
     lib = _lib.load()
     n = lib.slsmi_qk_norm_rope_backward_workspace_bytes(rows, D)
     ws = torch.empty(n, dtype=torch.uint8, device=qkv.device)
-    with torch.cuda.device(qkv.device):
-        rc = lib.slsmi_qk_norm_rope_backward(_p(dout), lddy, _p(qkv), ldx, _p(out), lddx, rows, heads, kv_heads, D, _p(q_weight),
-                                             _p(k_weight), float(eps), _p(freqs), R, int(interleaved), _p(positions), npos,
-                                             _p(dwq), _p(dwk), _p(ws), n, fmt, _s(qkv.device))
-    _lib.check(rc, None, "slsmi_qk_norm_rope_backward")
+    _on_device(index, lib.slsmi_qk_norm_rope_backward, dout.data_ptr(), lddy, qkv.data_ptr(), ldx, out.data_ptr(), lddx, rows,
+               heads, kv_heads, D, wq, wk, eps, fr, R, interleaved, pos, npos, dwq.data_ptr(), dwk.data_ptr(), ws.data_ptr(), n,
+               fmt)
     return out, dwq, dwk
 
 
@@ -638,19 +691,16 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: Op
     recording's nframes (int32 [batch] on the device; None: all).  None for left or right: no limit.  scale: 1 / sqrt(D)
     unless given.  Returns [batch, frames, heads, D], zeros at padded frames; with return_lse also the rows'
     log-sum-exp, fp32 [batch, heads, frames], for window_attention_backward."""
-    _same_device(q, k, v, nframes, out)
-    _require(q.dim() == 4 and k.dim() == 4, f"q, k, v [batch, frames, heads, D] expected, got {tuple(q.shape)}, {tuple(k.shape)}")
-    B, T, H, D = q.shape
-    shape = _window_shape(q, k.shape[2], left, right, sinks, scale)
-    kv = (B, T, k.shape[2], D)
-    out = torch.empty(B, T, H, D, dtype=q.dtype, device=q.device) if out is None else out
-    args = [_heads_arg(q, "q", q.shape, q.dtype), _heads_arg(k, "k", kv, q.dtype), _heads_arg(v, "v", kv, q.dtype),
-            _heads_arg(out, "out", q.shape, q.dtype, written=True)]
-    lse = torch.empty(B, H, T, dtype=torch.float32, device=q.device) if return_lse else None
-    with torch.cuda.device(q.device):
-        rc = _lib.load().slsmi_window_attention(C.byref(shape), *(C.byref(x) for x in args), _p(lse),
-                                                _p(_nframes_arg(nframes, B)), _s(q.device))
-    _lib.check(rc, None, "slsmi_window_attention")
+    index = _device_of(q)
+    qs, ks, shape = _window_shape(q, k, left, right, sinks, scale)
+    dtype = q.dtype
+    if out is None:
+        out = q.new_empty(qs)
+    aq, ak, av = _heads_arg(q, "q", qs, dtype, index), _heads_arg(k, "k", ks, dtype, index), _heads_arg(v, "v", ks, dtype, index)
+    ao = _heads_arg(out, "out", qs, dtype, index, True)
+    lse = torch.empty(qs[0], qs[2], qs[1], dtype=torch.float32, device=q.device) if return_lse else None
+    _on_device(index, _lib.load().slsmi_window_attention, shape, aq, ak, av, ao, lse.data_ptr() if return_lse else None,
+               _vector(nframes, "nframes", torch.int32, qs[:1], index))
     return (out, lse) if return_lse else out
 
 
@@ -662,39 +712,35 @@ def window_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tens
     """Gradient of window_attention at q, k, v from its out and lse, the other arguments as given to it
     (slsmi_window_attention_backward).  dq, dk, dv: where the gradients go (views of packed rows, say); new tensors unless
     given.  Gradients at padded frames are zeros.  Returns (dq, dk, dv)."""
-    _same_device(q, dout, k, v, out, lse, nframes, dq, dk, dv)
-    _require(q.dim() == 4 and k.dim() == 4, f"q, k, v [batch, frames, heads, D] expected, got {tuple(q.shape)}, {tuple(k.shape)}")
-    B, T, H, D = q.shape
-    shape = _window_shape(q, k.shape[2], left, right, sinks, scale)
-    kv = (B, T, k.shape[2], D)
-    _require(lse.dtype == torch.float32 and tuple(lse.shape) == (B, H, T) and lse.is_contiguous(),
-             f"lse: contiguous float32 {(B, H, T)} expected, got {lse.dtype} {tuple(lse.shape)}")
-    dq = torch.empty(B, T, H, D, dtype=q.dtype, device=q.device) if dq is None else dq
-    dk = torch.empty(kv, dtype=q.dtype, device=q.device) if dk is None else dk
-    dv = torch.empty(kv, dtype=q.dtype, device=q.device) if dv is None else dv
-    ins = [_heads_arg(t, n, s, q.dtype) for t, n, s in ((dout, "dout", q.shape), (q, "q", q.shape), (k, "k", kv), (v, "v", kv),
-                                                       (out, "out", q.shape))]
-    outs = [_heads_arg(t, n, s, q.dtype, written=True) for t, n, s in ((dq, "dq", q.shape), (dk, "dk", kv), (dv, "dv", kv))]
+    index = _device_of(q)
+    qs, ks, shape = _window_shape(q, k, left, right, sinks, scale)
+    dtype = q.dtype
+    dq = q.new_empty(qs) if dq is None else dq
+    dk = q.new_empty(ks) if dk is None else dk
+    dv = q.new_empty(ks) if dv is None else dv
+    args = [_heads_arg(t, n, s, dtype, index) for t, n, s in ((dout, "dout", qs), (q, "q", qs), (k, "k", ks), (v, "v", ks),
+                                                             (out, "out", qs))]
+    outs = [_heads_arg(t, n, s, dtype, index, True) for t, n, s in ((dq, "dq", qs), (dk, "dk", ks), (dv, "dv", ks))]
+    lse_at = _vector(lse, "lse", torch.float32, (qs[0], qs[2], qs[1]), index)
     lib = _lib.load()
-    n = lib.slsmi_window_attention_backward_workspace_bytes(C.byref(shape))
+    n = lib.slsmi_window_attention_backward_workspace_bytes(shape)
     ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-    with torch.cuda.device(q.device):
-        rc = lib.slsmi_window_attention_backward(C.byref(shape), *(C.byref(x) for x in ins), _p(lse),
-                                                 _p(_nframes_arg(nframes, B)), *(C.byref(x) for x in outs), _p(ws), n,
-                                                 _s(q.device))
-    _lib.check(rc, None, "slsmi_window_attention_backward")
+    _on_device(index, lib.slsmi_window_attention_backward, shape, *args, lse_at,
+               _vector(nframes, "nframes", torch.int32, qs[:1], index), *outs, ws.data_ptr(), n)
     return dq, dk, dv
 
 
-def _cache_args(k_cache: torch.Tensor, v_cache: torch.Tensor, sinks: int):
-    _require(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.dtype == v_cache.dtype and
-             k_cache.is_contiguous() and v_cache.is_contiguous(),
-             f"k_cache, v_cache: contiguous [batch, kv_heads, slots, D] of one type expected, got {tuple(k_cache.shape)}, "
-             f"{tuple(v_cache.shape)}")
-    slots = k_cache.shape[2]
-    _require(0 <= sinks < slots <= 1 << 24, f"sinks + window slots (window at least 1, at most 2^24 in all) expected, got {slots} "
-             f"slots for {sinks} sinks")
-    return slots
+def _cache_args(k_cache: torch.Tensor, v_cache: torch.Tensor, sinks: int, index: int):
+    """(cache shape, addresses of both)"""
+    cs = k_cache.shape
+    if len(cs) != 4:
+        _refuse(f"k_cache, v_cache: [batch, kv_heads, slots, D] expected, got {tuple(cs)}")
+    if not 0 <= sinks < cs[2] <= 1 << 24:
+        _refuse(f"sinks + window slots (window at least 1, at most 2^24 in all) expected, got {cs[2]} slots for {sinks} sinks")
+    kc, vc = _vector(k_cache, "k_cache", k_cache.dtype, cs, index), _vector(v_cache, "v_cache", k_cache.dtype, cs, index)
+    if kc == vc and k_cache.numel():
+        _refuse("k_cache and v_cache are the same memory")
+    return cs, kc, vc
 
 
 def window_cache_fill(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, sinks: int,
@@ -702,19 +748,15 @@ def window_cache_fill(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v
     """Prefill of a rolling cache (slsmi_window_cache_fill): the keys and values [batch, frames, kv_heads, D] of
     recordings that begin at position 0 go to the slots their first `sinks` and their last (slots - sinks) frames live in.
     k_cache, v_cache [batch, kv_heads, slots, D]."""
-    _same_device(k, v, k_cache, v_cache, nframes)
-    slots = _cache_args(k_cache, v_cache, sinks)
-    _require(k.dim() == 4, f"k, v [batch, frames, kv_heads, D] expected, got {tuple(k.shape)}")
-    B, T, H, D = k.shape
-    _require(tuple(k_cache.shape) == (B, H, slots, D) and D in (64, 128) and H >= 1,
-             f"a cache {(B, H, slots, D)} with D 64 or 128 expected, got {tuple(k_cache.shape)}")
-    _require(k_cache.dtype == k.dtype, f"cache of {k_cache.dtype}, keys of {k.dtype}")
-    shape = _lib.WindowShape(B, T, H, H, D, -1, 0, int(sinks), _fmt(k), 1.0)
-    args = [_heads_arg(k, "k", k.shape, k.dtype), _heads_arg(v, "v", k.shape, k.dtype)]
-    with torch.cuda.device(k.device):
-        rc = _lib.load().slsmi_window_cache_fill(C.byref(shape), slots, C.byref(args[0]), C.byref(args[1]), _p(k_cache),
-                                                 _p(v_cache), _p(_nframes_arg(nframes, B)), _s(k.device))
-    _lib.check(rc, None, "slsmi_window_cache_fill")
+    index = _device_of(k)
+    cs, kc, vc = _cache_args(k_cache, v_cache, sinks, index)
+    ks, dtype = k.shape, k.dtype
+    if len(ks) != 4 or cs[0] != ks[0] or cs[1] != ks[2] or cs[3] != ks[3] or k_cache.dtype != dtype:
+        _refuse(f"k {k.dtype} {tuple(ks)} does not fit a cache {k_cache.dtype} {tuple(cs)}")
+    B, T, H, D = ks
+    shape = _SHAPE.pack(B, T, H, H, D, -1, 0, sinks, _group(H, H, D, dtype), 1.0)
+    _on_device(index, _lib.load().slsmi_window_cache_fill, shape, cs[2], _heads_arg(k, "k", ks, dtype, index),
+               _heads_arg(v, "v", ks, dtype, index), kc, vc, _vector(nframes, "nframes", torch.int32, (B,), index))
 
 
 def window_attention_step(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, positions: torch.Tensor, heads: int,
@@ -726,31 +768,30 @@ def window_attention_step(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     frame now).  The key and value go to the rolling cache k_cache, v_cache [batch, kv_heads, slots, D] and the result
     [batch, heads, D] is what window_attention(left=slots - sinks - 1, right=0, sinks=sinks) gives for that frame.  With
     q_weight and k_weight the norms and the rotation of qk_norm_rope happen inside.  The caller advances positions."""
-    _same_device(qkv, k_cache, v_cache, positions, q_weight, k_weight, freqs)
-    slots = _cache_args(k_cache, v_cache, sinks)
-    B, Hk, _, D = k_cache.shape
-    _require(D in (64, 128), f"head width 64 or 128 expected, got {D}")
-    _require(Hk >= 1 and heads >= 1 and heads % Hk == 0, f"{heads} query heads cannot share {Hk} key heads")
-    _require(qkv.dim() == 2 and tuple(qkv.shape) == (B, (heads + 2 * Hk) * D) and qkv.dtype == k_cache.dtype,
-             f"qkv: {k_cache.dtype} {(B, (heads + 2 * Hk) * D)} expected, got {qkv.dtype} {tuple(qkv.shape)}")
-    _require(positions.dtype == torch.int64 and tuple(positions.shape) == (B,) and positions.is_contiguous(),
-             f"positions: contiguous int64 [{B}] expected, got {positions.dtype} {tuple(positions.shape)}")
-    _require((q_weight is None) == (k_weight is None) and (q_weight is not None or freqs is None),
-             "the rotation needs both norm weights")
-    R = 0
-    if q_weight is not None:
-        n, R, _, _ = _norm_args(qkv, q_weight, k_weight, freqs, None, qkv.shape[:-1])
-        _require(n == D, f"norm weights of {D} channels expected, got {n}")
+    index = _device_of(qkv)
+    (B, Hk, slots, D), kc, vc = _cache_args(k_cache, v_cache, sinks, index)
+    dtype = qkv.dtype
+    fmt = _group(heads, Hk, D, dtype)
+    width = (heads + 2 * Hk) * D
+    if qkv.shape != (B, width) or k_cache.dtype != dtype:
+        _refuse(f"qkv: {k_cache.dtype} {(B, width)} expected, got {dtype} {tuple(qkv.shape)}")
+    ld = _rows_arg(qkv, "qkv", width, dtype, index)
+    pos = _vector(positions, "positions", torch.int64, (B,), index)
+    R, wq, wk, fr = 0, None, None, None
+    if q_weight is not None or k_weight is not None:
+        if q_weight is None or k_weight is None or q_weight.numel() != D:
+            _refuse(f"both norm weights, of {D} channels, expected")
+        _, R, _, _, wq, wk, fr, _ = _norm_args(q_weight, k_weight, freqs, None, (B,), index)
+    elif freqs is not None:
+        _refuse("the rotation needs both norm weights")
     scale = D ** -0.5 if scale is None else float(scale)
-    _require(0.0 < scale < float("inf"), f"scale must be positive, got {scale}")
-    _, ld = _rows_arg(qkv, "qkv", qkv.shape[1], qkv.dtype)
-    shape = _lib.WindowShape(B, 1, heads, Hk, D, -1, 0, int(sinks), _fmt(qkv), scale)
-    out = torch.empty(B, heads, D, dtype=qkv.dtype, device=qkv.device)
+    if not 0.0 < scale < float("inf"):
+        _refuse(f"scale must be positive, got {scale}")
+    shape = _SHAPE.pack(B, 1, heads, Hk, D, -1, 0, sinks, fmt, scale)
+    out = qkv.new_empty((B, heads, D))
     lib = _lib.load()
-    n = lib.slsmi_window_step_workspace_bytes(C.byref(shape), slots)
+    n = lib.slsmi_window_step_workspace_bytes(shape, slots)
     ws = torch.empty(n, dtype=torch.uint8, device=qkv.device) if n else None
-    with torch.cuda.device(qkv.device):
-        rc = lib.slsmi_window_step(C.byref(shape), slots, _p(qkv), ld, _p(k_cache), _p(v_cache), _p(positions), _p(q_weight),
-                                   _p(k_weight), float(eps), _p(freqs), R, int(interleaved), _p(out), _p(ws), n, _s(qkv.device))
-    _lib.check(rc, None, "slsmi_window_step")
+    _on_device(index, lib.slsmi_window_step, shape, slots, qkv.data_ptr(), ld, kc, vc, pos, wq, wk, eps, fr, R, interleaved,
+               out.data_ptr(), ws.data_ptr() if n else None, n)
     return out
