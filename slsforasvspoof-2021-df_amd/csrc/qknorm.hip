@@ -197,21 +197,23 @@ __global__ __launch_bounds__(QN_WAVES * 64) void qk_norm_rope_bwd_kernel(QkNormA
     }
 }
 
-// dwq, dwk [D] = sums of the partials [n][2][D] in a fixed order: 16 columns per workgroup, 16 rows of threads
-__global__ __launch_bounds__(256) void qk_norm_dw_kernel(const float* __restrict__ partial, int n, int D, float* __restrict__ dwq,
-                                                         float* __restrict__ dwk) {
-    __shared__ float red[16][17];
-    const int col = blockIdx.x * 16 + (threadIdx.x & 15), rg = threadIdx.x >> 4;
+// dwq, dwk [D] = sums of the partials [n][2][D] in a fixed order: 16 columns per workgroup, 64 threads each, added in a
+// tree
+__global__ __launch_bounds__(1024) void qk_norm_dw_kernel(const float* __restrict__ partial, int n, int D, float* __restrict__ dwq,
+                                                          float* __restrict__ dwk) {
+    __shared__ float red[64][17];
+    const int lc = threadIdx.x & 15, col = blockIdx.x * 16 + lc, rg = threadIdx.x >> 4;
     float s = 0.f;
-    for (int i = rg; i < n; i += 16) s += partial[(long)i * 2 * D + col];
-    red[rg][threadIdx.x & 15] = s;
+#pragma unroll 16
+    for (int i = rg; i < n; i += 64) s += partial[(long)i * 2 * D + col];
+    red[rg][lc] = s;
     __syncthreads();
-    if (rg == 0) {
-        float t = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) t += red[i][threadIdx.x & 15];
-        (col < D ? dwq : dwk)[col < D ? col : col - D] = t;
+    for (int o = 32; o > 0; o >>= 1) {
+        if (rg < o) red[rg][lc] += red[rg + o][lc];
+        __syncthreads();
     }
+    if (rg == 0) (col < D ? dwq : dwk)[col < D ? col : col - D] = red[0][lc];
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -284,7 +286,7 @@ hipError_t launch_qk_norm_rope_bwd(const QkNormParams& p, const bf16_t* dy, long
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL(qk_norm_dw_kernel, dim3(2 * p.D / 16), dim3(256), 0, s, ws, nb, p.D, dwq, dwk);
+    hipLaunchKernelGGL(qk_norm_dw_kernel, dim3(2 * p.D / 16), dim3(1024), 0, s, ws, nb, p.D, dwq, dwk);
     return hipGetLastError();
 }
 

@@ -512,8 +512,8 @@ __global__ __launch_bounds__(256, bwd_waves(D)) void window_dq_kernel(WinArgs a)
 //
 // The sinks' keys are seen by every later query: the queries past the near ones of a sink block (32 keys) are cut into
 // chunks of far_chunk, one workgroup each, whose four waves share the block's keys and take 32 of 128 queries in turn.
-// Those sums, and the near workgroup's for sink rows, go as fp32 to `part` [B][Hk][sink block][1 + 4 far_blocks][dK, dV]
-// [32 keys][D] and are added in that order by window_sink_kernel.
+// Their sums for the sinks' rows, and the near workgroup's for all rows of the block, go as fp32 to `part`
+// [B][Hk][sink block][1 + 4 far_blocks][dK, dV][32 keys][D] and are added in that order by window_sink_kernel.
 template <int FMT, int D>
 __global__ __launch_bounds__(256, bwd_waves(D)) void window_dkv_kernel(WinArgs a) {
     constexpr int NS = D / 16, DT = D / 32, BQ = tile_rows(D), TILE = BQ * D * 2, BUF = 2 * TILE + 2 * BQ * 4;
@@ -652,6 +652,7 @@ __global__ __launch_bounds__(256, bwd_waves(D)) void window_dkv_kernel(WinArgs a
     }
     if (far || (k0w < a.sinks && a.far_blocks > 0)) {
         const int blk = far ? block : k0w / 32, slot = far ? 1 + chunk * 4 + wave : 0;
+        if (far && key >= a.sinks) return;
         float* dst = a.part + ((((long)bh * sink_blocks + blk) * (1 + 4 * a.far_blocks) + slot) * 2 * 32 + col) * D + 4 * hi;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
@@ -680,25 +681,33 @@ __global__ __launch_bounds__(256, bwd_waves(D)) void window_dkv_kernel(WinArgs a
     }
 }
 
-// the partial sums of a sink block (32 keys) in slot order -> its rows of dK and dV; one workgroup per (block, head, 8 keys)
+// The partial sums of a sink block (32 keys) -> its rows of dK and dV.  A workgroup takes one of dK, dV for 1024 / D keys;
+// four threads share a sum, each every fourth slot in ascending order, and are added in their order.
 template <int FMT, int D>
-__global__ __launch_bounds__(256) void window_sink_kernel(WinArgs a) {
+__global__ __launch_bounds__(1024) void window_sink_kernel(WinArgs a) {
+    constexpr int KEYS = 1024 / D, PARTS = 32 / KEYS;
+    __shared__ f32x4 red[3][256];
     const int sink_blocks = (a.sinks + 31) / 32, slots = 1 + 4 * a.far_blocks;
-    const int kq = blockIdx.x & 3, n = blockIdx.x >> 2, blk = n % sink_blocks, bh = n / sink_blocks, b = bh / a.Hk, hk = bh % a.Hk;
+    const int which = blockIdx.x & 1, part = (blockIdx.x >> 1) % PARTS, n = (blockIdx.x >> 1) / PARTS, blk = n % sink_blocks,
+              bh = n / sink_blocks, b = bh / a.Hk, hk = bh % a.Hk;
     const int len = frames_of(a, b);
-    for (int i = threadIdx.x; i < 2 * 8 * D / 4; i += 256) {
-        const int which = i / (8 * D / 4), at = i % (8 * D / 4), kl = kq * 8 + at / (D / 4), c = (at % (D / 4)) * 4;
-        const int key = blk * 32 + kl;
-        if (key >= a.T) continue;
-        const float* src = a.part + (((long)n * slots * 2 + which) * 32 + kl) * D + c;
-        f32x4 s = {0.f, 0.f, 0.f, 0.f};
-        if (key < len)
-            for (int j = 0; j < slots; ++j) s += *reinterpret_cast<const f32x4*>(src + (long)j * 2 * 32 * D);
-        const HeadOut& d = which ? a.dv : a.dk;
-        typedef __attribute__((ext_vector_type(2))) uint32_t u32x2_t;
-        *reinterpret_cast<u32x2_t*>(d.p + b * d.b + hk * d.h + (long)key * d.r + c) =
-            u32x2_t{Op<FMT>::pack2(s[0], s[1]), Op<FMT>::pack2(s[2], s[3])};
+    const int at = threadIdx.x & 255, sg = threadIdx.x >> 8, kl = part * KEYS + at / (D / 4), c = (at % (D / 4)) * 4;
+    const int key = blk * 32 + kl, mine = key < a.sinks ? slots : 1;
+    const float* src = a.part + (((long)n * slots * 2 + which) * 32 + kl) * D + c;
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    if (key < len) {
+#pragma unroll 8
+        for (int j = sg; j < mine; j += 4) s += *reinterpret_cast<const f32x4*>(src + (long)j * 2 * 32 * D);
     }
+    if (sg) red[sg - 1][at] = s;
+    __syncthreads();
+    if (sg || key >= a.T) return;
+#pragma unroll
+    for (int j = 0; j < 3; ++j) s += red[j][at];
+    const HeadOut& d = which ? a.dv : a.dk;
+    typedef __attribute__((ext_vector_type(2))) uint32_t u32x2_t;
+    *reinterpret_cast<u32x2_t*>(d.p + b * d.b + hk * d.h + (long)key * d.r + c) =
+        u32x2_t{Op<FMT>::pack2(s[0], s[1]), Op<FMT>::pack2(s[2], s[3])};
 }
 
 constexpr int FAR_CHUNK = 1024;
@@ -755,7 +764,7 @@ hipError_t launch_bwd(const WinArgs& a, hipStream_t s) {
     hipLaunchKernelGGL((window_dq_kernel<FMT, D>), dim3((unsigned)(a.B * a.Hq * a.tiles)), dim3(256), 4 * 8192, s, a);
     hipLaunchKernelGGL((window_dkv_kernel<FMT, D>), dim3((unsigned)(a.B * a.Hk * (a.tiles + sb * a.far_blocks))), dim3(256),
                        2 * (2 * 8192 + 2 * tile_rows(D) * 4), s, a);
-    if (a.far_blocks > 0) hipLaunchKernelGGL((window_sink_kernel<FMT, D>), dim3(a.B * a.Hk * sb * 4), dim3(256), 0, s, a);
+    if (a.far_blocks > 0) hipLaunchKernelGGL((window_sink_kernel<FMT, D>), dim3(a.B * a.Hk * sb * (D / 16)), dim3(1024), 0, s, a);
     return hipGetLastError();
 }
 

@@ -17,6 +17,8 @@ namespace slsmi {
 namespace {
 
 constexpr int ST_WAVES = 4;
+constexpr int MAX_SPLITS = 128;   // workgroups that share a (stream, key head)
+constexpr int MIN_SLOTS = 512;    // per workgroup
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct StepArgs {
@@ -29,7 +31,8 @@ struct StepArgs {
     const float* wq;       // null: q and k come normalised and turned already
     const float* wk;
     const double* freqs;
-    float* ws;             // [B][Hq][splits][D + 2]
+    float* ml;             // [B][Hq][splits][2]: maximum and sum of a share
+    float* acc;            // [B][Hq][splits][D]: its weighted values
     float eps, scale;
     int half, interleaved;
     int Hq, Hk, slots, sinks;
@@ -52,14 +55,13 @@ __global__ __launch_bounds__(ST_WAVES * 64) void window_step_kernel(StepArgs a) 
     const long long pos = a.positions[b];
     const int s0 = split * a.per_split, s1 = min(s0 + a.per_split, a.slots);
     const int n = pos < 0 ? 0 : (int)min(pos + 1, (long long)a.slots);
-    float* const wsp = a.ws + (((long)b * a.Hq + hk * grp + g0) * a.splits + split) * (D + 2);
+    const long share = ((long)b * a.Hq + hk * grp + g0) * a.splits + split;
     if (s0 >= n) {   // nothing here (also: no frame for this stream)
         if (a.splits == 1) {
             for (int i = tid; i < GP * D; i += ST_WAVES * 64)
                 if (g0 + i / D < grp) a.out[((long)b * a.Hq + hk * grp + g0) * D + i] = 0;
         } else if (tid < GP && g0 + tid < grp) {
-            wsp[(long)tid * a.splits * (D + 2) + D] = -INFINITY;
-            wsp[(long)tid * a.splits * (D + 2) + D + 1] = 0.f;
+            *reinterpret_cast<f32x2*>(a.ml + (share + (long)tid * a.splits) * 2) = f32x2{-INFINITY, 0.f};
         }
         return;
     }
@@ -230,32 +232,60 @@ __global__ __launch_bounds__(ST_WAVES * 64) void window_step_kernel(StepArgs a) 
         if (a.splits == 1) {
             a.out[((long)b * a.Hq + hk * grp + g0 + i) * D + d] = Op<FMT>::pack(acc / sum);
         } else {
-            float* dst = wsp + (long)i * a.splits * (D + 2);
-            dst[d] = acc;
-            if (d == 0) {
-                dst[D] = mx;
-                dst[D + 1] = sum;
-            }
+            a.acc[(share + (long)i * a.splits) * D + d] = acc;
+            if (d == 0) *reinterpret_cast<f32x2*>(a.ml + (share + (long)i * a.splits) * 2) = f32x2{mx, sum};
         }
     }
 }
 
-// joins the workgroups that shared a stream's axis, in their order
+// Joins the shares of one query head: a wave forms the shares' weights, then D / 4 threads times 1024 / D groups of shares
+// (every (1024 / D)th, in order) sum the values, and the groups are added in their order.
 template <int FMT, int D>
-__global__ __launch_bounds__(D) void window_step_join_kernel(const float* __restrict__ ws, bf16_t* __restrict__ out, int splits) {
-    const float* p = ws + (long)blockIdx.x * splits * (D + 2);
-    const int d = threadIdx.x;
-    float mx = -INFINITY;
-    for (int s = 0; s < splits; ++s) mx = fmaxf(mx, p[(long)s * (D + 2) + D]);
-    float sum = 0.f, acc = 0.f;
-    for (int s = 0; s < splits; ++s) {
-        const float* r = p + (long)s * (D + 2);
-        if (r[D + 1] == 0.f) continue;   // an empty share: its sums were not written
-        const float corr = __builtin_amdgcn_exp2f(r[D] - mx);
-        sum = fmaf(r[D + 1], corr, sum);
-        acc = fmaf(r[d], corr, acc);
+__global__ __launch_bounds__(256) void window_step_join_kernel(const float* __restrict__ ml, const float* __restrict__ acc,
+                                                               bf16_t* __restrict__ out, int splits) {
+    constexpr int G = 1024 / D, C = D / 4;
+    __shared__ float wt[MAX_SPLITS];
+    __shared__ float total;
+    __shared__ f32x4 red[G][C];
+    const int tid = threadIdx.x;
+    if (tid < 64) {
+        float mx = -INFINITY, m[MAX_SPLITS / 64], l[MAX_SPLITS / 64];
+#pragma unroll
+        for (int i = 0; i < MAX_SPLITS / 64; ++i) {
+            const int s = tid + 64 * i;
+            const f32x2 v = s < splits ? *reinterpret_cast<const f32x2*>(ml + ((long)blockIdx.x * splits + s) * 2) : f32x2{-INFINITY, 0.f};
+            m[i] = v[0];
+            l[i] = v[1];
+            mx = fmaxf(mx, m[i]);
+        }
+        mx = wave_max(mx);
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < MAX_SPLITS / 64; ++i) {
+            const float w = __builtin_amdgcn_exp2f(m[i] - (mx == -INFINITY ? 0.f : mx));
+            sum = fmaf(l[i], w, sum);
+            wt[tid + 64 * i] = l[i] == 0.f ? 0.f : w;   // an empty share: its values were not written
+        }
+        sum = wave_sum(sum);
+        if (tid == 0) total = sum;
     }
-    out[(long)blockIdx.x * D + d] = Op<FMT>::pack(sum == 0.f ? 0.f : acc / sum);
+    __syncthreads();
+    const int c = tid % C, g = tid / C;
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = g; i < splits; i += G) {
+        const float w = wt[i];
+        if (w != 0.f) s += w * *reinterpret_cast<const f32x4*>(acc + ((long)blockIdx.x * splits + i) * D + c * 4);
+    }
+    red[g][c] = s;
+    __syncthreads();
+    if (g) return;
+#pragma unroll
+    for (int i = 1; i < G; ++i) s += red[i][c];
+    const float inv = total == 0.f ? 0.f : 1.0f / total;
+    typedef __attribute__((ext_vector_type(2))) uint32_t u32x2_t;
+    *reinterpret_cast<u32x2_t*>(out + (long)blockIdx.x * D + c * 4) =
+        u32x2_t{Op<FMT>::pack2(s[0] * inv, s[1] * inv), Op<FMT>::pack2(s[2] * inv, s[3] * inv)};
 }
 
 // k, v [B][T] heads -> the slots their newest positions live in; slots without a position keep what they hold
@@ -286,14 +316,12 @@ __global__ __launch_bounds__(256) void window_fill_kernel(FillArgs a) {
     *reinterpret_cast<u16x8*>(a.vc + dst) = *reinterpret_cast<const u16x8*>(a.v + b * a.vb + hk * a.vh + (long)pos * a.vr + c * 8);
 }
 
-// How many workgroups share a (stream, key head): enough to give every CU two, none with fewer than 128 slots.
+// How many workgroups share a (stream, key head): enough to give every CU two, none with fewer than MIN_SLOTS slots --
+// the join is a launch of its own (about 3 us), which is what one workgroup takes for a few hundred slots.
 int step_splits(int B, int heads, int slots) {
-    const long have = (long)B * heads;
-    long want = (512 + have - 1) / have;
-    const long most = (slots + 127) / 128;
-    if (want > most) want = most;
-    if (want > 64) want = 64;
-    return want < 1 ? 1 : (int)want;
+    const long have = (long)B * heads, want = (512 + have - 1) / have;
+    const long most = slots / MIN_SLOTS < MAX_SPLITS ? slots / MIN_SLOTS : MAX_SPLITS;
+    return (int)(want < most ? want : (most > 1 ? most : 1));
 }
 
 // query heads a workgroup serves at once
@@ -324,17 +352,21 @@ void launch_step_one(int gp, dim3 grid, hipStream_t s, const StepArgs& a) {
 
 }  // namespace
 
+static size_t step_ml_bytes(const WindowStepParams& p, int splits) {
+    return ((size_t)p.B * p.Hq * splits * 2 * sizeof(float) + 15) & ~(size_t)15;
+}
+
 size_t window_step_workspace(const WindowStepParams& p) {
     if (!step_ok(p) || p.B == 0) return 0;
     const int splits = step_splits(p.B, p.Hk * step_qblocks(p), p.slots);
-    return splits > 1 ? (size_t)p.B * p.Hq * splits * (p.D + 2) * sizeof(float) : 0;
+    return splits > 1 ? step_ml_bytes(p, splits) + (size_t)p.B * p.Hq * splits * p.D * sizeof(float) : 0;
 }
 
 hipError_t launch_window_step(const WindowStepParams& p, void* ws, size_t ws_bytes, hipStream_t s) {
     if (!step_ok(p)) return hipErrorInvalidValue;
     if (p.B == 0) return hipSuccess;
     auto al = [](const void* x) { return x && ((uintptr_t)x & 15) == 0; };
-    if (!al(p.qkv) || !al(p.k_cache) || !al(p.v_cache) || !p.positions || !p.out || p.ld % 8) return hipErrorInvalidValue;
+    if (!al(p.qkv) || !al(p.k_cache) || !al(p.v_cache) || !p.positions || !al(p.out) || p.ld % 8) return hipErrorInvalidValue;
     if (p.B > 1 && p.ld < (long)(p.Hq + 2 * p.Hk) * p.D) return hipErrorInvalidValue;
     if ((p.wq == nullptr) != (p.wk == nullptr) || !(p.scale > 0.f)) return hipErrorInvalidValue;
     if (p.half < 0 || 2 * p.half > p.D || p.half % 8 || (p.half > 0 && (!p.freqs || !p.wq))) return hipErrorInvalidValue;
@@ -345,7 +377,8 @@ hipError_t launch_window_step(const WindowStepParams& p, void* ws, size_t ws_byt
     a.qblocks = step_qblocks(p);
     a.splits = step_splits(p.B, p.Hk * a.qblocks, p.slots);
     a.per_split = ((p.slots + a.splits - 1) / a.splits + 31) / 32 * 32;
-    a.ws = reinterpret_cast<float*>(ws);
+    a.ml = reinterpret_cast<float*>(ws);
+    a.acc = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + step_ml_bytes(p, a.splits));
     if (a.splits > 1 && (!al(ws) || ws_bytes < window_step_workspace(p))) return hipErrorOutOfMemory;
     const int gp = step_heads(p.Hq / p.Hk);
     const dim3 grid(a.splits, p.Hk * a.qblocks, p.B);
@@ -353,8 +386,8 @@ hipError_t launch_window_step(const WindowStepParams& p, void* ws, size_t ws_byt
         if (p.D == 64) launch_step_one<F, 64>(gp, grid, s, a);
         else launch_step_one<F, 128>(gp, grid, s, a);
         if (a.splits > 1) {
-            if (p.D == 64) hipLaunchKernelGGL((window_step_join_kernel<F, 64>), dim3(p.B * p.Hq), dim3(64), 0, s, a.ws, a.out, a.splits);
-            else hipLaunchKernelGGL((window_step_join_kernel<F, 128>), dim3(p.B * p.Hq), dim3(128), 0, s, a.ws, a.out, a.splits);
+            if (p.D == 64) hipLaunchKernelGGL((window_step_join_kernel<F, 64>), dim3(p.B * p.Hq), dim3(256), 0, s, a.ml, a.acc, a.out, a.splits);
+            else hipLaunchKernelGGL((window_step_join_kernel<F, 128>), dim3(p.B * p.Hq), dim3(256), 0, s, a.ml, a.acc, a.out, a.splits);
         }
     });
     return hipGetLastError();
