@@ -69,14 +69,18 @@ __global__ __launch_bounds__(QN_WAVES * 64) void qk_norm_rope_kernel(QkNormArgs 
     const int h0 = blockIdx.y * a.heads_per_wave, h1 = min(h0 + a.heads_per_wave, H);
     const bf16_t* x = a.x + row * a.ldx + c * 8;
     bf16_t* y = a.y + row * a.ldy + c * 8;
+    constexpr int U = 4;   // heads in flight per lane
+    u16x8 v[U];
+    auto request = [&](int h) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const u16x8*>(x + (long)min(h + u * HW, H - 1) * D);
+    };
+    request(h0 + g);   // (on their way while the angles are computed)
     const NormLane t = norm_lane<D>(lane, row_position(a, row), a.freqs, a.half, a.interleaved, tab[wave]);
     float wq[8], wk[8], pwq[8], pwk[8];
     lane_weights<D>(a, c, t.partner & (GL - 1), wq, wk, pwq, pwk);
-    constexpr int U = 4;   // heads in flight per lane
     for (int h = h0 + g; h - g < h1; h += U * HW) {
-        u16x8 v[U];
-#pragma unroll
-        for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const u16x8*>(x + (long)min(h + u * HW, H - 1) * D);
+        if (h - g > h0) request(h);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int hh = h + u * HW;
@@ -117,23 +121,27 @@ __global__ __launch_bounds__(QN_WAVES * 64) void qk_norm_rope_bwd_kernel(QkNormA
         wk[e] = a.wk[c * 8 + e];
     }
     for (long row = (long)blockIdx.x * QN_WAVES + wave; row < a.rows; row += (long)gridDim.x * QN_WAVES) {
-        const NormLane t = norm_lane<D>(lane, row_position(a, row), a.freqs, a.half, a.interleaved, tab[wave]);
         const bf16_t* x = a.x + row * a.ldx + c * 8;
         const bf16_t* dy = a.dy + row * a.lddy + c * 8;
         bf16_t* y = a.y + row * a.ldy + c * 8;
-        constexpr int U = 2;
-        for (int h = g; h - g < H; h += U * HW) {
-            u16x8 xv[U], dv[U];
+        constexpr int U = 4;
+        u16x8 xv[U], dv[U];
+        auto request = [&](int h) {
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const long at = (long)min(h + u * HW, H - 1) * D;
                 xv[u] = *reinterpret_cast<const u16x8*>(x + at);
                 dv[u] = *reinterpret_cast<const u16x8*>(dy + at);
             }
+        };
+        request(g);
+        const NormLane t = norm_lane<D>(lane, row_position(a, row), a.freqs, a.half, a.interleaved, tab[wave]);
+        for (int h = g; h - g < H; h += U * HW) {
+            if (h > g) request(h);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                const int hh = h + u * HW;
-                const bool isq = hh < a.Hq, live = hh < H;
+                const int hh = h + u * HW, hb = hh - g;   // hb: the wave's first head
+                if (hb >= H) break;
                 const float r = head_rstd<FMT, D>(xv[u], a.eps);
                 const u16x8 pd = lane_exchange(dv[u], t.partner);
                 float dn[8], xh[8];
@@ -150,27 +158,41 @@ __global__ __launch_bounds__(QN_WAVES * 64) void qk_norm_rope_bwd_kernel(QkNormA
                         dn[e + 1] = q * t.cs[e] - p * t.sn[e];
                     }
                 } else if (t.role != 0) {
+                    const float sign = t.role == 1 ? 1.f : -1.f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) dn[e] = dn[e] * t.cs[e] + Op<FMT>::unpack(pd[e]) * (sign * t.sn[e]);
+                }
+                // dn <- dn w, and the weights' sums; a wave's heads are all queries, all keys, or (one of a row's) both
+                float dot = 0.f;
+                auto weigh = [&](const float(&w)[8], float(&gw)[8]) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const float o = Op<FMT>::unpack(pd[e]);
-                        dn[e] = t.role == 1 ? dn[e] * t.cs[e] + o * t.sn[e] : dn[e] * t.cs[e] - o * t.sn[e];
+                        gw[e] = fmaf(dn[e], xh[e], gw[e]);
+                        dn[e] *= w[e];
+                        dot = fmaf(dn[e], xh[e], dot);
+                    }
+                };
+                if (hb + HW <= a.Hq) {
+                    weigh(wq, gq);
+                } else if (hb >= a.Hq && hb + HW <= H) {
+                    weigh(wk, gk);
+                } else {
+                    const bool isq = hh < a.Hq, isk = !isq && hh < H;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float dw = dn[e] * xh[e];
+                        gq[e] += isq ? dw : 0.f;
+                        gk[e] += isk ? dw : 0.f;
+                        dn[e] *= isq ? wq[e] : wk[e];
+                        dot = fmaf(dn[e], xh[e], dot);
                     }
                 }
-                float dot = 0.f, gn[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    gn[e] = dn[e] * (isq ? wq[e] : wk[e]);
-                    dot = fmaf(gn[e], xh[e], dot);
-                    const float dw = dn[e] * xh[e];
-                    gq[e] += live && isq ? dw : 0.f;
-                    gk[e] += live && !isq ? dw : 0.f;
-                }
                 dot = lane_group_sum<GL>(dot) * (1.0f / D);
-                if (live) {
+                if (hh < H) {
                     u32x4 o;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        o[i] = Op<FMT>::pack2(r * (gn[2 * i] - xh[2 * i] * dot), r * (gn[2 * i + 1] - xh[2 * i + 1] * dot));
+                        o[i] = Op<FMT>::pack2(r * (dn[2 * i] - xh[2 * i] * dot), r * (dn[2 * i + 1] - xh[2 * i + 1] * dot));
                     *reinterpret_cast<u32x4*>(y + (long)hh * D) = o;
                 }
             }
@@ -237,10 +259,11 @@ QkNormArgs qk_norm_args(const QkNormParams& p) {
     return a;
 }
 
-// workgroups of the backward: up to four per CU, so that a wave's partial sums cover several rows of a large batch
+// workgroups of the backward: at most six per CU, so that a wave's partial sums cover several rows of a large batch, and
+// every wave the same number of rows
 int qk_norm_bwd_blocks(long rows) {
-    const long b = (rows + QN_WAVES - 1) / QN_WAVES;
-    return (int)(b < 1024 ? b : 1024);
+    const long waves = 1536 * QN_WAVES, per_wave = (rows + waves - 1) / waves;
+    return (int)((rows + per_wave * QN_WAVES - 1) / (per_wave * QN_WAVES));
 }
 
 }  // namespace

@@ -40,8 +40,8 @@ struct WinArgs {
     HeadPtr q, k, v, o, d;   // o, d (dO): backward
     HeadOut out, dq, dk, dv;
     float* lse;              // [B][Hq][T]
-    float* delta;            // [B][Hq][T]: rowsum(dO o O), written by the dQ kernel
-    float* part;             // sink keys' partial sums (see window_dkv_kernel)
+    float* delta;            // [B][Hq][T]: rowsum(dO o O)
+    float* part;             // sink keys' partial sums (see window_dkv)
     const int* nframes;
     int B, T, Hq, Hk;
     int left, right, sinks;  // left, right in [0, T]; sinks in [0, SINK_MAX]
@@ -404,21 +404,36 @@ __global__ __launch_bounds__(256, fwd_waves(D)) void window_fwd_kernel(WinArgs a
     }
 }
 
-// ---- backward, queries: dQ and delta = rowsum(dO o O); the forward's loop with P recomputed from lse.  The product
-// dO V^T starts from -delta, so dP - delta leaves the matrix units.
+// ---- backward, first launch: delta = rowsum(dO o O).  D / 8 lanes hold a (row, head), 16 bytes of both each.
 template <int FMT, int D>
-__global__ __launch_bounds__(256, bwd_waves(D)) void window_dq_kernel(WinArgs a) {
+__global__ __launch_bounds__(256) void window_delta_kernel(WinArgs a) {
+    constexpr int GL = D / 8;
+    const long i = (long)blockIdx.x * (256 / GL) + threadIdx.x / GL, rows = (long)a.T * a.Hq;   // row-major [T][Hq]
+    const int b = blockIdx.y, c = (threadIdx.x & (GL - 1)) * 8;
+    if (i >= rows) return;   // whole lane groups leave
+    const int q = (int)(i / a.Hq), h = (int)(i % a.Hq);
+    if (q >= frames_of(a, b)) return;   // (never read)
+    const u16x8 x = *reinterpret_cast<const u16x8*>(a.d.p + b * a.d.b + h * a.d.h + (long)q * a.d.r + c);
+    const u16x8 y = *reinterpret_cast<const u16x8*>(a.o.p + b * a.o.b + h * a.o.h + (long)q * a.o.r + c);
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s = fmaf(Op<FMT>::unpack(x[e]), Op<FMT>::unpack(y[e]), s);
+    s = lane_group_sum<GL>(s);
+    if (c == 0) a.delta[((long)b * a.Hq + h) * a.T + q] = s;
+}
+
+// ---- backward, queries: dQ; the forward's loop with P recomputed from lse.  The product dO V^T starts from -delta, so
+// dP - delta leaves the matrix units.
+template <int FMT, int D>
+__device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* lds) {
     constexpr int BN = tile_rows(D), NS = D / 16, DT = D / 32, TILE = BN * D * 2;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, hi = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const unsigned w = xcd_order(blockIdx.x, gridDim.x);
     const int tile = a.tiles - 1 - (int)(w % a.tiles);
     const int bh = w / a.tiles, b = bh / a.Hq, h = bh % a.Hq, hk = h / (a.Hq / a.Hk);
     const int len = frames_of(a, b);
     const int q0 = tile * 128, qw = q0 + wave * 32, q = qw + col;
     bf16_t* const dqrow = a.dq.p + b * a.dq.b + h * a.dq.h + (long)q * a.dq.r;
-    float* const drow = a.delta + (long)bh * a.T + q;
     if (q0 >= len) {
         if (q < a.T) {
 #pragma unroll
@@ -434,26 +449,20 @@ __global__ __launch_bounds__(256, bwd_waves(D)) void window_dq_kernel(WinArgs a)
     lk.issue(kh, a.k.r, kt.tile(0) * BN, len, lds, wave);
     lv.issue(vh, a.v.r, kt.tile(0) * BN, len, lds + TILE, wave);
     u16x8 qf[NS], df[NS];
-    float delta = 0.f;
     {
         const int row = min(q, len - 1);
         const bf16_t* qr = a.q.p + b * a.q.b + h * a.q.h + (long)row * a.q.r + hi * 8;
         const bf16_t* dr = a.d.p + b * a.d.b + h * a.d.h + (long)row * a.d.r + hi * 8;
-        const bf16_t* pr = a.o.p + b * a.o.b + h * a.o.h + (long)row * a.o.r + hi * 8;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
             qf[s] = *reinterpret_cast<const u16x8*>(qr + s * 16);
             df[s] = *reinterpret_cast<const u16x8*>(dr + s * 16);
-            const u16x8 of = *reinterpret_cast<const u16x8*>(pr + s * 16);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) delta = fmaf(Op<FMT>::unpack(df[s][e]), Op<FMT>::unpack(of[e]), delta);
         }
-        delta = halves_sum(delta);
     }
     const bool live = q < len;
-    if (live && hi == 0) *drow = delta;
     const float sc = a.scale * LOG2E;
-    const float ls = a.lse[(long)bh * a.T + min(q, len - 1)] * LOG2E;
+    const long stat = (long)bh * a.T + min(q, len - 1);
+    const float ls = a.lse[stat] * LOG2E, delta = a.delta[stat];
     f32x16 acc[DT], start;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt] = zero16();
@@ -515,14 +524,12 @@ __global__ __launch_bounds__(256, bwd_waves(D)) void window_dq_kernel(WinArgs a)
 // Their sums for the sinks' rows, and the near workgroup's for all rows of the block, go as fp32 to `part`
 // [B][Hk][sink block][1 + 4 far_blocks][dK, dV][32 keys][D] and are added in that order by window_sink_kernel.
 template <int FMT, int D>
-__global__ __launch_bounds__(256, bwd_waves(D)) void window_dkv_kernel(WinArgs a) {
-    constexpr int NS = D / 16, DT = D / 32, BQ = tile_rows(D), TILE = BQ * D * 2, BUF = 2 * TILE + 2 * BQ * 4;
-    extern __shared__ __attribute__((aligned(16))) char lds[];   // two buffers of Q, dO, -lse / scale, -delta
+__device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* lds) {
+    constexpr int NS = D / 16, DT = D / 32, BQ = tile_rows(D), TILE = BQ * D * 2, BUF = 2 * TILE + 2 * BQ * 4;   // Q, dO, -lse / scale, -delta
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, hi = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int sink_blocks = (a.sinks + 31) / 32;
     const int per_head = a.tiles + sink_blocks * a.far_blocks;
-    const unsigned w = xcd_order(blockIdx.x, gridDim.x);
     const int bh = w / per_head, item = w % per_head, b = bh / a.Hk, hk = bh % a.Hk;
     const int len = frames_of(a, b);
     const int grp = a.Hq / a.Hk;
@@ -681,6 +688,18 @@ __global__ __launch_bounds__(256, bwd_waves(D)) void window_dkv_kernel(WinArgs a
     }
 }
 
+// Both sides of the backward in one launch: the key-side workgroups (the longer ones) first, the query-side ones behind
+// them fill the CUs that these leave.  The key side's count is rounded up to the XCDs, so that both have their order.
+template <int FMT, int D>
+__global__ __launch_bounds__(256, bwd_waves(D)) void window_bwd_kernel(WinArgs a, unsigned key_side, unsigned key_blocks) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    if (blockIdx.x < key_blocks) {
+        if (blockIdx.x < key_side) window_dkv<FMT, D>(a, xcd_order(blockIdx.x, key_side), lds);
+    } else {
+        window_dq<FMT, D>(a, xcd_order(blockIdx.x - key_blocks, gridDim.x - key_blocks), lds);
+    }
+}
+
 // The partial sums of a sink block (32 keys) -> its rows of dK and dV.  A workgroup takes one of dK, dV for 1024 / D keys;
 // four threads share a sum, each every fourth slot in ascending order, and are added in their order.
 template <int FMT, int D>
@@ -730,7 +749,7 @@ bool head_ok(const WindowHeads& x, int heads, int T, int D) {
 
 // the ranges every call has to keep; clamps the window
 bool window_args(const WindowParams& p, WinArgs& a) {
-    if (p.B < 0 || p.T < 0 || p.T > (1 << 29) || p.Hk < 1 || p.Hq < p.Hk || p.Hq % p.Hk || p.Hq > 4096) return false;
+    if (p.B < 0 || p.B > 65535 || p.T < 0 || p.T > (1 << 29) || p.Hk < 1 || p.Hq < p.Hk || p.Hq % p.Hk || p.Hq > 4096) return false;
     if (p.D != 64 && p.D != 128) return false;
     if (p.fmt != FMT_BF16 && p.fmt != FMT_F16) return false;
     if (!(p.scale > 0.f) || p.left < -1 || p.right < -1 || p.sinks < 0 || p.sinks > SINK_MAX) return false;
@@ -761,9 +780,10 @@ hipError_t launch_fwd(const WinArgs& a, hipStream_t s) {
 template <int FMT, int D>
 hipError_t launch_bwd(const WinArgs& a, hipStream_t s) {
     const int sb = (a.sinks + 31) / 32;
-    hipLaunchKernelGGL((window_dq_kernel<FMT, D>), dim3((unsigned)(a.B * a.Hq * a.tiles)), dim3(256), 4 * 8192, s, a);
-    hipLaunchKernelGGL((window_dkv_kernel<FMT, D>), dim3((unsigned)(a.B * a.Hk * (a.tiles + sb * a.far_blocks))), dim3(256),
-                       2 * (2 * 8192 + 2 * tile_rows(D) * 4), s, a);
+    const unsigned ks = a.B * a.Hk * (a.tiles + sb * a.far_blocks), kb = (ks + 7) & ~7u, qs = a.B * a.Hq * a.tiles;
+    const long rows = (long)a.T * a.Hq, per = 256 / (D / 8);
+    hipLaunchKernelGGL((window_delta_kernel<FMT, D>), dim3((unsigned)((rows + per - 1) / per), a.B), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((window_bwd_kernel<FMT, D>), dim3(kb + qs), dim3(256), 2 * (2 * 8192 + 2 * tile_rows(D) * 4), s, a, ks, kb);
     if (a.far_blocks > 0) hipLaunchKernelGGL((window_sink_kernel<FMT, D>), dim3(a.B * a.Hk * sb * (D / 16)), dim3(1024), 0, s, a);
     return hipGetLastError();
 }
