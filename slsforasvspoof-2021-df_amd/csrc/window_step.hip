@@ -18,7 +18,7 @@ namespace {
 
 constexpr int ST_WAVES = 4;
 constexpr int MAX_SPLITS = 128;   // workgroups that share a (stream, key head)
-constexpr int MIN_SLOTS = 512;    // per workgroup
+constexpr int MIN_SLOTS = 128;    // per workgroup, where an axis is shared
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct StepArgs {
@@ -316,12 +316,14 @@ __global__ __launch_bounds__(256) void window_fill_kernel(FillArgs a) {
     *reinterpret_cast<u16x8*>(a.vc + dst) = *reinterpret_cast<const u16x8*>(a.v + b * a.vb + hk * a.vh + (long)pos * a.vr + c * 8);
 }
 
-// How many workgroups share a (stream, key head): enough to give every CU two, none with fewer than MIN_SLOTS slots --
-// the join is a launch of its own (about 3 us), which is what one workgroup takes for a few hundred slots.
-int step_splits(int B, int heads, int slots) {
-    const long have = (long)B * heads, want = (512 + have - 1) / have;
-    const long most = slots / MIN_SLOTS < MAX_SPLITS ? slots / MIN_SLOTS : MAX_SPLITS;
-    return (int)(want < most ? want : (most > 1 ? most : 1));
+// How many workgroups share a (stream, key head).  The join is a launch of its own: up to 512 slots of 64 channels (or the
+// same bytes) one workgroup is faster alone (one stream, 16 heads x 64, graph replay: 5.0 against 6.6 us at 512 slots, 10.1
+// against 6.7 at 2048).  Beyond that, enough to give every CU two, none with fewer than 128 slots.
+int step_splits(int B, int heads, int slots, int D) {
+    if ((long)slots * D <= 512 * 64) return 1;
+    const long have = (long)B * heads, want = (512 + have - 1) / have, most = (slots + MIN_SLOTS - 1) / MIN_SLOTS;
+    const long n = want < most ? want : most;
+    return (int)(n < MAX_SPLITS ? n : MAX_SPLITS);
 }
 
 // query heads a workgroup serves at once
@@ -358,7 +360,7 @@ static size_t step_ml_bytes(const WindowStepParams& p, int splits) {
 
 size_t window_step_workspace(const WindowStepParams& p) {
     if (!step_ok(p) || p.B == 0) return 0;
-    const int splits = step_splits(p.B, p.Hk * step_qblocks(p), p.slots);
+    const int splits = step_splits(p.B, p.Hk * step_qblocks(p), p.slots, p.D);
     return splits > 1 ? step_ml_bytes(p, splits) + (size_t)p.B * p.Hq * splits * p.D * sizeof(float) : 0;
 }
 
@@ -375,7 +377,7 @@ hipError_t launch_window_step(const WindowStepParams& p, void* ws, size_t ws_byt
     a.wq = p.wq; a.wk = p.wk; a.freqs = p.freqs; a.eps = p.eps; a.scale = p.scale; a.half = p.half;
     a.interleaved = p.interleaved; a.Hq = p.Hq; a.Hk = p.Hk; a.slots = p.slots; a.sinks = p.sinks;
     a.qblocks = step_qblocks(p);
-    a.splits = step_splits(p.B, p.Hk * a.qblocks, p.slots);
+    a.splits = step_splits(p.B, p.Hk * a.qblocks, p.slots, p.D);
     a.per_split = ((p.slots + a.splits - 1) / a.splits + 31) / 32 * 32;
     a.ml = reinterpret_cast<float*>(ws);
     a.acc = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + step_ml_bytes(p, a.splits));
