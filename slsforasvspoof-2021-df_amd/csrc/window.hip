@@ -41,6 +41,7 @@ struct WinArgs {
     HeadOut out, dq, dk, dv;
     float* lse;              // [B][Hq][T]
     float* delta;            // [B][Hq][T]: rowsum(dO o O)
+    float* dmax;             // [B][Hq][T / DELTA_ROWS]: largest |dO| (half precision)
     float* part;             // sink keys' partial sums (see window_dkv)
     const int* nframes;
     int B, T, Hq, Hk;
@@ -245,6 +246,28 @@ __device__ __forceinline__ u16x8 pack_step_unit(const f32x16& p, int s) {
                                            Op<FMT>::pack2_unit(p[8 * s + 4], p[8 * s + 5]), Op<FMT>::pack2_unit(p[8 * s + 6], p[8 * s + 7])});
 }
 
+// The same as the sum of two operands: dS to twice the mantissa.  Rounded once, dS and the rounding of the result each add
+// 2^-9 (2^-12) of the gradient, and rows of few keys, whose dS feels the rounding of O through delta, up to as much again.
+template <int FMT>
+__device__ __forceinline__ void split_step(const f32x16& p, int s, u16x8& hi, u16x8& lo) {
+    uint32_t h[4], l[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float a = p[8 * s + 2 * i], b = p[8 * s + 2 * i + 1];
+        if constexpr (FMT == FMT_F16) {   // towards zero: past the largest value it stays there
+            const auto t = __builtin_amdgcn_cvt_pkrtz(a, b);
+            h[i] = __builtin_bit_cast(uint32_t, t);
+            l[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a - (float)t[0], b - (float)t[1]));
+        } else {   // the upper halves of the words
+            const uint32_t x = __builtin_bit_cast(uint32_t, a), y = __builtin_bit_cast(uint32_t, b);
+            h[i] = __builtin_amdgcn_perm(y, x, 0x07060302);
+            l[i] = Op<FMT_BF16>::pack2(a - __builtin_bit_cast(float, x & 0xffff0000u), b - __builtin_bit_cast(float, y & 0xffff0000u));
+        }
+    }
+    hi = __builtin_bit_cast(u16x8, u32x4{h[0], h[1], h[2], h[3]});
+    lo = __builtin_bit_cast(u16x8, u32x4{l[0], l[1], l[2], l[3]});
+}
+
 __device__ __forceinline__ f32x16 zero16() {
     return f32x16{0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 }
@@ -404,22 +427,56 @@ __global__ __launch_bounds__(256, fwd_waves(D)) void window_fwd_kernel(WinArgs a
     }
 }
 
-// ---- backward, first launch: delta = rowsum(dO o O).  D / 8 lanes hold a (row, head), 16 bytes of both each.
+// ---- backward, first launch: delta = rowsum(dO o O) of DELTA_ROWS rows of a head per workgroup, and (half precision) the
+// largest |dO| among them.  D / 8 lanes hold a row, 16 bytes of both each.
+constexpr int DELTA_ROWS = 128;
+
 template <int FMT, int D>
 __global__ __launch_bounds__(256) void window_delta_kernel(WinArgs a) {
-    constexpr int GL = D / 8;
-    const long i = (long)blockIdx.x * (256 / GL) + threadIdx.x / GL, rows = (long)a.T * a.Hq;   // row-major [T][Hq]
-    const int b = blockIdx.y, c = (threadIdx.x & (GL - 1)) * 8;
-    if (i >= rows) return;   // whole lane groups leave
-    const int q = (int)(i / a.Hq), h = (int)(i % a.Hq);
-    if (q >= frames_of(a, b)) return;   // (never read)
-    const u16x8 x = *reinterpret_cast<const u16x8*>(a.d.p + b * a.d.b + h * a.d.h + (long)q * a.d.r + c);
-    const u16x8 y = *reinterpret_cast<const u16x8*>(a.o.p + b * a.o.b + h * a.o.h + (long)q * a.o.r + c);
-    float s = 0.f;
+    constexpr int GL = D / 8, PER = 256 / GL;
+    __shared__ float red[4];
+    const int b = blockIdx.z, h = blockIdx.y, c = (threadIdx.x & (GL - 1)) * 8;
+    const int len = frames_of(a, b);
+    const long bh = (long)b * a.Hq + h;
+    float top = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < DELTA_ROWS / PER; ++i) {
+        const int q = blockIdx.x * DELTA_ROWS + i * PER + threadIdx.x / GL, row = min(q, max(len - 1, 0));   // (a batch has a row 0)
+        const u16x8 x = *reinterpret_cast<const u16x8*>(a.d.p + b * a.d.b + h * a.d.h + (long)row * a.d.r + c);
+        const u16x8 y = *reinterpret_cast<const u16x8*>(a.o.p + b * a.o.b + h * a.o.h + (long)row * a.o.r + c);
+        float s = 0.f, m = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) s = fmaf(Op<FMT>::unpack(x[e]), Op<FMT>::unpack(y[e]), s);
-    s = lane_group_sum<GL>(s);
-    if (c == 0) a.delta[((long)b * a.Hq + h) * a.T + q] = s;
+        for (int e = 0; e < 8; ++e) {
+            const float d = Op<FMT>::unpack(x[e]);
+            s = fmaf(d, Op<FMT>::unpack(y[e]), s);
+            m = fmaxf(m, fabsf(d));
+        }
+        s = lane_group_sum<GL>(s);
+        if (q < len) {
+            top = fmaxf(top, m);
+            if (c == 0) a.delta[bh * a.T + q] = s;
+        }
+    }
+    if constexpr (FMT == FMT_F16) {
+        top = wave_max(top);
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+        __syncthreads();
+        if (threadIdx.x == 0) a.dmax[bh * gridDim.x + blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    }
+}
+
+// Half precision holds P and dS as c P and c dS: a power of two c >= 1 (as its logarithm) that brings the largest dO of the
+// query heads first .. first + n - 1 to about 2^4, so that neither long rows nor small gradients push them below the
+// format's normal range.  c comes out again with the scale of the result.  bfloat16 has the range: c = 1.
+template <int FMT>
+__device__ __forceinline__ float grad_lift(const WinArgs& a, long first, int n) {
+    if constexpr (FMT != FMT_F16) return 0.f;
+    const int parts = (a.T + DELTA_ROWS - 1) / DELTA_ROWS;
+    float top = 0.f;
+    for (int i = threadIdx.x & 63; i < parts * n; i += 64) top = fmaxf(top, a.dmax[first * parts + i]);
+    top = wave_max(top);
+    const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;   // 0: -127, infinity and NaN: 128
+    return (float)min(max(4 - e, 0), 15);
 }
 
 // ---- backward, queries: dQ; the forward's loop with P recomputed from lse.  The product dO V^T starts from -delta, so
@@ -462,7 +519,8 @@ __device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* ld
     const bool live = q < len;
     const float sc = a.scale * LOG2E;
     const long stat = (long)bh * a.T + min(q, len - 1);
-    const float ls = a.lse[stat] * LOG2E, delta = a.delta[stat];
+    const float lift = grad_lift<FMT>(a, bh, 1);
+    const float ls = a.lse[stat] * LOG2E - lift, delta = a.delta[stat];
     f32x16 acc[DT], start;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt] = zero16();
@@ -498,17 +556,22 @@ __device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* ld
             for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], sc, -ls)) * dp[r];
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
-                const u16x8 e = pack_step<FMT>(s, st);
+                u16x8 e, rest;
+                split_step<FMT>(s, st, e, rest);
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) acc[dt] = mfma32<FMT>(kt2[st][dt], e, acc[dt]);
+                for (int dt = 0; dt < DT; ++dt) {
+                    acc[dt] = mfma32<FMT>(kt2[st][dt], e, acc[dt]);
+                    acc[dt] = mfma32<FMT>(kt2[st][dt], rest, acc[dt]);
+                }
             }
         }
         if (more) tiles_landed();
     }
+    const float fin = a.scale * __builtin_amdgcn_exp2f(-lift);
     if (q < a.T) {
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-            const f32x16 v = live ? acc[dt] * a.scale : zero16();
+            const f32x16 v = live ? acc[dt] * fin : zero16();
             store_column<FMT, false>(dqrow, dt, v, hi);
         }
     }
@@ -523,7 +586,7 @@ __device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* ld
 // chunks of far_chunk, one workgroup each, whose four waves share the block's keys and take 32 of 128 queries in turn.
 // Their sums for the sinks' rows, and the near workgroup's for all rows of the block, go as fp32 to `part`
 // [B][Hk][sink block][1 + 4 far_blocks][dK, dV][32 keys][D] and are added in that order by window_sink_kernel.
-template <int FMT, int D>
+template <int FMT, int D, bool SPLIT>
 __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* lds) {
     constexpr int NS = D / 16, DT = D / 32, BQ = tile_rows(D), TILE = BQ * D * 2, BUF = 2 * TILE + 2 * BQ * 4;   // Q, dO, -lse / scale, -delta
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, hi = lane >> 5;
@@ -566,6 +629,7 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) ak[dt] = av[dt] = zero16();
     const float sc = a.scale * LOG2E, lsc = 1.0f / a.scale;
+    const float lift = grad_lift<FMT>(a, (long)b * a.Hq + hk * grp, grp), lift_sc = lift / sc;
     const int t0 = qa / BQ, nt = qb < qa ? 0 : qb / BQ - t0 + 1;
     const int total = nt * grp;
     const LaneAt<D> at(lane);
@@ -580,7 +644,7 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
             const int q = q0 + (tid & (BQ - 1));
             const long at = ((long)b * a.Hq + rh) * a.T + min(q, len - 1);
             const bool in = q >= qa && q <= qb;
-            stat = tid < BQ ? (in ? -a.lse[at] * lsc : -INFINITY) : (in ? -a.delta[at] : 0.f);
+            stat = tid < BQ ? (in ? fmaf(-a.lse[at], lsc, lift_sc) : -INFINITY) : (in ? -a.delta[at] : 0.f);
         }
         if (++rt == t0 + nt) {
             rt = t0;
@@ -645,18 +709,25 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
                 constexpr int OFF = decltype(off)::value;
                 u16x8 t[DT];
                 tr_frags<D, OFF>(q_at + TILE, at, t);
-                const u16x8 pf = pack_step_unit<FMT>(s, st), ef = pack_step<FMT>(dp, st);
+                const u16x8 pf = pack_step_unit<FMT>(s, st);
+                u16x8 ef, rest;
+                if constexpr (SPLIT) split_step<FMT>(dp, st, ef, rest);
+                else ef = pack_step<FMT>(dp, st);
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) av[dt] = mfma32<FMT>(t[dt], pf, av[dt]);
                 tr_frags<D, OFF>(q_at, at, t);
 #pragma unroll
-                for (int dt = 0; dt < DT; ++dt) ak[dt] = mfma32<FMT>(t[dt], ef, ak[dt]);
+                for (int dt = 0; dt < DT; ++dt) {
+                    ak[dt] = mfma32<FMT>(t[dt], ef, ak[dt]);
+                    if constexpr (SPLIT) ak[dt] = mfma32<FMT>(t[dt], rest, ak[dt]);
+                }
             };
             step(std::integral_constant<int, 0>{}, 0);
             step(std::integral_constant<int, 32 * D>{}, 1);
         }
         if (more) landed(next);
     }
+    const float vfin = __builtin_amdgcn_exp2f(-lift), kfin = a.scale * vfin;
     if (far || (k0w < a.sinks && a.far_blocks > 0)) {
         const int blk = far ? block : k0w / 32, slot = far ? 1 + chunk * 4 + wave : 0;
         if (far && key >= a.sinks) return;
@@ -668,8 +739,8 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
                 f32x4 x, y;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    x[j] = ak[dt][4 * g + j] * a.scale;
-                    y[j] = av[dt][4 * g + j];
+                    x[j] = ak[dt][4 * g + j] * kfin;
+                    y[j] = av[dt][4 * g + j] * vfin;
                 }
                 *reinterpret_cast<f32x4*>(dst + dt * 32 + 8 * g) = x;
                 *reinterpret_cast<f32x4*>(dst + 32 * D + dt * 32 + 8 * g) = y;
@@ -682,19 +753,19 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
         const bool live = key < len;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-            store_column<FMT, false>(dk, dt, live ? ak[dt] * a.scale : zero16(), hi);
-            store_column<FMT, false>(dv, dt, live ? av[dt] : zero16(), hi);
+            store_column<FMT, false>(dk, dt, live ? ak[dt] * kfin : zero16(), hi);
+            store_column<FMT, false>(dv, dt, live ? av[dt] * vfin : zero16(), hi);
         }
     }
 }
 
 // Both sides of the backward in one launch: the key-side workgroups (the longer ones) first, the query-side ones behind
 // them fill the CUs that these leave.  The key side's count is rounded up to the XCDs, so that both have their order.
-template <int FMT, int D>
+template <int FMT, int D, bool SPLIT>
 __global__ __launch_bounds__(256, bwd_waves(D)) void window_bwd_kernel(WinArgs a, unsigned key_side, unsigned key_blocks) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     if (blockIdx.x < key_blocks) {
-        if (blockIdx.x < key_side) window_dkv<FMT, D>(a, xcd_order(blockIdx.x, key_side), lds);
+        if (blockIdx.x < key_side) window_dkv<FMT, D, SPLIT>(a, xcd_order(blockIdx.x, key_side), lds);
     } else {
         window_dq<FMT, D>(a, xcd_order(blockIdx.x - key_blocks, gridDim.x - key_blocks), lds);
     }
@@ -767,6 +838,9 @@ bool window_args(const WindowParams& p, WinArgs& a) {
 HeadPtr in_head(const WindowHeads& x) { return {x.p, x.batch, x.row, x.head}; }
 HeadOut out_head(const WindowHeads& x) { return {const_cast<bf16_t*>(x.p), x.batch, x.row, x.head}; }
 
+size_t dmax_bytes(const WinArgs& a) {
+    return ((size_t)a.B * a.Hq * ((a.T + DELTA_ROWS - 1) / DELTA_ROWS) * sizeof(float) + 255) & ~(size_t)255;
+}
 size_t delta_bytes(const WinArgs& a) { return ((size_t)a.B * a.Hq * a.T * sizeof(float) + 255) & ~(size_t)255; }
 
 }  // namespace
@@ -777,13 +851,22 @@ hipError_t launch_fwd(const WinArgs& a, hipStream_t s) {
     return hipGetLastError();
 }
 
+// Whether dK's dS is split in two operands as well.  Against rounding everything once at the end, dK's error is 1.6 to 1.7
+// times larger with dS rounded once where rows see few keys (52 to 268 frames, or one side only: the early rows), 1.44 to
+// 1.49 from about 160 keys on both sides or 1024 on one; split it is 1.02 to 1.4, for 25 % of the key side's time.
+bool few_keys(const WinArgs& a) {
+    const int span = a.left + a.right + 1 + a.sinks, keys = span < a.T ? span : a.T;
+    return keys <= 160 || (a.right < a.left && a.T <= 1024);
+}
+
 template <int FMT, int D>
 hipError_t launch_bwd(const WinArgs& a, hipStream_t s) {
     const int sb = (a.sinks + 31) / 32;
     const unsigned ks = a.B * a.Hk * (a.tiles + sb * a.far_blocks), kb = (ks + 7) & ~7u, qs = a.B * a.Hq * a.tiles;
-    const long rows = (long)a.T * a.Hq, per = 256 / (D / 8);
-    hipLaunchKernelGGL((window_delta_kernel<FMT, D>), dim3((unsigned)((rows + per - 1) / per), a.B), dim3(256), 0, s, a);
-    hipLaunchKernelGGL((window_bwd_kernel<FMT, D>), dim3(kb + qs), dim3(256), 2 * (2 * 8192 + 2 * tile_rows(D) * 4), s, a, ks, kb);
+    hipLaunchKernelGGL((window_delta_kernel<FMT, D>), dim3((a.T + DELTA_ROWS - 1) / DELTA_ROWS, a.Hq, a.B), dim3(256), 0, s, a);
+    constexpr int LDS = 2 * (2 * 8192 + 2 * tile_rows(D) * 4);
+    if (few_keys(a)) hipLaunchKernelGGL((window_bwd_kernel<FMT, D, true>), dim3(kb + qs), dim3(256), LDS, s, a, ks, kb);
+    else hipLaunchKernelGGL((window_bwd_kernel<FMT, D, false>), dim3(kb + qs), dim3(256), LDS, s, a, ks, kb);
     if (a.far_blocks > 0) hipLaunchKernelGGL((window_sink_kernel<FMT, D>), dim3(a.B * a.Hk * sb * (D / 16)), dim3(1024), 0, s, a);
     return hipGetLastError();
 }
@@ -806,7 +889,7 @@ size_t window_attention_bwd_workspace(const WindowParams& p) {
     WinArgs a{};
     if (!window_args(p, a) || p.B == 0 || p.T == 0) return 0;
     const size_t fb = far_blocks_of(p.T, a.left, a.sinks), sb = (a.sinks + 31) / 32;
-    return delta_bytes(a) + (fb ? (size_t)p.B * p.Hk * sb * (1 + 4 * fb) * 2 * 32 * p.D * sizeof(float) : 0);
+    return delta_bytes(a) + dmax_bytes(a) + (fb ? (size_t)p.B * p.Hk * sb * (1 + 4 * fb) * 2 * 32 * p.D * sizeof(float) : 0);
 }
 
 hipError_t launch_window_attention_bwd(const WindowParams& p, const float* lse, const WindowHeads& dout, const WindowHeads& dq,
@@ -823,7 +906,8 @@ hipError_t launch_window_attention_bwd(const WindowParams& p, const float* lse, 
     a.dq = out_head(dq); a.dk = out_head(dk); a.dv = out_head(dv);
     a.lse = const_cast<float*>(lse);
     a.delta = reinterpret_cast<float*>(ws);
-    a.part = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + delta_bytes(a));
+    a.dmax = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + delta_bytes(a));
+    a.part = reinterpret_cast<float*>(reinterpret_cast<char*>(a.dmax) + dmax_bytes(a));
     a.far_chunk = FAR_CHUNK;
     a.far_blocks = far_blocks_of(p.T, a.left, a.sinks);
     hipError_t rc = hipSuccess;

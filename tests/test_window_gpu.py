@@ -556,3 +556,19 @@ def test_refusals():
         with pytest.raises(_lib.SlsmiError):
             f()
             print("not refused:", i)
+
+
+@pytest.mark.parametrize("power", [-14, -7, 6])
+def test_half_precision_gradients_follow_small_and_large_dout(power):
+    """Gradients are linear in dout: scaled by a power of two they keep their bits, but for what falls below half
+    precision's normal range (spacing 2^-24, so 2^-25 per rounding of the result, and of a 16-bit dout itself)."""
+    case = (1, 700, 2, 1, 64, None, 0, 0, None)
+    q, k, v, _ = win_case(*case, torch.float16)
+    do = rnd(1, 700, 2, 64, seed=9, dtype=torch.float16)
+    small = (do.float() * 2.0 ** power).to(torch.float16)
+    out, lse = ops.window_attention(q, k, v, None, 0, return_lse=True)
+    r = attention64(q, k, v, None, None, 0, 0, 64 ** -0.5, small)
+    got = ops.window_attention_backward(small, q, k, v, out, lse, None, 0)
+    u = unit(torch.float16)
+    for g, n, m, c in ((got[0], "dq", "Mq", 3), (got[1], "dk", "Mk", 3), (got[2], "dv", "Mv", 1)):
+        close(g, r[n], u * (r[n].abs() + c * r[m]) + 3 * SLACK * r[m] + 2.0 ** -25, n)
