@@ -33,7 +33,8 @@ from slsmi.model import Model, WindowTopKModel  # noqa: E402
 
 
 def build_model(args, device):
-    kw = dict(cp_path=args.cp_path, precision=args.precision)
+    kw = dict(cp_path=args.cp_path, precision=args.precision,
+              attention_window=args.attention_window, attention_sinks=args.attention_sinks)
     if args.head == "sls":
         return Model(args, device, **kw)
     kw.update(use_sae=True, use_sparse_features=args.use_sparse_features, sae_dict_size=args.sae_dict_size,
@@ -95,6 +96,11 @@ def main() -> int:
     ap.add_argument("--log_scores", action="store_true", help="write log-probabilities (the upstream SLS convention)")
     ap.add_argument("--variable_length", action="store_true")
     ap.add_argument("--max_seconds", type=float, default=10.0)
+    ap.add_argument("--attention_window", type=int, nargs=2, metavar=("BEFORE", "AFTER"), default=None,
+                    help="in-tree heads: the encoder attends by a sliding window of so many frames before and after (-1: no "
+                         "limit; 50 frames a second), which takes recordings of up to 16384 frames (raise --max_seconds)")
+    ap.add_argument("--attention_sinks", type=int, default=0,
+                    help="with --attention_window: first frames that stay visible (0 to 128)")
     ap.add_argument("--max_frames", type=int, default=0,
                     help="with --variable_length: frame budget of a batch (clips x frames of its padded length; batches of "
                          "up to 4 x --batch_size clips); 12896 fills one round of the encoder GEMM tiles; 0 = --batch_size clips")

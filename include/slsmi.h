@@ -102,6 +102,12 @@ int slsmi_set_low_latency(slsmi_ctx* ctx, int enable);
  * Both forms compute the reference's Linear(LayerNorm(x)); they round at different points, so scores differ in
  * their last bits (within the tolerance of the path). */
 int slsmi_set_ln_fold(slsmi_ctx* ctx, int enable);   /* 2 (tests): the 208 x 256 form for every batch it can run */
+/* Recordings of more than 512 frames (no counterpart in the reference, whose encoder attends over a whole clip,
+ * wav2vec2.py:1046-1052): with enable != 0 the encoder of the scoring forward attends by a sliding window with sinks --
+ * slsmi_window_attention with these left, right, sinks (frames; -1: no limit; sinks 0 .. 128) -- and takes clips of up to
+ * 16384 frames (5.5 minutes), at most 32768 frames in a batch of clips of more than 512.  left = right = -1 is the
+ * reference's attention at any length.  Takes effect at the next forward; training steps are refused meanwhile. */
+int slsmi_set_attention_window(slsmi_ctx* ctx, int enable, int left, int right, int sinks);
 /* 1 (default): the scoring forward runs the positional conv on the slab-resident kernel where it applies
  * (clips in segments of 208 frames; same bits as the batched-GEMM form, which 0 selects everywhere). */
 int slsmi_set_posconv_slab(slsmi_ctx* ctx, int enable);

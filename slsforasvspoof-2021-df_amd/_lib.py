@@ -81,6 +81,7 @@ SIGNATURES = {
     "slsmi_forward_varlen": (C.c_int, [_P, _P, C.c_int, C.c_int, _P, _P, C.c_size_t, _P, _P, _P, _P]),
     "slsmi_enable_training": (C.c_int, [_P]),
     "slsmi_set_low_latency": (C.c_int, [_P, C.c_int]),
+    "slsmi_set_attention_window": (C.c_int, [_P, C.c_int, C.c_int, C.c_int, C.c_int]),
     "slsmi_set_ln_fold": (C.c_int, [_P, C.c_int]),
     "slsmi_set_posconv_slab": (C.c_int, [_P, C.c_int]),
     "slsmi_set_conv_precision": (C.c_int, [_P, C.c_uint, C.c_uint]),

@@ -112,6 +112,8 @@ struct slsmi_ctx {
     slsmi::TrainState* train = nullptr;  // set by slsmi_enable_training
     float* split_ws = nullptr;           // K-split scratch of this context's GEMMs (made by slsmi_finalize)
     bool split_scoring = false;          // slsmi_set_low_latency: the scoring forward may split K too
+    bool att_window = false;             // slsmi_set_attention_window: the scoring forward's encoder attends by a window
+    int att_left = -1, att_right = -1, att_sinks = 0;
     bool ln_fold = true;                 // the scoring forward folds the encoder's LayerNorms into its GEMMs
     bool ln_fold_force_wide = false;     // (tests) the 208 x 256 form for every batch it can run, not only where it wins
     bool posconv_slab = true;            // the scoring forward runs the positional conv on the slab-resident kernel (clips of <= 208 frames)

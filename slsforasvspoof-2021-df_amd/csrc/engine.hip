@@ -118,7 +118,9 @@ bool make_plan(const slsmi_ctx* c, int B, int L, Plan* p) {
     if (!conv_frames(cfg, L, p->T)) return false;
     const int n = cfg.n_conv;
     p->frames = p->T[n - 1];
-    if (p->frames > 512 || p->frames < 3) return false;
+    // the whole-clip attention kernel holds 512 frames; the windowed one any number (and the batch as a whole stays
+    // within what 64 clips of 512 frames reach)
+    if (p->frames < 3 || (p->frames > 512 && (!c->att_window || p->frames > 16384 || (long)B * p->frames > 32768))) return false;
     // Rows stored per utterance after every conv layer: P[i-1] = stride_i * P[i], so
     // that output row m of the whole batch reads input rows stride*m .. stride*m + k - 1
     // and each conv layer is ONE flat GEMM over all utterances.
@@ -611,7 +613,8 @@ int forward_impl(slsmi_ctx* c, const float* wav, int B, int L, const int32_t* le
     const slsmi_config& cfg = c->cfg;
     Plan p;
     if (!make_plan(c, B, L, &p))
-        return fail(c, SLSMI_ERR_INVALID, "unsupported batch/length (frames must be in [3, 512] and at least sae_window)");
+        return fail(c, SLSMI_ERR_INVALID, "unsupported batch/length (frames must be in [3, 512] and at least sae_window; with an attention "
+                                          "window up to 16384, and up to 32768 in a batch of longer clips)");
     if (workspace_bytes < p.total || (reinterpret_cast<uintptr_t>(workspace) & (ALIGN - 1)))
         return fail(c, SLSMI_ERR_WORKSPACE, "workspace too small or not 256-byte aligned");
     if (cfg.head == SLSMI_HEAD_SLS && p.sls_in != c->sls_in)
@@ -786,7 +789,19 @@ int forward_impl(slsmi_ctx* c, const float* wav, int B, int L, const int32_t* le
         HIP_TRY(c, RANGE(SLSMI_RANGE_LAYER0 + SLSMI_RANGE_PER_LAYER * l + 0, B16(p.h), M, 1024, 1024));   // LayerNorm 1 operand
         HIP_TRY(c, launch_gemm(g, s));
         HIP_TRY(c, RANGE(SLSMI_RANGE_LAYER0 + SLSMI_RANGE_PER_LAYER * l + 1, B16(p.qkv), M, 3072, 3072));
-        HIP_TRY(c, launch_attention(B16(p.qkv), B16(p.ao), B, T, fmt, s, nframes));
+        if (c->att_window) {
+            WindowParams w;   // q arrives scaled
+            w.q = {B16(p.qkv), (long)T * 3 * 1024, 3 * 1024, 64};
+            w.k = {B16(p.qkv) + 1024, (long)T * 3 * 1024, 3 * 1024, 64};
+            w.v = {B16(p.qkv) + 2048, (long)T * 3 * 1024, 3 * 1024, 64};
+            w.o = {B16(p.ao), (long)T * 1024, 1024, 64};
+            w.nframes = nframes;
+            w.B = B; w.T = T; w.Hq = w.Hk = 16; w.D = 64; w.fmt = fmt; w.scale = 1.f;
+            w.left = c->att_left; w.right = c->att_right; w.sinks = c->att_sinks;
+            HIP_TRY(c, launch_window_attention(w, nullptr, s));
+        } else {
+            HIP_TRY(c, launch_attention(B16(p.qkv), B16(p.ao), B, T, fmt, s, nframes));
+        }
         HIP_TRY(c, RANGE(SLSMI_RANGE_LAYER0 + SLSMI_RANGE_PER_LAYER * l + 2, B16(p.ao), M, 1024, 1024));
         g = GemmArgs();
         g.fmt = fmt;
@@ -942,6 +957,17 @@ const char* slsmi_last_error(const slsmi_ctx* c) { return c ? c->err.c_str() : "
 int slsmi_set_low_latency(slsmi_ctx* c, int enable) {
     if (!c) return SLSMI_ERR_INVALID;
     c->split_scoring = enable != 0;
+    return SLSMI_OK;
+}
+
+int slsmi_set_attention_window(slsmi_ctx* c, int enable, int left, int right, int sinks) {
+    if (!c) return SLSMI_ERR_INVALID;
+    if (enable && (left < -1 || right < -1 || sinks < 0 || sinks > 128))
+        return fail(c, SLSMI_ERR_INVALID, "attention window: left and right are frames or -1, sinks 0 to 128");
+    c->att_window = enable != 0;
+    c->att_left = left;
+    c->att_right = right;
+    c->att_sinks = sinks;
     return SLSMI_OK;
 }
 

@@ -110,6 +110,7 @@ bool make_tplan(const slsmi_ctx* c, int B, int L, TPlan* p) {
     if (!conv_frames(cfg, L, p->T)) return false;
     const int n = cfg.n_conv;
     p->frames = p->T[n - 1];
+    if (c->att_window) return false;                     // the training step attends over whole clips
     if (p->frames > 256 || p->frames < 3) return false;  // the attention backward holds T <= 256 frames
     int last = (p->frames + 7) / 8 * 8;
     for (;; last += 8) {

@@ -48,7 +48,7 @@ class Engine:
 
     def __init__(self, device: torch.device, cfg: BackboneConfig = XLSR_300M, head: str = "sls",
                  sae_dict: int = 4096, sae_k: int = 128, precision: str = "f16", sae_window: int = 1,
-                 low_latency: bool = False, ln_fold: Optional[bool] = None):
+                 low_latency: bool = False, ln_fold: Optional[bool] = None, attention_window=None, attention_sinks: int = 0):
         device = torch.device(device)
         if precision not in _lib.FORMATS:
             raise ValueError(f"precision must be one of {sorted(_lib.FORMATS)}, got {precision!r}")
@@ -67,6 +67,10 @@ class Engine:
         if low_latency:  # small batches: GEMMs cut along K to fill the chip (scores then depend on the batch size
             # in their last bits; see slsmi_set_low_latency)
             _lib.check(self.lib.slsmi_set_low_latency(self._ctx, 1), self._ctx, "slsmi_set_low_latency")
+        if attention_window is not None:  # (frames before, frames after), None for no limit: slsmi_set_attention_window
+            left, right = (-1 if n is None else int(n) for n in attention_window)
+            _lib.check(self.lib.slsmi_set_attention_window(self._ctx, 1, left, right, int(attention_sinks)), self._ctx,
+                       "slsmi_set_attention_window")
         # ln_fold (or SLSMI_LN_FOLD=0/1; on by default): the scoring forward folds the encoder's LayerNorms into the
         # GEMMs around them (slsmi_set_ln_fold)
         if ln_fold is None:

@@ -126,6 +126,8 @@ class SSLModel(nn.Module):
         self._owner = None  # weakref to the Model that owns the engine, if any
         self._engine: Optional[Engine] = None
         self._stamp = None
+        # the attention window of the Model this extractor belongs to, kept should it outlive that Model
+        self.attention_window, self.attention_sinks = None, 0
         # dropout / layerdrop probabilities of the backbone in train mode, as the checkpoint's embedded
         # configuration gives them (None: the file had none, or seeded weights)
         self.train_stochastic: Optional[Dict[str, float]] = None
@@ -149,7 +151,8 @@ class SSLModel(nn.Module):
         stamp = _stamp(self)
         if self._engine is None or self._engine.device != device or self._stamp != stamp:
             if self._engine is None or self._engine.device != device:
-                self._engine = Engine(device, self.cfg, "none", precision=self.precision)
+                self._engine = Engine(device, self.cfg, "none", precision=self.precision,
+                                      attention_window=self.attention_window, attention_sinks=self.attention_sinks)
             self._engine.load_tensors((BACKBONE_PREFIX + k, v) for k, v in self.model.state_dict().items())
             self._stamp = stamp
         return self._engine
@@ -358,8 +361,16 @@ class Model(nn.Module):
                  use_sparse_features: bool = True, sae_dict_size: int = 4096, sae_k: int = 128,
                  sae_weight: float = 0.1, head: Optional[str] = None, cfg: BackboneConfig = XLSR_300M,
                  num_samples: int = 64600, seed: int = 1234, precision: Optional[str] = None,
-                 sae_window_size: int = 1, low_latency: Optional[bool] = None):
+                 sae_window_size: int = 1, low_latency: Optional[bool] = None, attention_window=None,
+                 attention_sinks: int = 0):
         super().__init__()
+        # attention_window=(frames before, frames after), None for no limit on a side: the encoder attends by a sliding
+        # window in which the first attention_sinks frames stay visible, and scores recordings of up to 16384 frames
+        # (slsmi_set_attention_window; in-tree heads, evaluation only)
+        if attention_window is not None and len(tuple(attention_window)) != 2:
+            raise ValueError(f"attention_window is (frames before, frames after), got {attention_window!r}")
+        self.attention_window = tuple(attention_window) if attention_window is not None else None
+        self.attention_sinks = int(attention_sinks)
         # low_latency (or SLSMI_LOW_LATENCY=1): small batches score faster (GEMMs cut along K to fill the chip),
         # at the price that a score depends on the batch size in its last bits (slsmi_set_low_latency)
         self.low_latency = bool(int(os.environ.get("SLSMI_LOW_LATENCY", "0"))) if low_latency is None else bool(low_latency)
@@ -393,6 +404,7 @@ class Model(nn.Module):
         self.sae_dict_size, self.sae_k = sae_dict_size, sae_k
         self.ssl_model = SSLModel(device=device, cp_path=cp_path, cfg=cfg, seed=seed, precision=self.precision)
         self.ssl_model._owner = weakref.ref(self)
+        self.ssl_model.attention_window, self.ssl_model.attention_sinks = self.attention_window, self.attention_sinks
         frames = cfg.num_frames(num_samples)
         if head == "sls":
             self.first_bn = nn.BatchNorm2d(num_features=1)
@@ -421,7 +433,8 @@ class Model(nn.Module):
         stamp = _stamp(self)
         if self._engine is None or self._engine.device != device:
             self._engine = Engine(device, self.cfg, self.head, self.sae_dict_size, self.sae_k, self.precision,
-                                  self.sae_window_size if self.use_sae else 1, low_latency=self.low_latency)
+                                  self.sae_window_size if self.use_sae else 1, low_latency=self.low_latency,
+                                  attention_window=self.attention_window, attention_sinks=self.attention_sinks)
             self._engine_stamp = None
         if training and not self._engine.training_enabled:
             self._engine.enable_training()
@@ -549,7 +562,8 @@ class Model(nn.Module):
             entry = engines.get(dev.index)
             if entry is None:
                 entry = [Engine(dev, self.cfg, self.head, self.sae_dict_size, self.sae_k, self.precision,
-                                self.sae_window_size if self.use_sae else 1, low_latency=self.low_latency), None]
+                                self.sae_window_size if self.use_sae else 1, low_latency=self.low_latency,
+                                attention_window=self.attention_window, attention_sinks=self.attention_sinks), None]
                 engines[dev.index] = entry
             if entry[1] != stamp:
                 entry[0].load_state_dict(_replica_state_dict(self))   # this copy's tensors are on `dev`
@@ -589,6 +603,8 @@ class Model(nn.Module):
                        backbone_masks=None):
         if lengths is not None or return_interpretability:
             raise NotImplementedError("lengths= / return_interpretability are scoring options")
+        if self.attention_window is not None:
+            raise _lib.SlsmiError("attention_window is a scoring option: the training step attends over whole clips")
         # the reference's extract_feat leaves the backbone in train mode (model.py:130-132): what the checkpoint's
         # configuration sets applies while fine-tuning.  dropout_features acts on a copy this path never reads.
         st = self.ssl_model.train_stochastic or {}
