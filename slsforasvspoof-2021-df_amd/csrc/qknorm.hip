@@ -102,6 +102,15 @@ __global__ __launch_bounds__(QN_WAVES * 64) void qk_norm_rope_kernel(QkNormArgs 
     }
 }
 
+// The gradient at a whole head is zero: a padded frame, as a rule.  Its dx is zero and it adds nothing to dw, also where
+// the head itself holds infinities or NaN, so its values are replaced.
+template <int GL>
+__device__ __forceinline__ bool dead_head(u16x8 dy, int g) {
+    const u32x4 v = __builtin_bit_cast(u32x4, dy);
+    const unsigned long long live = __ballot(((v[0] | v[1] | v[2] | v[3]) & 0x7fff7fffu) != 0);
+    return ((live >> (g * GL)) & ((1u << GL) - 1)) == 0;
+}
+
 // dx of a wave's rows; the weights' gradients stay in registers over the rows of a wave and leave as one partial sum per
 // workgroup (summed in workgroup order by the kernel below: the result does not depend on timing).
 template <int FMT, int D>
@@ -125,6 +134,7 @@ __global__ __launch_bounds__(QN_WAVES * 64) void qk_norm_rope_bwd_kernel(QkNormA
         const bf16_t* dy = a.dy + row * a.lddy + c * 8;
         bf16_t* y = a.y + row * a.ldy + c * 8;
         constexpr int U = 4;
+        const u16x8 one = 0x3f80;   // (any finite value, in both formats)
         u16x8 xv[U], dv[U];
         auto request = [&](int h) {
 #pragma unroll
@@ -142,6 +152,7 @@ __global__ __launch_bounds__(QN_WAVES * 64) void qk_norm_rope_bwd_kernel(QkNormA
             for (int u = 0; u < U; ++u) {
                 const int hh = h + u * HW, hb = hh - g;   // hb: the wave's first head
                 if (hb >= H) break;
+                xv[u] = dead_head<GL>(dv[u], g) ? one : xv[u];
                 const float r = head_rstd<FMT, D>(xv[u], a.eps);
                 const u16x8 pd = lane_exchange(dv[u], t.partner);
                 float dn[8], xh[8];

@@ -654,7 +654,8 @@ def qk_norm_rope_backward(dout: torch.Tensor, qkv: torch.Tensor, heads: int, kv_
                           positions: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False,
                           out: Optional[torch.Tensor] = None):
     """Gradient of qk_norm_rope: dout at its result, qkv as it was given -> (dqkv [..., (heads + kv_heads) * D],
-    dq_weight, dk_weight).  out: where dqkv goes (dout itself, or the packed gradient whose value columns
+    dq_weight, dk_weight).  A head whose dout is all zeros (a padded frame's) may hold anything: its gradient is zero and it
+    adds nothing to the weights'.  out: where dqkv goes (dout itself, or the packed gradient whose value columns
     window_attention_backward wrote)."""
     index = _device_of(qkv)
     lead = qkv.shape[:-1]
