@@ -11,6 +11,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from . import _lib
 from .weights import BACKBONE_PREFIX
 
 # pre-training leftovers of the fairseq checkpoint that the forward never reads (wav2vec2.py:313-362)
@@ -79,6 +80,70 @@ class GradSync:
             self._flat.copy_(buf)
         self._flat.mul_(1.0 / dist.get_world_size(self.group))
         torch._foreach_copy_([p.grad for p in ps], views)
+
+
+class _WindowedAttention(torch.autograd.Function):
+    """windowed_attention as one node.  Kept for the backward pass: qkv as it was given, the normalised and rotated heads
+    (a copy: the norm's gradient needs the heads from before it), the result and the rows' log-sum-exp."""
+
+    @staticmethod
+    def forward(ctx, qkv, q_weight, k_weight, heads, kv_heads, D, freqs, positions, nframes, eps, interleaved, window):
+        from . import ops
+        B, T = qkv.shape[:2]
+        split = lambda t: t.split((heads, kv_heads), 2)  # noqa: E731
+        packed = qkv.view(B, T, heads + 2 * kv_heads, D)
+        if q_weight is None:
+            normed, (q, k) = None, split(packed[:, :, :heads + kv_heads])
+        else:
+            normed = ops.qk_norm_rope(qkv, heads, kv_heads, q_weight, k_weight, freqs, positions, eps, interleaved)
+            q, k = split(normed.view(B, T, heads + kv_heads, D))
+        out, lse = ops.window_attention(q, k, packed[:, :, heads + kv_heads:], nframes=nframes, return_lse=True, **window)
+        ctx.save_for_backward(qkv, normed, out, lse, q_weight, k_weight, freqs, positions, nframes)
+        ctx.args = heads, kv_heads, D, eps, interleaved, window
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        from . import ops
+        qkv, normed, out, lse, q_weight, k_weight, freqs, positions, nframes = ctx.saved_tensors
+        heads, kv_heads, D, eps, interleaved, window = ctx.args
+        B, T = qkv.shape[:2]
+        n = heads + kv_heads
+        packed = qkv.view(B, T, n + kv_heads, D)
+        grad = torch.empty_like(qkv)
+        to = grad.view(B, T, n + kv_heads, D)
+        qk = packed if normed is None else normed.view(B, T, n, D)
+        ops.window_attention_backward(dout.contiguous(), qk[:, :, :heads], qk[:, :, heads:n], packed[:, :, n:], out, lse,
+                                      nframes=nframes, dq=to[:, :, :heads], dk=to[:, :, heads:n], dv=to[:, :, n:], **window)
+        dwq = dwk = None
+        if normed is not None:   # in place over the query and key columns; the value columns stay
+            _, dwq, dwk = ops.qk_norm_rope_backward(grad, qkv, heads, kv_heads, q_weight, k_weight, freqs, positions, eps,
+                                                    interleaved, out=grad)
+        return (grad, dwq, dwk) + (None,) * 9
+
+
+def windowed_attention(qkv: torch.Tensor, heads: int, kv_heads: int, left: Optional[int], right: Optional[int] = 0,
+                       sinks: int = 0, nframes: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                       q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                       freqs: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                       interleaved: bool = False) -> torch.Tensor:
+    """Windowed attention over packed heads with its gradient: ops.window_attention of the query, key and value heads of
+    qkv [batch, frames, (heads + 2 kv_heads) * D] (16 bits, contiguous), query and key heads first through
+    ops.qk_norm_rope where q_weight and k_weight (fp32 [D]) are given.  Returns [batch, frames, heads, D]; autograd
+    carries gradients to qkv, q_weight and k_weight.  Without norms the head width is what qkv holds for each head; the
+    gradient is that of one differentiation."""
+    if qkv.dim() != 3 or not qkv.is_contiguous() or heads < 1 or kv_heads < 1 or qkv.shape[2] % (heads + 2 * kv_heads):
+        raise _lib.SlsmiError(f"qkv: contiguous [batch, frames, ({heads} + 2 * {kv_heads}) * D] expected, got {tuple(qkv.shape)}, "
+                              f"strides {qkv.stride()}")
+    D = qkv.shape[2] // (heads + 2 * kv_heads)
+    if (q_weight is None) != (k_weight is None) or (q_weight is not None and q_weight.numel() != D):
+        raise _lib.SlsmiError(f"both norm weights, of {D} channels, or neither")
+    if q_weight is None and (freqs is not None or positions is not None):
+        raise _lib.SlsmiError("the rotation needs both norm weights")
+    window = dict(left=left, right=right, sinks=sinks, scale=scale)
+    return _WindowedAttention.apply(qkv, q_weight, k_weight, heads, kv_heads, D, freqs, positions, nframes, eps, interleaved,
+                                    window)
 
 
 class Adam(torch.optim.Optimizer):
