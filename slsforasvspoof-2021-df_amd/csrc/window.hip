@@ -465,18 +465,38 @@ __global__ __launch_bounds__(256) void window_delta_kernel(WinArgs a) {
     }
 }
 
-// Half precision holds P and dS as c P and c dS: a power of two c >= 1 (as its logarithm) that brings the largest dO of the
-// query heads first .. first + n - 1 to about 2^4, so that neither long rows nor small gradients push them below the
-// format's normal range.  c comes out again with the scale of the result.  bfloat16 has the range: c = 1.
+// Half precision holds dS as c dS, c a power of two (here its logarithm) that brings the largest |dO| it is formed with to
+// about 1: gradients scaled up by a loss scale stay below the format's largest value (|dS| is at most 2 D |dO| |V|), small
+// ones and long rows, with their small P, above its smallest normal one.  1 / c comes out again with the scale of the
+// result.  P is held as 2^15 P.  bfloat16 has the range: c = 1.
+constexpr float P_LIFT = 15.f;
+
+__device__ __forceinline__ float lift_of(float top) {
+    const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;   // 0: -127, infinity and NaN: 128
+    return (float)min(max(-e, -24), 24);
+}
+// of queries qa .. qb of the heads first .. first + n - 1
 template <int FMT>
-__device__ __forceinline__ float grad_lift(const WinArgs& a, long first, int n) {
+__device__ __forceinline__ float grad_lift(const WinArgs& a, long first, int n, int qa, int qb) {
     if constexpr (FMT != FMT_F16) return 0.f;
     const int parts = (a.T + DELTA_ROWS - 1) / DELTA_ROWS;
     float top = 0.f;
-    for (int i = threadIdx.x & 63; i < parts * n; i += 64) top = fmaxf(top, a.dmax[first * parts + i]);
-    top = wave_max(top);
-    const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;   // 0: -127, infinity and NaN: 128
-    return (float)min(max(4 - e, 0), 15);
+    for (int h = 0; h < n; ++h)
+        for (int i = qa / DELTA_ROWS + (threadIdx.x & 63); i * DELTA_ROWS <= qb; i += 64)
+            top = fmaxf(top, a.dmax[(first + h) * parts + i]);
+    return lift_of(wave_max(top));
+}
+// of the row that a lane and the lane 32 further hold
+template <int FMT, int NS>
+__device__ __forceinline__ float row_lift(const u16x8 (&d)[NS]) {
+    if constexpr (FMT != FMT_F16) return 0.f;
+    float top = 0.f;
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(Op<FMT>::unpack(d[s][e])));
+    const f32x2 two = both_halves(top);
+    return lift_of(fmaxf(two[0], two[1]));
 }
 
 // ---- backward, queries: dQ; the forward's loop with P recomputed from lse.  The product dO V^T starts from -delta, so
@@ -519,7 +539,7 @@ __device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* ld
     const bool live = q < len;
     const float sc = a.scale * LOG2E;
     const long stat = (long)bh * a.T + min(q, len - 1);
-    const float lift = grad_lift<FMT>(a, bh, 1);
+    const float lift = row_lift<FMT>(df);
     const float ls = a.lse[stat] * LOG2E - lift, delta = a.delta[stat];
     f32x16 acc[DT], start;
 #pragma unroll
@@ -629,7 +649,8 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) ak[dt] = av[dt] = zero16();
     const float sc = a.scale * LOG2E, lsc = 1.0f / a.scale;
-    const float lift = grad_lift<FMT>(a, (long)b * a.Hq + hk * grp, grp), lift_sc = lift / sc;
+    const float p_lift = FMT == FMT_F16 ? P_LIFT : 0.f, lift_sc = p_lift / sc;
+    const float ds_lift = grad_lift<FMT>(a, (long)b * a.Hq + hk * grp, grp, qa, qb), turn = __builtin_amdgcn_exp2f(ds_lift - p_lift);
     const int t0 = qa / BQ, nt = qb < qa ? 0 : qb / BQ - t0 + 1;
     const int total = nt * grp;
     const LaneAt<D> at(lane);
@@ -702,7 +723,7 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 s[r] = __builtin_amdgcn_exp2f(s[r] * sc);
-                dp[r] *= s[r];
+                dp[r] *= FMT == FMT_F16 ? s[r] * turn : s[r];
             }
             const uint32_t q_at = lds_offset(Qs) + 64 * D * u;
             auto step = [&](auto off, int st) {
@@ -727,7 +748,7 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
         }
         if (more) landed(next);
     }
-    const float vfin = __builtin_amdgcn_exp2f(-lift), kfin = a.scale * vfin;
+    const float vfin = __builtin_amdgcn_exp2f(-p_lift), kfin = a.scale * __builtin_amdgcn_exp2f(-ds_lift);
     if (far || (k0w < a.sinks && a.far_blocks > 0)) {
         const int blk = far ? block : k0w / 32, slot = far ? 1 + chunk * 4 + wave : 0;
         if (far && key >= a.sinks) return;

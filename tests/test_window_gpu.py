@@ -572,3 +572,34 @@ def test_half_precision_gradients_follow_small_and_large_dout(power):
     u = unit(torch.float16)
     for g, n, m, c in ((got[0], "dq", "Mq", 3), (got[1], "dk", "Mk", 3), (got[2], "dv", "Mv", 1)):
         close(g, r[n], u * (r[n].abs() + c * r[m]) + 3 * SLACK * r[m] + 2.0 ** -25, n)
+
+
+@pytest.mark.parametrize("window", [(None, 0, 0), (12, 4, 0), (40, 0, 70)])
+def test_half_precision_gradients_under_a_loss_scale(window):
+    """dout of thousands against values of tens to a hundred: dS itself passes half precision's largest value, the gradients do not."""
+    left, right, sinks = window
+    q, k, v, _ = win_case(1, 300, 2, 1, 64, left, right, sinks, None, torch.float16)
+    v = v * 32
+    do = rnd(1, 300, 2, 64, seed=9, dtype=torch.float16) * 2048
+    args, scale = (left, right, sinks), 2.0 ** -10
+    out, lse = ops.window_attention(q, k, v, *args, scale=scale, return_lse=True)
+    r = attention64(q, k, v, None, *args, scale, do)
+    assert bool((r["dq"].abs().max() < 60000) & (r["dk"].abs().max() < 60000) & (r["dv"].abs().max() < 60000))
+    got = ops.window_attention_backward(do, q, k, v, out, lse, *args, scale=scale)
+    u = unit(torch.float16)
+    for g, n, m, c in ((got[0], "dq", "Mq", 3), (got[1], "dk", "Mk", 3), (got[2], "dv", "Mv", 1)):
+        close(g, r[n], u * (r[n].abs() + c * r[m]) + 3 * SLACK * r[m] + 2 ** -24, n)
+
+
+def test_half_precision_gradient_of_quiet_rows_beside_loud_ones():
+    """A row's dq keeps its own precision however large its neighbours' dout is (2^3 against 2^-20 in turn)."""
+    q, k, v, _ = win_case(1, 200, 1, 1, 128, 1, 1, 0, None, torch.float16)
+    q, k = q / 1024, k * 1024
+    do = rnd(1, 200, 1, 128, seed=9) * torch.where(torch.arange(200, device=DEV) % 2 == 0, 8.0, 2.0 ** -20)[None, :, None, None]
+    do = do.half()
+    out, lse = ops.window_attention(q, k, v, 1, 1, return_lse=True)
+    r = attention64(q, k, v, None, 1, 1, 0, 128 ** -0.5, do)
+    assert bool(r["dq"].abs().max() < 60000)
+    dq, _, _ = ops.window_attention_backward(do, q, k, v, out, lse, 1, 1)
+    u = unit(torch.float16)
+    close(dq, r["dq"], u * (r["dq"].abs() + 3 * r["Mq"]) + 3 * SLACK * r["Mq"] + 2 ** -25, "dq")
