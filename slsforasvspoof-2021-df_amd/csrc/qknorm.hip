@@ -95,7 +95,7 @@ __global__ __launch_bounds__(QN_WAVES * 64) void qk_norm_rope_kernel(QkNormArgs 
             if (hh < h1) {
                 u32x4 r;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) r[i] = Op<FMT>::pack2(o[2 * i], o[2 * i + 1]);
+                for (int i = 0; i < 4; ++i) r[i] = result2<FMT>(o[2 * i], o[2 * i + 1]);
                 *reinterpret_cast<u32x4*>(y + (long)hh * D) = r;
             }
         }
@@ -203,7 +203,7 @@ __global__ __launch_bounds__(QN_WAVES * 64) void qk_norm_rope_bwd_kernel(QkNormA
                     u32x4 o;
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        o[i] = Op<FMT>::pack2(r * (dn[2 * i] - xh[2 * i] * dot), r * (dn[2 * i + 1] - xh[2 * i + 1] * dot));
+                        o[i] = result2<FMT>(r * (dn[2 * i] - xh[2 * i] * dot), r * (dn[2 * i + 1] - xh[2 * i + 1] * dot));
                     *reinterpret_cast<u32x4*>(y + (long)hh * D) = o;
                 }
             }

@@ -7,7 +7,6 @@ namespace slsmi {
 
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(4))) short s16x4;
-typedef __attribute__((address_space(3))) s16x4* lds_s16x4_ptr;
 
 template <int FMT>
 __device__ __forceinline__ f32x16 mfma32(u16x8 a, u16x8 b, f32x16 c) {
@@ -15,6 +14,17 @@ __device__ __forceinline__ f32x16 mfma32(u16x8 a, u16x8 b, f32x16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     else
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// A result's two values in 16 bits: finite ones past half precision's largest become that, as everywhere in this library;
+// infinities and NaN stay what they are (a loss scale is found too large by them).
+template <int FMT>
+__device__ __forceinline__ uint32_t result2(float a, float b) {
+    if constexpr (FMT == FMT_F16) {
+        const float x = __builtin_amdgcn_fmed3f(a, -65504.0f, 65504.0f), y = __builtin_amdgcn_fmed3f(b, -65504.0f, 65504.0f);
+        return Op<FMT>::pack2_unit(fabsf(a) < INFINITY ? x : a, fabsf(b) < INFINITY ? y : b);
+    }
+    return Op<FMT>::pack2(a, b);
 }
 
 // Lane j's value <- lane j's value of a neighbour inside its row of 16 lanes (no LDS): after the sums over 2, 4, 8, 16

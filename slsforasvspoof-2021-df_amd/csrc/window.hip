@@ -41,7 +41,7 @@ struct WinArgs {
     HeadOut out, dq, dk, dv;
     float* lse;              // [B][Hq][T]
     float* delta;            // [B][Hq][T]: rowsum(dO o O)
-    float* dmax;             // [B][Hq][T / DELTA_ROWS]: largest |dO| (half precision)
+    f32x2* dmax;             // [B][Hq][T / DELTA_ROWS]: largest |dO|, |delta| (half precision)
     float* part;             // sink keys' partial sums (see window_dkv)
     const int* nframes;
     int B, T, Hq, Hk;
@@ -219,16 +219,13 @@ __device__ __forceinline__ KeyTiles key_tiles(int qa, int qb, int len, int left,
 
 // 32 x 32 tile of a transposed result (row = 8 (r / 4) + 4 hi + r % 4, column = lane % 32), rows dt * 32 .. of D: the
 // halves of the wave exchange so that each lane stores 16 contiguous bytes of its column's row of memory.
-template <int FMT, bool UNIT>
+template <int FMT>
 __device__ __forceinline__ void store_column(bf16_t* dst, int dt, f32x16 v, int hi) {
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
         uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float a = v[8 * p + 2 * i], b = v[8 * p + 2 * i + 1];
-            w[i] = UNIT ? Op<FMT>::pack2_unit(a, b) : Op<FMT>::pack2(a, b);
-        }
+        for (int i = 0; i < 4; ++i) w[i] = result2<FMT>(v[8 * p + 2 * i], v[8 * p + 2 * i + 1]);
         const auto x = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
         const auto y = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
         *reinterpret_cast<u32x4*>(dst + dt * 32 + p * 16 + hi * 8) = u32x4{x[0], y[0], x[1], y[1]};
@@ -237,11 +234,6 @@ __device__ __forceinline__ void store_column(bf16_t* dst, int dt, f32x16 v, int 
 
 template <int FMT>
 __device__ __forceinline__ u16x8 pack_step(const f32x16& p, int s) {
-    return __builtin_bit_cast(u16x8, u32x4{Op<FMT>::pack2(p[8 * s], p[8 * s + 1]), Op<FMT>::pack2(p[8 * s + 2], p[8 * s + 3]),
-                                           Op<FMT>::pack2(p[8 * s + 4], p[8 * s + 5]), Op<FMT>::pack2(p[8 * s + 6], p[8 * s + 7])});
-}
-template <int FMT>
-__device__ __forceinline__ u16x8 pack_step_unit(const f32x16& p, int s) {
     return __builtin_bit_cast(u16x8, u32x4{Op<FMT>::pack2_unit(p[8 * s], p[8 * s + 1]), Op<FMT>::pack2_unit(p[8 * s + 2], p[8 * s + 3]),
                                            Op<FMT>::pack2_unit(p[8 * s + 4], p[8 * s + 5]), Op<FMT>::pack2_unit(p[8 * s + 6], p[8 * s + 7])});
 }
@@ -331,7 +323,7 @@ __global__ __launch_bounds__(256, fwd_waves(D)) void window_fwd_kernel(WinArgs a
     if (q0 >= len) {
         if (q < a.T) {
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) store_column<FMT, true>(orow, dt, zero16(), hi);
+            for (int dt = 0; dt < DT; ++dt) store_column<FMT>(orow, dt, zero16(), hi);
             if (lse && hi == 0) *lse = -INFINITY;
         }
         return;
@@ -403,7 +395,7 @@ __global__ __launch_bounds__(256, fwd_waves(D)) void window_fwd_kernel(WinArgs a
             l += sum;
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
-                const u16x8 p = pack_step_unit<FMT>(s, st);
+                const u16x8 p = pack_step<FMT>(s, st);
                 if constexpr (D != 64) {
                     if (st == 0) tr_frags<D, 0>(v_at, at, vt[0]);
                     else tr_frags<D, 32 * D>(v_at, at, vt[1]);
@@ -421,24 +413,24 @@ __global__ __launch_bounds__(256, fwd_waves(D)) void window_fwd_kernel(WinArgs a
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
             const f32x16 v = live ? o[dt] * inv : zero16();
-            store_column<FMT, true>(orow, dt, v, hi);
+            store_column<FMT>(orow, dt, v, hi);
         }
         if (lse && hi == 0) *lse = live ? (m + __builtin_amdgcn_logf(l)) * LN2 : -INFINITY;
     }
 }
 
 // ---- backward, first launch: delta = rowsum(dO o O) of DELTA_ROWS rows of a head per workgroup, and (half precision) the
-// largest |dO| among them.  D / 8 lanes hold a row, 16 bytes of both each.
+// largest |dO| and |delta| among them.  D / 8 lanes hold a row, 16 bytes of both each.
 constexpr int DELTA_ROWS = 128;
 
 template <int FMT, int D>
 __global__ __launch_bounds__(256) void window_delta_kernel(WinArgs a) {
     constexpr int GL = D / 8, PER = 256 / GL;
-    __shared__ float red[4];
+    __shared__ f32x2 red[4];
     const int b = blockIdx.z, h = blockIdx.y, c = (threadIdx.x & (GL - 1)) * 8;
     const int len = frames_of(a, b);
     const long bh = (long)b * a.Hq + h;
-    float top = 0.f;
+    f32x2 top = {0.f, 0.f};
 #pragma unroll 4
     for (int i = 0; i < DELTA_ROWS / PER; ++i) {
         const int q = blockIdx.x * DELTA_ROWS + i * PER + threadIdx.x / GL, row = min(q, max(len - 1, 0));   // (a batch has a row 0)
@@ -449,54 +441,60 @@ __global__ __launch_bounds__(256) void window_delta_kernel(WinArgs a) {
         for (int e = 0; e < 8; ++e) {
             const float d = Op<FMT>::unpack(x[e]);
             s = fmaf(d, Op<FMT>::unpack(y[e]), s);
-            m = fmaxf(m, fabsf(d));
+            m = fmaxf(m, fabsf(d) < INFINITY ? fabsf(d) : 0.f);   // (infinite rows say nothing about the others')
         }
         s = lane_group_sum<GL>(s);
         if (q < len) {
-            top = fmaxf(top, m);
+            top = f32x2{fmaxf(top[0], m), fmaxf(top[1], fabsf(s) < INFINITY ? fabsf(s) : 0.f)};
             if (c == 0) a.delta[bh * a.T + q] = s;
         }
     }
     if constexpr (FMT == FMT_F16) {
-        top = wave_max(top);
+        top = f32x2{wave_max(top[0]), wave_max(top[1])};
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
         __syncthreads();
-        if (threadIdx.x == 0) a.dmax[bh * gridDim.x + blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        if (threadIdx.x == 0) {
+#pragma unroll
+            for (int w = 1; w < 4; ++w) top = f32x2{fmaxf(top[0], red[w][0]), fmaxf(top[1], red[w][1])};
+            a.dmax[bh * gridDim.x + blockIdx.x] = top;
+        }
     }
 }
 
-// Half precision holds dS as c dS, c a power of two (here its logarithm) that brings the largest |dO| it is formed with to
-// about 1: gradients scaled up by a loss scale stay below the format's largest value (|dS| is at most 2 D |dO| |V|), small
-// ones and long rows, with their small P, above its smallest normal one.  1 / c comes out again with the scale of the
-// result.  P is held as 2^15 P.  bfloat16 has the range: c = 1.
+// Half precision holds dS as c dS, c a power of two (here its logarithm), so that gradients under a loss scale stay below
+// the format's largest value, and small ones and long rows, with their small P, above its smallest normal one; 1 / c comes
+// out again with the scale of the result.  P is held as 2^15 P.  bfloat16 has the range: c = 1.
+//   Keys: c of each key (a lane) brings sqrt(D) max|dO| max|v| + max|delta| to about 2^8.  |dS| <= D max|dO| max|v| +
+// max|delta|: nothing saturates.
+//   Queries: the values are not known beforehand; c of each row brings its largest |dO| to about 1, which leaves room for
+// values of hundreds however they are aligned, of thousands as a rule (and dS, in two operands, has the bits to spare).
 constexpr float P_LIFT = 15.f;
 
-__device__ __forceinline__ float lift_of(float top) {
+__device__ __forceinline__ float lift_of(float top, int to) {
     const int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;   // 0: -127, infinity and NaN: 128
-    return (float)min(max(-e, -24), 24);
+    return (float)min(max(to - e, -40), 40);
 }
-// of queries qa .. qb of the heads first .. first + n - 1
-template <int FMT>
-__device__ __forceinline__ float grad_lift(const WinArgs& a, long first, int n, int qa, int qb) {
-    if constexpr (FMT != FMT_F16) return 0.f;
+// largest |dO| and |delta| of queries qa .. qb of the heads first .. first + n - 1
+__device__ __forceinline__ f32x2 grad_size(const WinArgs& a, long first, int n, int qa, int qb) {
     const int parts = (a.T + DELTA_ROWS - 1) / DELTA_ROWS;
-    float top = 0.f;
+    f32x2 top = {0.f, 0.f};
     for (int h = 0; h < n; ++h)
-        for (int i = qa / DELTA_ROWS + (threadIdx.x & 63); i * DELTA_ROWS <= qb; i += 64)
-            top = fmaxf(top, a.dmax[(first + h) * parts + i]);
-    return lift_of(wave_max(top));
+        for (int i = qa / DELTA_ROWS + (threadIdx.x & 63); i * DELTA_ROWS <= qb; i += 64) {
+            const f32x2 v = a.dmax[(first + h) * parts + i];
+            top = f32x2{fmaxf(top[0], v[0]), fmaxf(top[1], v[1])};
+        }
+    return f32x2{wave_max(top[0]), wave_max(top[1])};
 }
-// of the row that a lane and the lane 32 further hold
+// largest value of the row that a lane and the lane 32 further hold
 template <int FMT, int NS>
-__device__ __forceinline__ float row_lift(const u16x8 (&d)[NS]) {
-    if constexpr (FMT != FMT_F16) return 0.f;
+__device__ __forceinline__ float row_size(const u16x8 (&d)[NS]) {
     float top = 0.f;
 #pragma unroll
     for (int s = 0; s < NS; ++s)
 #pragma unroll
         for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(Op<FMT>::unpack(d[s][e])));
     const f32x2 two = both_halves(top);
-    return lift_of(fmaxf(two[0], two[1]));
+    return fmaxf(two[0], two[1]);
 }
 
 // ---- backward, queries: dQ; the forward's loop with P recomputed from lse.  The product dO V^T starts from -delta, so
@@ -514,7 +512,7 @@ __device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* ld
     if (q0 >= len) {
         if (q < a.T) {
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) store_column<FMT, true>(dqrow, dt, zero16(), hi);
+            for (int dt = 0; dt < DT; ++dt) store_column<FMT>(dqrow, dt, zero16(), hi);
         }
         return;
     }
@@ -539,7 +537,7 @@ __device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* ld
     const bool live = q < len;
     const float sc = a.scale * LOG2E;
     const long stat = (long)bh * a.T + min(q, len - 1);
-    const float lift = row_lift<FMT>(df);
+    const float lift = FMT == FMT_F16 ? lift_of(row_size<FMT>(df), 0) : 0.f;
     const float ls = a.lse[stat] * LOG2E - lift, delta = a.delta[stat];
     f32x16 acc[DT], start;
 #pragma unroll
@@ -592,7 +590,7 @@ __device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* ld
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
             const f32x16 v = live ? acc[dt] * fin : zero16();
-            store_column<FMT, false>(dqrow, dt, v, hi);
+            store_column<FMT>(dqrow, dt, v, hi);
         }
     }
 }
@@ -650,7 +648,12 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
     for (int dt = 0; dt < DT; ++dt) ak[dt] = av[dt] = zero16();
     const float sc = a.scale * LOG2E, lsc = 1.0f / a.scale;
     const float p_lift = FMT == FMT_F16 ? P_LIFT : 0.f, lift_sc = p_lift / sc;
-    const float ds_lift = grad_lift<FMT>(a, (long)b * a.Hq + hk * grp, grp, qa, qb), turn = __builtin_amdgcn_exp2f(ds_lift - p_lift);
+    float ds_lift = 0.f;
+    if constexpr (FMT == FMT_F16) {
+        const f32x2 top = grad_size(a, (long)b * a.Hq + hk * grp, grp, qa, qb);
+        ds_lift = lift_of(fmaf(top[0] * (D == 64 ? 8.f : 11.f), row_size<FMT>(vf), top[1]), 8);
+    }
+    const float turn = __builtin_amdgcn_exp2f(ds_lift - p_lift);
     const int t0 = qa / BQ, nt = qb < qa ? 0 : qb / BQ - t0 + 1;
     const int total = nt * grp;
     const LaneAt<D> at(lane);
@@ -730,7 +733,7 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
                 constexpr int OFF = decltype(off)::value;
                 u16x8 t[DT];
                 tr_frags<D, OFF>(q_at + TILE, at, t);
-                const u16x8 pf = pack_step_unit<FMT>(s, st);
+                const u16x8 pf = pack_step<FMT>(s, st);
                 u16x8 ef, rest;
                 if constexpr (SPLIT) split_step<FMT>(dp, st, ef, rest);
                 else ef = pack_step<FMT>(dp, st);
@@ -774,8 +777,8 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
         const bool live = key < len;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-            store_column<FMT, false>(dk, dt, live ? ak[dt] * kfin : zero16(), hi);
-            store_column<FMT, false>(dv, dt, live ? av[dt] * vfin : zero16(), hi);
+            store_column<FMT>(dk, dt, live ? ak[dt] * kfin : zero16(), hi);
+            store_column<FMT>(dv, dt, live ? av[dt] * vfin : zero16(), hi);
         }
     }
 }
@@ -818,7 +821,7 @@ __global__ __launch_bounds__(1024) void window_sink_kernel(WinArgs a) {
     const HeadOut& d = which ? a.dv : a.dk;
     typedef __attribute__((ext_vector_type(2))) uint32_t u32x2_t;
     *reinterpret_cast<u32x2_t*>(d.p + b * d.b + hk * d.h + (long)key * d.r + c) =
-        u32x2_t{Op<FMT>::pack2(s[0], s[1]), Op<FMT>::pack2(s[2], s[3])};
+        u32x2_t{result2<FMT>(s[0], s[1]), result2<FMT>(s[2], s[3])};
 }
 
 constexpr int FAR_CHUNK = 1024;
@@ -860,7 +863,7 @@ HeadPtr in_head(const WindowHeads& x) { return {x.p, x.batch, x.row, x.head}; }
 HeadOut out_head(const WindowHeads& x) { return {const_cast<bf16_t*>(x.p), x.batch, x.row, x.head}; }
 
 size_t dmax_bytes(const WinArgs& a) {
-    return ((size_t)a.B * a.Hq * ((a.T + DELTA_ROWS - 1) / DELTA_ROWS) * sizeof(float) + 255) & ~(size_t)255;
+    return ((size_t)a.B * a.Hq * ((a.T + DELTA_ROWS - 1) / DELTA_ROWS) * sizeof(f32x2) + 255) & ~(size_t)255;
 }
 size_t delta_bytes(const WinArgs& a) { return ((size_t)a.B * a.Hq * a.T * sizeof(float) + 255) & ~(size_t)255; }
 
@@ -927,7 +930,7 @@ hipError_t launch_window_attention_bwd(const WindowParams& p, const float* lse, 
     a.dq = out_head(dq); a.dk = out_head(dk); a.dv = out_head(dv);
     a.lse = const_cast<float*>(lse);
     a.delta = reinterpret_cast<float*>(ws);
-    a.dmax = reinterpret_cast<float*>(reinterpret_cast<char*>(ws) + delta_bytes(a));
+    a.dmax = reinterpret_cast<f32x2*>(reinterpret_cast<char*>(ws) + delta_bytes(a));
     a.part = reinterpret_cast<float*>(reinterpret_cast<char*>(a.dmax) + dmax_bytes(a));
     a.far_chunk = FAR_CHUNK;
     a.far_blocks = far_blocks_of(p.T, a.left, a.sinks);

@@ -104,7 +104,7 @@ __global__ __launch_bounds__(ST_WAVES * 64) void window_step_kernel(StepArgs a) 
                 norm_rope_lane<FMT, D>(nk, w, pw, t, a.eps, y);
                 u32x4 r;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) r[i] = Op<FMT>::pack2(y[2 * i], y[2 * i + 1]);
+                for (int i = 0; i < 4; ++i) r[i] = result2<FMT>(y[2 * i], y[2 * i + 1]);
                 nk = __builtin_bit_cast(u16x8, r);
             }
         } else {
@@ -230,7 +230,7 @@ __global__ __launch_bounds__(ST_WAVES * 64) void window_step_kernel(StepArgs a) 
             acc = fmaf(red_o[w][i][d], corr, acc);
         }
         if (a.splits == 1) {
-            a.out[((long)b * a.Hq + hk * grp + g0 + i) * D + d] = Op<FMT>::pack(acc / sum);
+            a.out[((long)b * a.Hq + hk * grp + g0 + i) * D + d] = (bf16_t)result2<FMT>(acc / sum, 0.f);
         } else {
             a.acc[(share + (long)i * a.splits) * D + d] = acc;
             if (d == 0) *reinterpret_cast<f32x2*>(a.ml + (share + (long)i * a.splits) * 2) = f32x2{mx, sum};
@@ -285,7 +285,7 @@ __global__ __launch_bounds__(256) void window_step_join_kernel(const float* __re
     const float inv = total == 0.f ? 0.f : 1.0f / total;
     typedef __attribute__((ext_vector_type(2))) uint32_t u32x2_t;
     *reinterpret_cast<u32x2_t*>(out + (long)blockIdx.x * D + c * 4) =
-        u32x2_t{Op<FMT>::pack2(s[0] * inv, s[1] * inv), Op<FMT>::pack2(s[2] * inv, s[3] * inv)};
+        u32x2_t{result2<FMT>(s[0] * inv, s[1] * inv), result2<FMT>(s[2] * inv, s[3] * inv)};
 }
 
 // k, v [B][T] heads -> the slots their newest positions live in; slots without a position keep what they hold

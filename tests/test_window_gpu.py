@@ -603,3 +603,55 @@ def test_half_precision_gradient_of_quiet_rows_beside_loud_ones():
     dq, _, _ = ops.window_attention_backward(do, q, k, v, out, lse, 1, 1)
     u = unit(torch.float16)
     close(dq, r["dq"], u * (r["dq"].abs() + 3 * r["Mq"]) + 3 * SLACK * r["Mq"] + 2 ** -25, "dq")
+
+
+@pytest.mark.parametrize("size", [1000.0, 2.0 ** -9])
+def test_half_precision_key_gradients_with_large_and_small_values(size):
+    """dK under a loss scale, values of a thousand; and with values of thousandths beside ordinary ones in turn."""
+    q, k, v, _ = win_case(1, 300, 2, 1, 64, 20, 20, 0, None, torch.float16)
+    v = v * torch.where(torch.arange(300, device=DEV) % 2 == 0, size, 1.0).half()[None, :, None, None]
+    do = rnd(1, 300, 2, 64, seed=9, dtype=torch.float16) * (256 if size > 1 else 2.0 ** -6)
+    scale = 2.0 ** (-10 if size > 1 else -3)
+    out, lse = ops.window_attention(q, k, v, 20, 20, scale=scale, return_lse=True)
+    r = attention64(q, k, v, None, 20, 20, 0, scale, do)
+    assert bool((r["dk"].abs().max() < 60000) & (r["dv"].abs().max() < 60000))
+    _, dk, dv = ops.window_attention_backward(do, q, k, v, out, lse, 20, 20, scale=scale)
+    u = unit(torch.float16)
+    for g, n, m, c in ((dk, "dk", "Mk", 3), (dv, "dv", "Mv", 1)):
+        close(g, r[n], u * (r[n].abs() + c * r[m]) + 3 * SLACK * r[m] + 2 ** -25, n)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_infinities_and_nan_reach_what_sees_them(dtype):
+    """A NaN among the values makes the rows that see it NaN, one in dout its row's dq and the dv of the keys it sees; the
+    norms keep one, and an infinity in dout stays out of range rather than becoming a large number."""
+    case = (1, 300, 2, 2, 64, 20, 4, 0, None)
+    q, k, v, _ = win_case(*case, dtype)
+    do = rnd(1, 300, 2, 64, seed=9, dtype=dtype)
+    out, lse = ops.window_attention(q, k, v, 20, 4, return_lse=True)
+    bad = v.clone()
+    bad[0, 100, 1, 7] = math.nan
+    got = ops.window_attention(q, k, bad, 20, 4)
+    assert bool(got[0, 96:121, 1, 7].isnan().all())
+    far = torch.ones(300, dtype=torch.bool, device=DEV)
+    far[0:256] = False     # (tiles of up to 64 keys, workgroups of 128 rows: beyond these nothing is near)
+    assert torch.equal(got[:, far], out[:, far]) and torch.equal(got[:, :, 0], out[:, :, 0])
+    for value in (math.nan, math.inf):
+        bad = do.clone()
+        bad[0, 100, 1, 7] = value
+        dq, dk, dv = ops.window_attention_backward(bad, q, k, v, out, lse, 20, 4)
+        assert not bool(dq[0, 100, 1].isfinite().any()) and not bool(dv[0, 80:105, 1, 7].isfinite().any())
+        assert not bool(dk[0, 80:105, 1].isfinite().any())
+        assert all(bool(t[:, :, 0].isfinite().all()) and bool(t[:, 256:].isfinite().all()) for t in (dq, dk, dv))
+    x = rnd(5, 3 * 64, seed=4, dtype=dtype)
+    x[2, 70] = math.nan
+    w = torch.ones(64, device=DEV)
+    y = ops.qk_norm_rope(x, 2, 1, w, w, freqs_of(64))
+    assert bool(y[2, 64:128].isnan().all()) and int(y.isnan().sum()) == 64
+    dx, dwq, dwk = ops.qk_norm_rope_backward(rnd(5, 192, seed=5, dtype=dtype), x, 2, 1, w, w, freqs_of(64))
+    assert bool(dx[2, 64:128].isnan().all()) and int(dx.isnan().sum()) == 64 and bool(dwk.isfinite().all())
+    assert bool(dwq.isnan().all())
+    cache = [rnd(1, 2, 40, 64, seed=i, dtype=dtype) for i in (6, 7)]
+    cache[1][0, 1, 3, 5] = math.nan
+    o = ops.window_attention_step(rnd(1, 6 * 64, seed=8, dtype=dtype), *cache, torch.tensor([100], device=DEV), 2, 0)
+    assert bool(o[0, 1, 5].isnan()) and int(o.isnan().sum()) == 1
