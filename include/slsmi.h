@@ -618,13 +618,14 @@ size_t slsmi_window_topk_scratch_bytes(int B, int T, int dict, int window);
  * rotary_dim channels of n as pairs turned by p * freqs[i] radians: (n_i, n_(i + rotary_dim / 2)), or with interleaved != 0
  * (n_2i, n_(2i + 1)).  freqs [rotary_dim / 2] doubles; rotary_dim a multiple of 16 up to head_dim, or 0 with freqs NULL.
  * p = positions[row % npos] (int64, device), or row % npos where positions is NULL: npos = rows, or frames per recording.
- * Angles are formed in 64 bits.  y [rows][ldy] may be x itself.  ldx, ldy multiples of 8, pointers 16-byte aligned. */
+ * Angles are formed in 64 bits.  y [rows][ldy] may be x itself, else shares no memory with it.  At most 2^25 rows.  ldx, ldy multiples of 8, pointers 16-byte aligned. */
 int slsmi_qk_norm_rope(const uint16_t* x, int64_t ldx, uint16_t* y, int64_t ldy, int64_t rows, int heads, int kv_heads,
                        int head_dim, const float* wq, const float* wk, float eps, const double* freqs, int rotary_dim,
                        int interleaved, const int64_t* positions, int64_t npos, int fmt, void* stream);
 
 /* Its gradient: dy at y, x as given to the forward (not its result) -> dx [rows][lddx] (may be dy itself; columns past the
- * heads are left alone) and dwq, dwk [head_dim] fp32, written whole (rows == 0: zeros), summed in a fixed order.
+ * heads are left alone) and dwq, dwk [head_dim] fp32, written whole (rows == 0: zeros), summed in a fixed order.  A head
+ * whose dy is all zeros (a padded frame's) may hold anything: its dx is zero and it adds nothing to dwq, dwk.
  * workspace: slsmi_qk_norm_rope_backward_workspace_bytes() bytes, 16-byte aligned, free again when the call's work is done. */
 int slsmi_qk_norm_rope_backward(const uint16_t* dy, int64_t lddy, const uint16_t* x, int64_t ldx, uint16_t* dx, int64_t lddx,
                                 int64_t rows, int heads, int kv_heads, int head_dim, const float* wq, const float* wk,
@@ -647,18 +648,21 @@ typedef struct slsmi_window_shape {
     int32_t left, right;       /* frames a query sees before and after itself; -1: no limit; right 0: causal */
     int32_t sinks;             /* 0 .. 128: first frames that stay visible to every later query */
     int32_t fmt;
-    float scale;               /* of the scores, > 0 */
+    float scale;               /* of the scores, 2^-64 .. 2^64 */
 } slsmi_window_shape;
 
 /* Attention with a sliding window and sinks: query i of a recording of n frames (nframes [batch] int32 on the device,
  * clamped to [0, frames]; NULL: frames) sees key j where j < n, j <= i + right and (j >= i - left or j < sinks).
  * out rows of padded frames are written as zeros; what q, k, v hold there is never used.  lse: NULL or fp32
- * [batch][heads][frames], the log of the sum of exponentials per row (-inf at padded frames): what the backward needs. */
+ * [batch][heads][frames], the log of the sum of exponentials per row (-inf at padded frames): what the backward needs.
+ * out may be q, but shares no memory with k and v.  What a recording's own frames hold is finite: an infinity or NaN
+ * there reaches the rows that see it and may reach others up to a tile away.  batch * heads * (frames / 128, rounded up)
+ * stays below 2^24, in the backward both sides together. */
 int slsmi_window_attention(const slsmi_window_shape* shape, const slsmi_heads* q, const slsmi_heads* k, const slsmi_heads* v,
                            const slsmi_heads* out, float* lse, const int32_t* nframes, void* stream);
 
 /* Its gradient, from the forward's out and lse: dq, dk, dv written whole (zeros at padded frames), the same bits on every
- * call.  workspace: slsmi_window_attention_backward_workspace_bytes() bytes, 16-byte aligned. */
+ * call; they share memory with nothing that is read, nor with each other.  workspace: slsmi_window_attention_backward_workspace_bytes() bytes, 16-byte aligned. */
 int slsmi_window_attention_backward(const slsmi_window_shape* shape, const slsmi_heads* dout, const slsmi_heads* q,
                                     const slsmi_heads* k, const slsmi_heads* v, const slsmi_heads* out, const float* lse,
                                     const int32_t* nframes, const slsmi_heads* dq, const slsmi_heads* dk,

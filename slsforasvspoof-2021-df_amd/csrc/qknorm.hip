@@ -249,10 +249,12 @@ __global__ __launch_bounds__(1024) void qk_norm_dw_kernel(const float* __restric
     if (rg == 0) (col < D ? dwq : dwk)[col < D ? col : col - D] = red[0][lc];
 }
 
+constexpr long ROWS_MAX = 1L << 25;   // the forward's launch counts 64 work-items a row in 32 bits
+
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 bool qk_norm_ok(const QkNormParams& p) {
-    if (p.rows < 0 || p.rows > 0x7fffffffL || p.Hq < 0 || p.Hk < 0 || p.Hq + p.Hk < 1 || p.Hq + p.Hk > 4096) return false;
+    if (p.rows < 0 || p.rows > ROWS_MAX || !eps_ok(p.eps) || p.Hq < 0 || p.Hk < 0 || p.Hq + p.Hk < 1 || p.Hq + p.Hk > 4096) return false;
     if (p.D != 64 && p.D != 128) return false;
     if (p.half < 0 || 2 * p.half > p.D || p.half % 8 != 0 || (p.half > 0 && !p.freqs)) return false;
     const long width = (long)(p.Hq + p.Hk) * p.D;

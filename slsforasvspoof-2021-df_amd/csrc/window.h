@@ -43,6 +43,10 @@ __device__ __forceinline__ float lane_group_sum(float v) {
     return v;
 }
 
+// Scales of scores whose inverse and whose products with ordinary scores 32 bits hold.
+inline bool scale_ok(float scale) { return scale >= 0x1p-64f && scale <= 0x1p64f; }
+inline bool eps_ok(float eps) { return eps >= 0.f && eps < INFINITY; }
+
 // Norm of one head and its position rotation (slsmi_qk_norm_rope), the part of one lane.  D / 8 consecutive lanes hold a
 // head, eight channels each (chunk c = lane within the head).  x: the lane's raw channels; w: their weights; px, pw: the
 // same of the lane that holds the other members of the pairs (chunk c +- R / 16; not read where pairs are neighbours);

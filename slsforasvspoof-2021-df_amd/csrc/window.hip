@@ -14,6 +14,7 @@
 #include "kernels.h"
 #include "window.h"
 
+#include <initializer_list>
 #include <type_traits>
 
 namespace slsmi {
@@ -825,6 +826,7 @@ __global__ __launch_bounds__(1024) void window_sink_kernel(WinArgs a) {
 }
 
 constexpr int FAR_CHUNK = 1024;
+constexpr long WG_MAX = 0xffffffffL / 256;   // workgroups of 256 in a launch, whose work-items a 32-bit number counts
 
 // queries past the near ones of the first sink block, in chunks (0: none)
 int far_blocks_of(int T, int left, int sinks) {
@@ -842,13 +844,20 @@ bool head_ok(const WindowHeads& x, int heads, int T, int D) {
     return true;
 }
 
+// a result that other workgroups would still read
+bool clashes(const WindowHeads& y, std::initializer_list<const WindowHeads*> others) {
+    for (const WindowHeads* x : others)
+        if (x->p == y.p) return true;
+    return false;
+}
+
 // the ranges every call has to keep; clamps the window
 bool window_args(const WindowParams& p, WinArgs& a) {
     if (p.B < 0 || p.B > 65535 || p.T < 0 || p.T > (1 << 29) || p.Hk < 1 || p.Hq < p.Hk || p.Hq % p.Hk || p.Hq > 4096) return false;
     if (p.D != 64 && p.D != 128) return false;
     if (p.fmt != FMT_BF16 && p.fmt != FMT_F16) return false;
-    if (!(p.scale > 0.f) || p.left < -1 || p.right < -1 || p.sinks < 0 || p.sinks > SINK_MAX) return false;
-    if ((long)p.B * p.Hq * ((p.T + 127L) / 128 + 4) > 0x7fffffffL / 8) return false;
+    if (!scale_ok(p.scale) || p.left < -1 || p.right < -1 || p.sinks < 0 || p.sinks > SINK_MAX) return false;
+    if ((long)p.B * p.Hq * ((p.T + 127L) / 128) > WG_MAX) return false;
     a.B = p.B; a.T = p.T; a.Hq = p.Hq; a.Hk = p.Hk;
     a.left = p.left < 0 || p.left > p.T ? p.T : p.left;
     a.right = p.right < 0 || p.right > p.T ? p.T : p.right;
@@ -900,7 +909,7 @@ hipError_t launch_window_attention(const WindowParams& p, float* lse, hipStream_
     if (!window_args(p, a)) return hipErrorInvalidValue;
     if (p.B == 0 || p.T == 0) return hipSuccess;
     if (!head_ok(p.q, p.Hq, p.T, p.D) || !head_ok(p.k, p.Hk, p.T, p.D) || !head_ok(p.v, p.Hk, p.T, p.D) ||
-        !head_ok(p.o, p.Hq, p.T, p.D))
+        !head_ok(p.o, p.Hq, p.T, p.D) || clashes(p.o, {&p.k, &p.v}))
         return hipErrorInvalidValue;
     a.q = in_head(p.q); a.k = in_head(p.k); a.v = in_head(p.v); a.out = out_head(p.o);
     a.lse = lse;
@@ -925,6 +934,9 @@ hipError_t launch_window_attention_bwd(const WindowParams& p, const float* lse, 
         !head_ok(p.o, p.Hq, p.T, p.D) || !head_ok(dout, p.Hq, p.T, p.D) || !head_ok(dq, p.Hq, p.T, p.D) ||
         !head_ok(dk, p.Hk, p.T, p.D) || !head_ok(dv, p.Hk, p.T, p.D) || !lse)
         return hipErrorInvalidValue;
+    if (clashes(dq, {&p.q, &p.k, &p.v, &p.o, &dout, &dk, &dv}) || clashes(dk, {&p.q, &p.k, &p.v, &p.o, &dout, &dv}) ||
+        clashes(dv, {&p.q, &p.k, &p.v, &p.o, &dout}))
+        return hipErrorInvalidValue;
     if (!ws || ((uintptr_t)ws & 15) || ws_bytes < window_attention_bwd_workspace(p)) return hipErrorOutOfMemory;
     a.q = in_head(p.q); a.k = in_head(p.k); a.v = in_head(p.v); a.o = in_head(p.o); a.d = in_head(dout);
     a.dq = out_head(dq); a.dk = out_head(dk); a.dv = out_head(dv);
@@ -934,6 +946,10 @@ hipError_t launch_window_attention_bwd(const WindowParams& p, const float* lse, 
     a.part = reinterpret_cast<float*>(reinterpret_cast<char*>(a.dmax) + dmax_bytes(a));
     a.far_chunk = FAR_CHUNK;
     a.far_blocks = far_blocks_of(p.T, a.left, a.sinks);
+    const long sb = (a.sinks + 31) / 32, heads = (long)p.B * p.Hk;
+    if (heads * (a.tiles + sb * a.far_blocks) + 8 + (long)p.B * p.Hq * a.tiles > WG_MAX ||
+        (a.far_blocks > 0 && heads * sb * (p.D / 16) > WG_MAX / 4))
+        return hipErrorInvalidValue;
     hipError_t rc = hipSuccess;
     SLSMI_FMT_DISPATCH(p.fmt, rc = p.D == 64 ? (launch_bwd<F, 64>(a, s)) : (launch_bwd<F, 128>(a, s)));
     return rc;

@@ -370,7 +370,7 @@ hipError_t launch_window_step(const WindowStepParams& p, void* ws, size_t ws_byt
     auto al = [](const void* x) { return x && ((uintptr_t)x & 15) == 0; };
     if (!al(p.qkv) || !al(p.k_cache) || !al(p.v_cache) || !p.positions || !al(p.out) || p.ld % 8) return hipErrorInvalidValue;
     if (p.B > 1 && p.ld < (long)(p.Hq + 2 * p.Hk) * p.D) return hipErrorInvalidValue;
-    if ((p.wq == nullptr) != (p.wk == nullptr) || !(p.scale > 0.f)) return hipErrorInvalidValue;
+    if ((p.wq == nullptr) != (p.wk == nullptr) || (p.wq && !eps_ok(p.eps)) || !scale_ok(p.scale)) return hipErrorInvalidValue;
     if (p.half < 0 || 2 * p.half > p.D || p.half % 8 || (p.half > 0 && (!p.freqs || !p.wq))) return hipErrorInvalidValue;
     StepArgs a{};
     a.qkv = p.qkv; a.ld = p.ld; a.kc = p.k_cache; a.vc = p.v_cache; a.positions = p.positions; a.out = p.out;

@@ -569,8 +569,8 @@ def _window_shape(q: torch.Tensor, k: torch.Tensor, left, right, sinks: int, sca
     if not 0 <= sinks <= 128:
         _refuse(f"sinks: 0 to 128 first frames, got {sinks}")
     scale = D ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < float("inf"):
-        _refuse(f"scale must be positive, got {scale}")
+    if not 2.0 ** -64 <= scale <= 2.0 ** 64:
+        _refuse(f"scale must lie in [2^-64, 2^64], got {scale}")
     return qs, (B, T, kv, D), _SHAPE.pack(B, T, H, kv, D, _window_side(left, "left"), _window_side(right, "right"), sinks, fmt, scale)
 
 
@@ -786,8 +786,8 @@ def window_attention_step(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: tor
     elif freqs is not None:
         _refuse("the rotation needs both norm weights")
     scale = D ** -0.5 if scale is None else float(scale)
-    if not 0.0 < scale < float("inf"):
-        _refuse(f"scale must be positive, got {scale}")
+    if not 2.0 ** -64 <= scale <= 2.0 ** 64:
+        _refuse(f"scale must lie in [2^-64, 2^64], got {scale}")
     shape = _SHAPE.pack(B, 1, heads, Hk, D, -1, 0, sinks, fmt, scale)
     out = qkv.new_empty((B, heads, D))
     lib = _lib.load()

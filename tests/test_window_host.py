@@ -119,3 +119,51 @@ def test_cache_fill_refuses():
 
     assert call(shape(), slots=4) == INVALID and call(shape(), k=heads(PTR + 2)) == INVALID and call(shape(), kc=None) == INVALID
     assert call(shape(head_dim=80)) == INVALID and call(shape(), k=heads(row=100)) == INVALID and call(shape(batch=0)) == 0
+
+
+@pytest.mark.parametrize("kw", [dict(scale=2.0 ** -65), dict(scale=2.0 ** 65), dict(scale=float("inf")), dict(batch=1 << 13, heads=4096, frames=1),
+                                dict(batch=1, heads=64, kv_heads=64, frames=1 << 26)])
+def test_launches_that_could_not_be_counted_and_scales_without_an_inverse(kw):
+    s = shape(**kw)
+    lib = _lib.load()
+    h = [C.byref(heads(PTR * (i + 1), row=512, batch=0)) for i in range(8)]
+    assert lib.slsmi_window_attention(C.byref(s), h[0], h[1], h[2], h[3], None, None, None) == INVALID
+    assert lib.slsmi_window_attention_backward(C.byref(s), *h[:5], PTR, None, *h[5:], PTR, 1 << 60, None) == INVALID
+
+
+def test_backward_refuses_too_many_workgroups_of_both_sides_and_of_the_sinks():
+    """Forwards that can be launched whose backward cannot."""
+    lib = _lib.load()
+    for s in (shape(batch=1, heads=64, kv_heads=64, frames=1 << 24, left=-1, sinks=0),
+              shape(batch=4096, heads=64, kv_heads=64, frames=300, left=0, sinks=128)):
+        h = [C.byref(heads(PTR * (i + 1), row=64 * 64, batch=0)) for i in range(8)]
+        need = lib.slsmi_window_attention_backward_workspace_bytes(C.byref(s))
+        assert need > 0
+        assert lib.slsmi_window_attention_backward(C.byref(s), *h[:5], PTR, None, *h[5:], PTR, need, None) == INVALID
+
+
+def test_results_in_the_place_of_what_is_read():
+    lib = _lib.load()
+    s = shape()
+    need = lib.slsmi_window_attention_backward_workspace_bytes(C.byref(s))
+    at = [heads(PTR * (i + 1)) for i in range(8)]   # dout q k v out dq dk dv
+    for target, other in [(3, 1), (3, 2)]:
+        args = [C.byref(at[other] if i == target else at[i]) for i in range(4)]
+        assert lib.slsmi_window_attention(C.byref(s), *args, None, None, None) == INVALID
+    for target in (5, 6, 7):
+        for other in range(8):
+            if other != target:
+                h = [C.byref(at[other] if i == target else at[i]) for i in range(8)]
+                assert lib.slsmi_window_attention_backward(C.byref(s), *h[:5], PTR, None, *h[5:], PTR, need, None) == INVALID
+
+
+@pytest.mark.parametrize("eps", [-1e-6, float("nan"), float("inf")])
+def test_norms_refuse_an_eps_without_a_root_and_more_rows_than_a_launch_counts(eps):
+    lib = _lib.load()
+
+    def norm(rows=8, eps=1e-6):
+        return lib.slsmi_qk_norm_rope(PTR, 256, 2 * PTR, 256, rows, 2, 1, 64, PTR, PTR, eps, None, 0, 0, None, rows, 1, None)
+    assert norm(eps=eps) == INVALID and norm(rows=(1 << 25) + 1) == INVALID
+    s = shape(frames=1, left=0)
+    assert lib.slsmi_window_step(C.byref(s), 40, PTR, 512, 2 * PTR, 3 * PTR, PTR, PTR, PTR, eps, None, 0, 0, 4 * PTR, None, 0,
+                                 None) == INVALID
