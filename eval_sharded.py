@@ -98,7 +98,7 @@ def main() -> int:
     ap.add_argument("--max_seconds", type=float, default=10.0)
     ap.add_argument("--attention_window", type=int, nargs=2, metavar=("BEFORE", "AFTER"), default=None,
                     help="in-tree heads: the encoder attends by a sliding window of so many frames before and after (-1: no "
-                         "limit; 50 frames a second), which takes recordings of up to 16384 frames (raise --max_seconds)")
+                         "limit; 50 frames a second), which takes recordings of up to 16384 frames (--variable_length --max_seconds 327)")
     ap.add_argument("--attention_sinks", type=int, default=0,
                     help="with --attention_window: first frames that stay visible (0 to 128)")
     ap.add_argument("--max_frames", type=int, default=0,
@@ -143,9 +143,12 @@ def main() -> int:
 
     t0 = time.perf_counter()
     if args.variable_length:
+        budget = args.max_frames if args.max_frames > 0 else None
+        if budget is None and args.attention_window:   # what a batch of long recordings may hold (slsmi_set_attention_window)
+            budget = 32768
         loader = data.VariableLengthLoader(ds, args.batch_size if args.max_frames <= 0 else 4 * args.batch_size, device,
                                            args.decode_threads, max_len=int(args.max_seconds * data.SAMPLE_RATE),
-                                           rank=rank, world=world, max_frames=args.max_frames if args.max_frames > 0 else None)
+                                           rank=rank, world=world, max_frames=budget)
         if args.quick_test:
             loader.batches = loader.batches[:5]
             ids_scored = sorted(j for idx, _ in loader.batches for j in idx)

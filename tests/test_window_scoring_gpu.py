@@ -137,3 +137,30 @@ def test_the_longest_recording():
     scale = x.pow(2).mean().sqrt()
     for whole, own in ((x[:, :400], head[:, :400]), (x[:, -400:], tail[:, -400:])):
         assert ((whole - own).pow(2).mean().sqrt() / scale).item() < 2 * LAYER_RMS["f16"]
+
+
+def test_eval_driver_scores_long_recordings(tmp_path):
+    """eval_sharded.py --variable_length --attention_window: thirteen recordings of 62 to 68 seconds and a short one at the default batch size;
+    together the long ones exceed what one batch may hold, and every trial gets its score."""
+    import os
+    import subprocess
+    import sys
+    import wave
+    import numpy as np
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    rng = np.random.default_rng(3)
+    ids = [f"{i}.wav" for i in range(14)]
+    for i, u in enumerate(ids):
+        n = 48000 if i == 13 else 16000 * 62 + 8000 * i
+        with wave.open(str(tmp_path / u), "wb") as w:
+            w.setnchannels(1), w.setsampwidth(2), w.setframerate(16000)
+            w.writeframes((rng.standard_normal(n) * 3000).clip(-32768, 32767).astype("<i2").tobytes())
+    (tmp_path / "trials.txt").write_text("".join(u + "\n" for u in ids))
+    out = tmp_path / "scores.txt"
+    r = subprocess.run([sys.executable, os.path.join(root, "eval_sharded.py"), "--track", "In-the-Wild", "--synthetic_weights",
+                        "--database_path", str(tmp_path) + "/", "--protocols_path", str(tmp_path / "trials.txt"),
+                        "--variable_length", "--max_seconds", "327", "--attention_window", "100", "100",
+                        "--attention_sinks", "4", "--eval_output", str(out)], capture_output=True, text=True, timeout=110)
+    assert r.returncode == 0, r.stdout[-1000:] + r.stderr[-3000:]
+    lines = [line.split() for line in out.read_text().splitlines()]
+    assert [u for u, _ in lines] == ids and all(0.0 <= float(s) <= 1.0 for _, s in lines)
