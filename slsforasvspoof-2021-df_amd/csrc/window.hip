@@ -316,7 +316,7 @@ __global__ __launch_bounds__(256, fwd_waves(D)) void window_fwd_kernel(WinArgs a
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const unsigned w = xcd_order(blockIdx.x, gridDim.x);
     const int tile = a.tiles - 1 - (int)(w % a.tiles);   // the tiles with the longest key ranges first
-    const int bh = w / a.tiles, b = bh / a.Hq, h = bh % a.Hq, hk = h / (a.Hq / a.Hk);
+    const int b = w / a.tiles % a.B, h = w / a.tiles / a.B, bh = b * a.Hq + h, hk = h / (a.Hq / a.Hk);
     const int len = frames_of(a, b);
     const int q0 = tile * 128, qw = q0 + wave * 32, q = qw + col;
     bf16_t* const orow = a.out.p + b * a.out.b + h * a.out.h + (long)q * a.out.r;
@@ -506,7 +506,7 @@ __device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* ld
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, hi = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int tile = a.tiles - 1 - (int)(w % a.tiles);
-    const int bh = w / a.tiles, b = bh / a.Hq, h = bh % a.Hq, hk = h / (a.Hq / a.Hk);
+    const int b = w / a.tiles % a.B, h = w / a.tiles / a.B, bh = b * a.Hq + h, hk = h / (a.Hq / a.Hk);
     const int len = frames_of(a, b);
     const int q0 = tile * 128, qw = q0 + wave * 32, q = qw + col;
     bf16_t* const dqrow = a.dq.p + b * a.dq.b + h * a.dq.h + (long)q * a.dq.r;
@@ -612,7 +612,7 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int sink_blocks = (a.sinks + 31) / 32;
     const int per_head = a.tiles + sink_blocks * a.far_blocks;
-    const int bh = w / per_head, item = w % per_head, b = bh / a.Hk, hk = bh % a.Hk;
+    const int item = w % per_head, b = w / per_head % a.B, hk = w / per_head / a.B, bh = b * a.Hk + hk;
     const int len = frames_of(a, b);
     const int grp = a.Hq / a.Hk;
     const bool far = item >= a.tiles;
