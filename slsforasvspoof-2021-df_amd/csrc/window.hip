@@ -22,6 +22,8 @@ namespace slsmi {
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
+template <int N>
+using Const = std::integral_constant<int, N>;
 constexpr float LN2 = 0.6931471805599453f;
 
 // Waves per SIMD the kernels are built for: the most that registers allow without spilling (128 / 168 / 256 per wave).
@@ -71,19 +73,34 @@ __device__ __forceinline__ int tile_at(int row, int chunk) {
     return row * D * 2 + ((chunk ^ chunk_turn<D>(row)) << 4);
 }
 
-// Byte offsets inside a tile of what a lane reads: the row operand of rows 0 .. 31 per 16 columns, and the transposed
-// operand (rows as columns' neighbours) of rows 0 .. 15 per 32 columns; other rows of a tile lie a constant further.
+__device__ __forceinline__ uint32_t lds_offset(const char* p) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
+}
+
+// What a lane reads of a tile: the row operand of rows 0 .. 31 per 16 columns, as byte offsets, and the transposed operand
+// (rows as columns' neighbours) of rows 0 .. 15 per 32 columns, as LDS addresses in the current one of two buffers; other
+// rows and tiles lie a constant further, which the instruction holds.
 template <int D>
 struct LaneAt {
-    int row[D / 16], tr[D / 32][2];
-    __device__ __forceinline__ explicit LaneAt(int lane) {
+    int row[D / 16];
+    uint32_t tr[D / 32][2];
+    __device__ __forceinline__ LaneAt(int lane, const char* lds) {
+        const uint32_t base = lds_offset(lds);
 #pragma unroll
         for (int e = 0; e < D / 16; ++e) row[e] = tile_at<D>(lane & 31, 2 * e + (lane >> 5));
 #pragma unroll
         for (int dt = 0; dt < D / 32; ++dt) {
             const int r = ((lane >> 5) << 2) + ((lane & 15) >> 2), c = dt * 32 + (lane & 16) + (lane & 3) * 4;
-            tr[dt][0] = tile_at<D>(r, c >> 3) + (c & 4) * 2;
-            tr[dt][1] = tile_at<D>(r + 8, c >> 3) + (c & 4) * 2;
+            tr[dt][0] = base + tile_at<D>(r, c >> 3) + (c & 4) * 2;
+            tr[dt][1] = base + tile_at<D>(r + 8, c >> 3) + (c & 4) * 2;
+        }
+    }
+    // to the other buffer, `by` bytes away
+    __device__ __forceinline__ void turn(int by) {
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) {
+            tr[dt][0] += by;
+            tr[dt][1] += by;
         }
     }
 };
@@ -92,18 +109,15 @@ template <int D>
 __device__ __forceinline__ u16x8 row_frag(const char* tile, int row0, const LaneAt<D>& at, int e) {
     return *reinterpret_cast<const u16x8*>(tile + row0 * D * 2 + at.row[e]);
 }
-__device__ __forceinline__ uint32_t lds_offset(const char* p) {
-    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
-}
 __device__ __forceinline__ u16x8 tr_pair(s16x4 lo, s16x4 hi) {
     return __builtin_bit_cast(u16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-// A operands of a transposed product for all column blocks (32 columns each) of the 16 rows that lie `OFF` bytes past
-// `tile`, rows enumerated as above.  The transposed read's builtin makes the compiler wait for every load into LDS that is
+// A operands of a transposed product for all column blocks (32 columns each) of the 16 rows that lie `OFF` bytes past the
+// buffer's begin, rows enumerated as above.  The transposed read's builtin makes the compiler wait for every load into LDS that is
 // under way (the next tile's), so the reads are written out, with their wait in the same block.
 template <int D, int OFF>
-__device__ __forceinline__ void tr_frags(uint32_t tile, const LaneAt<D>& at, u16x8 (&f)[D / 32]) {
+__device__ __forceinline__ void tr_frags(const LaneAt<D>& at, u16x8 (&f)[D / 32]) {
 #pragma unroll
     for (int d = 0; d < D / 32; d += 2) {
         s16x4 r0, r1, r2, r3;
@@ -113,7 +127,7 @@ __device__ __forceinline__ void tr_frags(uint32_t tile, const LaneAt<D>& at, u16
                      "ds_read_b64_tr_b16 %3, %7 offset:%8\n\t"
                      "s_waitcnt lgkmcnt(0)"
                      : "=&v"(r0), "=&v"(r1), "=&v"(r2), "=&v"(r3)
-                     : "v"(tile + at.tr[d][0]), "v"(tile + at.tr[d][1]), "v"(tile + at.tr[d + 1][0]), "v"(tile + at.tr[d + 1][1]), "n"(OFF)
+                     : "v"(at.tr[d][0]), "v"(at.tr[d][1]), "v"(at.tr[d + 1][0]), "v"(at.tr[d + 1][1]), "n"(OFF)
                      : "memory");
         f[d] = tr_pair(r0, r1);
         f[d + 1] = tr_pair(r2, r3);
@@ -121,7 +135,7 @@ __device__ __forceinline__ void tr_frags(uint32_t tile, const LaneAt<D>& at, u16
 }
 // the same for two 16-row steps, OFF and OFF + 32 D bytes
 template <int D, int OFF>
-__device__ __forceinline__ void tr_frags2(uint32_t tile, const LaneAt<D>& at, u16x8 (&f)[2][D / 32]) {
+__device__ __forceinline__ void tr_frags2(const LaneAt<D>& at, u16x8 (&f)[2][D / 32]) {
 #pragma unroll
     for (int d = 0; d < D / 32; d += 2) {
         s16x4 r0, r1, r2, r3, r4, r5, r6, r7;
@@ -135,7 +149,7 @@ __device__ __forceinline__ void tr_frags2(uint32_t tile, const LaneAt<D>& at, u1
                      "ds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
                      "s_waitcnt lgkmcnt(0)"
                      : "=&v"(r0), "=&v"(r1), "=&v"(r2), "=&v"(r3), "=&v"(r4), "=&v"(r5), "=&v"(r6), "=&v"(r7)
-                     : "v"(tile + at.tr[d][0]), "v"(tile + at.tr[d][1]), "v"(tile + at.tr[d + 1][0]), "v"(tile + at.tr[d + 1][1]), "n"(OFF),
+                     : "v"(at.tr[d][0]), "v"(at.tr[d][1]), "v"(at.tr[d + 1][0]), "v"(at.tr[d + 1][1]), "n"(OFF),
                        "n"(OFF + 32 * D)
                      : "memory");
         f[0][d] = tr_pair(r0, r1);
@@ -332,7 +346,7 @@ __global__ __launch_bounds__(256, fwd_waves(D)) void window_fwd_kernel(WinArgs a
     const bf16_t* kh = a.k.p + b * a.k.b + hk * a.k.h;
     const bf16_t* vh = a.v.p + b * a.v.b + hk * a.v.h;
     const KeyTiles kt = key_tiles(q0, min(q0 + 127, len - 1), len, a.left, a.right, a.sinks, BN);
-    const LaneAt<D> at(lane);
+    LaneAt<D> at(lane, lds);
     const TileLoad<D, BN> lk(a.k.r, lane, wave), lv(a.v.r, lane, wave);
     lk.issue(kh, a.k.r, kt.tile(0) * BN, len, lds, wave);
     lv.issue(vh, a.v.r, kt.tile(0) * BN, len, lds + TILE, wave);
@@ -352,25 +366,23 @@ __global__ __launch_bounds__(256, fwd_waves(D)) void window_fwd_kernel(WinArgs a
     for (int it = 0; it < kt.n; ++it) {
         const int k0 = kt.tile(it) * BN;
         char* const Ks = lds + (it & 1) * 2 * TILE;
-        char* const Vs = Ks + TILE;
         const bool more = it + 1 < kt.n;
         if (more) {
             char* const next = lds + ((it + 1) & 1) * 2 * TILE;
             lk.issue(kh, a.k.r, kt.tile(it + 1) * BN, len, next, wave);
             lv.issue(vh, a.v.r, kt.tile(it + 1) * BN, len, next + TILE, wave);
         }
-#pragma unroll
-        for (int u = 0; u < BN / 32; ++u) {
+        const auto block = [&](auto uc) {
+            constexpr int u = decltype(uc)::value, V_AT = TILE + 64 * D * u;
             const int kb = k0 + 32 * u;
-            if (!vis.any(kb)) continue;
+            if (!vis.any(kb)) return;
             f32x16 s = zero16();
 #pragma unroll
             for (int e = 0; e < NS; ++e) s = mfma32<FMT>(row_frag<D>(Ks, 32 * u, at, e), qf[e], s);
-            const uint32_t v_at = lds_offset(Vs) + 64 * D * u;
             u16x8 vt[2][DT];
             if constexpr (D == 64) {   // (wide heads have no registers to spare for this)
                 __builtin_amdgcn_sched_barrier(0);   // the value fragments are read while the scores are multiplied
-                tr_frags2<D, 0>(v_at, at, vt);
+                tr_frags2<D, V_AT>(at, vt);
             }
             if (!vis.all(kb)) hide_keys(s, kb, kb + 4 * hi, q, len, a.left, a.right, a.sinks);
             float mx = s[0];
@@ -398,14 +410,19 @@ __global__ __launch_bounds__(256, fwd_waves(D)) void window_fwd_kernel(WinArgs a
             for (int st = 0; st < 2; ++st) {
                 const u16x8 p = pack_step<FMT>(s, st);
                 if constexpr (D != 64) {
-                    if (st == 0) tr_frags<D, 0>(v_at, at, vt[0]);
-                    else tr_frags<D, 32 * D>(v_at, at, vt[1]);
+                    if (st == 0) tr_frags<D, V_AT>(at, vt[0]);
+                    else tr_frags<D, V_AT + 32 * D>(at, vt[1]);
                 }
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) o[dt] = mfma32<FMT>(vt[st][dt], p, o[dt]);
             }
+        };
+        block(Const<0>{});
+        if constexpr (BN == 64) block(Const<1>{});
+        if (more) {
+            at.turn(it & 1 ? -2 * TILE : 2 * TILE);
+            tiles_landed();
         }
-        if (more) tiles_landed();
     }
     l = halves_sum(l);
     const bool live = q < len;
@@ -520,7 +537,7 @@ __device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* ld
     const bf16_t* kh = a.k.p + b * a.k.b + hk * a.k.h;
     const bf16_t* vh = a.v.p + b * a.v.b + hk * a.v.h;
     const KeyTiles kt = key_tiles(q0, min(q0 + 127, len - 1), len, a.left, a.right, a.sinks, BN);
-    const LaneAt<D> at(lane);
+    LaneAt<D> at(lane, lds);
     const TileLoad<D, BN> lk(a.k.r, lane, wave), lv(a.v.r, lane, wave);
     lk.issue(kh, a.k.r, kt.tile(0) * BN, len, lds, wave);
     lv.issue(vh, a.v.r, kt.tile(0) * BN, len, lds + TILE, wave);
@@ -557,10 +574,10 @@ __device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* ld
             lk.issue(kh, a.k.r, kt.tile(it + 1) * BN, len, next, wave);
             lv.issue(vh, a.v.r, kt.tile(it + 1) * BN, len, next + TILE, wave);
         }
-#pragma unroll
-        for (int u = 0; u < BN / 32; ++u) {
+        const auto block = [&](auto uc) {
+            constexpr int u = decltype(uc)::value;
             const int kb = k0 + 32 * u;
-            if (!vis.any(kb)) continue;
+            if (!vis.any(kb)) return;
             f32x16 s = zero16(), dp = start;
 #pragma unroll
             for (int e = 0; e < NS; ++e) {
@@ -569,7 +586,7 @@ __device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* ld
             }
             __builtin_amdgcn_sched_barrier(0);
             u16x8 kt2[2][DT];
-            tr_frags2<D, 0>(lds_offset(Ks) + 64 * D * u, at, kt2);
+            tr_frags2<D, 64 * D * u>(at, kt2);
             if (!vis.all(kb)) hide_keys(s, kb, kb + 4 * hi, q, len, a.left, a.right, a.sinks);
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], sc, -ls)) * dp[r];
@@ -583,8 +600,13 @@ __device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* ld
                     acc[dt] = mfma32<FMT>(kt2[st][dt], rest, acc[dt]);
                 }
             }
+        };
+        block(Const<0>{});
+        if constexpr (BN == 64) block(Const<1>{});
+        if (more) {
+            at.turn(it & 1 ? -2 * TILE : 2 * TILE);
+            tiles_landed();
         }
-        if (more) tiles_landed();
     }
     const float fin = a.scale * __builtin_amdgcn_exp2f(-lift);
     if (q < a.T) {
@@ -657,7 +679,7 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
     const float turn = __builtin_amdgcn_exp2f(ds_lift - p_lift);
     const int t0 = qa / BQ, nt = qb < qa ? 0 : qb / BQ - t0 + 1;
     const int total = nt * grp;
-    const LaneAt<D> at(lane);
+    LaneAt<D> at(lane, lds);
     const TileLoad<D, BQ> lq(a.q.r, lane, wave), ld(a.d.r, lane, wave);
     float stat = 0.f;   // thread t: -lse / scale of row t of the tile for t < BQ, then -delta of row t - BQ
     int rt = t0, rh = hk * grp;   // tile and head of the next request
@@ -696,11 +718,11 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
         char* const next = lds + ((it + 1) & 1) * BUF;
         if (more) request(next);
         if (++qt == t0 + nt) qt = t0;
-#pragma unroll
-        for (int u = 0; u < BQ / 32; ++u) {
-            if (far && (BQ == 64 ? 2 * (it & 1) + u : it & 3) != wave) continue;
+        const auto block = [&](auto uc) {
+            constexpr int u = decltype(uc)::value, Q_AT = 64 * D * u;
+            if (far && (BQ == 64 ? 2 * (it & 1) + u : it & 3) != wave) return;
             const int qs = q0 + 32 * u;
-            if (!vis.any(qs)) continue;
+            if (!vis.any(qs)) return;
             f32x16 s, dp;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
@@ -729,28 +751,32 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
                 s[r] = __builtin_amdgcn_exp2f(s[r] * sc);
                 dp[r] *= FMT == FMT_F16 ? s[r] * turn : s[r];
             }
-            const uint32_t q_at = lds_offset(Qs) + 64 * D * u;
-            auto step = [&](auto off, int st) {
-                constexpr int OFF = decltype(off)::value;
+            const auto step = [&](auto stc) {
+                constexpr int st = decltype(stc)::value, OFF = Q_AT + 32 * D * st;
                 u16x8 t[DT];
-                tr_frags<D, OFF>(q_at + TILE, at, t);
+                tr_frags<D, TILE + OFF>(at, t);
                 const u16x8 pf = pack_step<FMT>(s, st);
                 u16x8 ef, rest;
                 if constexpr (SPLIT) split_step<FMT>(dp, st, ef, rest);
                 else ef = pack_step<FMT>(dp, st);
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) av[dt] = mfma32<FMT>(t[dt], pf, av[dt]);
-                tr_frags<D, OFF>(q_at, at, t);
+                tr_frags<D, OFF>(at, t);
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) {
                     ak[dt] = mfma32<FMT>(t[dt], ef, ak[dt]);
                     if constexpr (SPLIT) ak[dt] = mfma32<FMT>(t[dt], rest, ak[dt]);
                 }
             };
-            step(std::integral_constant<int, 0>{}, 0);
-            step(std::integral_constant<int, 32 * D>{}, 1);
+            step(Const<0>{});
+            step(Const<1>{});
+        };
+        block(Const<0>{});
+        if constexpr (BQ == 64) block(Const<1>{});
+        if (more) {
+            at.turn(it & 1 ? -BUF : BUF);
+            landed(next);
         }
-        if (more) landed(next);
     }
     const float vfin = __builtin_amdgcn_exp2f(-p_lift), kfin = a.scale * __builtin_amdgcn_exp2f(-ds_lift);
     if (far || (k0w < a.sinks && a.far_blocks > 0)) {
