@@ -318,8 +318,8 @@ __device__ __forceinline__ void hide_keys(f32x16& s, int k0, int kb, int q, int 
 // ---- forward: 128 queries per workgroup, 32 per wave; key tiles in two LDS buffers (one barrier per tile).
 //
 // The running maximum `m` of a query is only a reference for the exponent: it is moved (and the sums rescaled) when a
-// tile's scores pass it by more than 2^RISE, so almost never after the first tile; probabilities stay below 2^RISE times
-// the row's largest, well inside both formats.
+// score of its wave passes it by more than 2^RISE, so almost never after the first block; probabilities stay below 2^RISE
+// times the row's largest, well inside both formats.
 constexpr float RISE = 8.f;
 
 template <int FMT, int D>
@@ -357,7 +357,7 @@ __global__ __launch_bounds__(256, fwd_waves(D)) void window_fwd_kernel(WinArgs a
         for (int s = 0; s < NS; ++s) qf[s] = *reinterpret_cast<const u16x8*>(qr + s * 16);
     }
     const float sc = a.scale * LOG2E;
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, ref = 0.f, most = -INFINITY, l = 0.f;   // most: the score that moves the reference
     f32x16 o[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] = zero16();
@@ -388,17 +388,17 @@ __global__ __launch_bounds__(256, fwd_waves(D)) void window_fwd_kernel(WinArgs a
             float mx = s[0];
 #pragma unroll
             for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-            const f32x2 two = both_halves(mx);
-            mx = fmaxf(two[0], two[1]) * sc;
-            if (__builtin_amdgcn_ballot_w64(mx > m + RISE) != 0) {   // (m starts at -inf)
-                const float mn = fmaxf(m, mx);
-                const float corr = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+            if (__builtin_amdgcn_ballot_w64(mx > most) != 0) {   // (at the first block a query sees keys of, and seldom after)
+                const f32x2 two = both_halves(mx);
+                const float mn = fmaxf(m, fmaxf(two[0], two[1]) * sc);
+                ref = mn == -INFINITY ? 0.f : mn;
+                const float corr = __builtin_amdgcn_exp2f(m - ref);   // (0 where nothing was seen yet)
                 m = mn;
+                most = (m + RISE) / sc;
                 l *= corr;
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) o[dt] *= corr;
             }
-            const float ref = m == -INFINITY ? 0.f : m;
             float sum = 0.f;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
