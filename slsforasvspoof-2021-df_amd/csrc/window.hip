@@ -39,9 +39,25 @@ struct HeadOut {
     long b, r, h;
 };
 
+// n / d by a multiplication (n below 2^24, d at least 1): m = ceil(2^(24 + bits) / d) with 2^bits >= d is off by less than
+// d / 2^(24 + bits) <= 2^-24, too little to reach the next whole number.  (A division takes a wave some hundred cycles.)
+struct Div {
+    unsigned d, m;
+    int shift;
+    Div() = default;
+    explicit Div(unsigned by) : d(by) {
+        int bits = 0;
+        while ((1u << bits) < by) ++bits;
+        shift = 24 + bits;
+        m = (unsigned)(((1ull << shift) + by - 1) / by);
+    }
+    __device__ __forceinline__ unsigned of(unsigned n) const { return (unsigned)(((unsigned long long)n * m) >> shift); }
+};
+
 struct WinArgs {
     HeadPtr q, k, v, o, d;   // o, d (dO): backward
     HeadOut out, dq, dk, dv;
+    Div by_tiles, by_item, by_batch, by_group;   // tiles, workgroups of a key head, B, Hq / Hk
     float* lse;              // [B][Hq][T]
     float* delta;            // [B][Hq][T]: rowsum(dO o O)
     f32x2* dmax;             // [B][Hq][T / DELTA_ROWS]: largest |dO|, |delta| (half precision)
@@ -289,6 +305,11 @@ __device__ __forceinline__ float halves_sum(float v) {
     return p[0] + p[1];
 }
 
+// A kernel's arguments are wanted together: where each is loaded just before its first use, a workgroup begins with five
+// round trips to the scalar cache one after the other (2500 cycles before the first tile arrives became 1600).
+__device__ __forceinline__ void want(const HeadPtr& x) { asm volatile("" ::"s"(x.p), "s"(x.b), "s"(x.r), "s"(x.h)); }
+__device__ __forceinline__ void want(const HeadOut& x) { asm volatile("" ::"s"(x.p), "s"(x.b), "s"(x.r), "s"(x.h)); }
+
 __device__ __forceinline__ int frames_of(const WinArgs& a, int b) { return a.nframes ? min(max(a.nframes[b], 0), a.T) : a.T; }
 
 // Bounds of a query's keys relative to itself, for the masked blocks: key - q in [-left, right] and below len.
@@ -326,13 +347,24 @@ template <int FMT, int D>
 __global__ __launch_bounds__(256, fwd_waves(D)) void window_fwd_kernel(WinArgs a) {
     constexpr int BN = tile_rows(D), NS = D / 16, DT = D / 32, TILE = BN * D * 2;
     extern __shared__ __attribute__((aligned(16))) char lds[];   // two buffers of a K and a V tile
+    want(a.q);
+    want(a.k);
+    want(a.v);
+    want(a.out);
+    asm volatile("" ::"s"(a.lse), "s"(a.nframes), "s"(a.T), "s"(a.left), "s"(a.right), "s"(a.sinks), "s"(a.scale));
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, hi = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const unsigned w = xcd_order(blockIdx.x, gridDim.x);
-    const int tile = a.tiles - 1 - (int)(w % a.tiles);   // the tiles with the longest key ranges first
-    const int b = w / a.tiles % a.B, h = w / a.tiles / a.B, bh = b * a.Hq + h, hk = h / (a.Hq / a.Hk);
-    const int len = frames_of(a, b);
+    const unsigned wt = a.by_tiles.of(w), h = a.by_batch.of(wt), b = wt - h * a.B, hk = a.by_group.of(h), bh = b * a.Hq + h;
+    const int tile = a.tiles - 1 - (int)(w - wt * a.tiles);   // the tiles with the longest key ranges first
     const int q0 = tile * 128, qw = q0 + wave * 32, q = qw + col;
+    u16x8 qf[NS];   // (rows of padded frames too: a column of their own in every product, which nothing reads)
+    {
+        const bf16_t* qr = a.q.p + b * a.q.b + h * a.q.h + (long)min(q, a.T - 1) * a.q.r + hi * 8;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) qf[s] = *reinterpret_cast<const u16x8*>(qr + s * 16);
+    }
+    const int len = frames_of(a, b);
     bf16_t* const orow = a.out.p + b * a.out.b + h * a.out.h + (long)q * a.out.r;
     float* const lse = a.lse ? a.lse + (long)bh * a.T + q : nullptr;
     if (q0 >= len) {
@@ -350,24 +382,17 @@ __global__ __launch_bounds__(256, fwd_waves(D)) void window_fwd_kernel(WinArgs a
     const TileLoad<D, BN> lk(a.k.r, lane, wave), lv(a.v.r, lane, wave);
     lk.issue(kh, a.k.r, kt.tile(0) * BN, len, lds, wave);
     lv.issue(vh, a.v.r, kt.tile(0) * BN, len, lds + TILE, wave);
-    u16x8 qf[NS];
-    {
-        const bf16_t* qr = a.q.p + b * a.q.b + h * a.q.h + (long)min(q, len - 1) * a.q.r + hi * 8;
-#pragma unroll
-        for (int s = 0; s < NS; ++s) qf[s] = *reinterpret_cast<const u16x8*>(qr + s * 16);
-    }
     const float sc = a.scale * LOG2E;
     float m = -INFINITY, ref = 0.f, most = -INFINITY, l = 0.f;   // most: the score that moves the reference
     f32x16 o[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] = zero16();
-    tiles_landed();
     const BlockVis vis(qw, len, a.left, a.right, a.sinks);
     for (int it = 0; it < kt.n; ++it) {
         const int k0 = kt.tile(it) * BN;
         char* const Ks = lds + (it & 1) * 2 * TILE;
-        const bool more = it + 1 < kt.n;
-        if (more) {
+        tiles_landed();
+        if (it + 1 < kt.n) {
             char* const next = lds + ((it + 1) & 1) * 2 * TILE;
             lk.issue(kh, a.k.r, kt.tile(it + 1) * BN, len, next, wave);
             lv.issue(vh, a.v.r, kt.tile(it + 1) * BN, len, next + TILE, wave);
@@ -419,10 +444,7 @@ __global__ __launch_bounds__(256, fwd_waves(D)) void window_fwd_kernel(WinArgs a
         };
         block(Const<0>{});
         if constexpr (BN == 64) block(Const<1>{});
-        if (more) {
-            at.turn(it & 1 ? -2 * TILE : 2 * TILE);
-            tiles_landed();
-        }
+        at.turn(it & 1 ? -2 * TILE : 2 * TILE);
     }
     l = halves_sum(l);
     const bool live = q < len;
@@ -522,10 +544,21 @@ __device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* ld
     constexpr int BN = tile_rows(D), NS = D / 16, DT = D / 32, TILE = BN * D * 2;
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, hi = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int tile = a.tiles - 1 - (int)(w % a.tiles);
-    const int b = w / a.tiles % a.B, h = w / a.tiles / a.B, bh = b * a.Hq + h, hk = h / (a.Hq / a.Hk);
-    const int len = frames_of(a, b);
+    const unsigned wt = a.by_tiles.of(w), h = a.by_batch.of(wt), b = wt - h * a.B, hk = a.by_group.of(h), bh = b * a.Hq + h;
+    const int tile = a.tiles - 1 - (int)(w - wt * a.tiles);
     const int q0 = tile * 128, qw = q0 + wave * 32, q = qw + col;
+    u16x8 qf[NS], df[NS];
+    {
+        const int row = min(q, a.T - 1);
+        const bf16_t* qr = a.q.p + b * a.q.b + h * a.q.h + (long)row * a.q.r + hi * 8;
+        const bf16_t* dr = a.d.p + b * a.d.b + h * a.d.h + (long)row * a.d.r + hi * 8;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            qf[s] = *reinterpret_cast<const u16x8*>(qr + s * 16);
+            df[s] = *reinterpret_cast<const u16x8*>(dr + s * 16);
+        }
+    }
+    const int len = frames_of(a, b);
     bf16_t* const dqrow = a.dq.p + b * a.dq.b + h * a.dq.h + (long)q * a.dq.r;
     if (q0 >= len) {
         if (q < a.T) {
@@ -541,17 +574,6 @@ __device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* ld
     const TileLoad<D, BN> lk(a.k.r, lane, wave), lv(a.v.r, lane, wave);
     lk.issue(kh, a.k.r, kt.tile(0) * BN, len, lds, wave);
     lv.issue(vh, a.v.r, kt.tile(0) * BN, len, lds + TILE, wave);
-    u16x8 qf[NS], df[NS];
-    {
-        const int row = min(q, len - 1);
-        const bf16_t* qr = a.q.p + b * a.q.b + h * a.q.h + (long)row * a.q.r + hi * 8;
-        const bf16_t* dr = a.d.p + b * a.d.b + h * a.d.h + (long)row * a.d.r + hi * 8;
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            qf[s] = *reinterpret_cast<const u16x8*>(qr + s * 16);
-            df[s] = *reinterpret_cast<const u16x8*>(dr + s * 16);
-        }
-    }
     const bool live = q < len;
     const float sc = a.scale * LOG2E;
     const long stat = (long)bh * a.T + min(q, len - 1);
@@ -562,14 +584,13 @@ __device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* ld
     for (int dt = 0; dt < DT; ++dt) acc[dt] = zero16();
 #pragma unroll
     for (int r = 0; r < 16; ++r) start[r] = -delta;
-    tiles_landed();
     const BlockVis vis(qw, len, a.left, a.right, a.sinks);
     for (int it = 0; it < kt.n; ++it) {
         const int k0 = kt.tile(it) * BN;
         char* const Ks = lds + (it & 1) * 2 * TILE;
         char* const Vs = Ks + TILE;
-        const bool more = it + 1 < kt.n;
-        if (more) {
+        tiles_landed();
+        if (it + 1 < kt.n) {
             char* const next = lds + ((it + 1) & 1) * 2 * TILE;
             lk.issue(kh, a.k.r, kt.tile(it + 1) * BN, len, next, wave);
             lv.issue(vh, a.v.r, kt.tile(it + 1) * BN, len, next + TILE, wave);
@@ -603,10 +624,7 @@ __device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* ld
         };
         block(Const<0>{});
         if constexpr (BN == 64) block(Const<1>{});
-        if (more) {
-            at.turn(it & 1 ? -2 * TILE : 2 * TILE);
-            tiles_landed();
-        }
+        at.turn(it & 1 ? -2 * TILE : 2 * TILE);
     }
     const float fin = a.scale * __builtin_amdgcn_exp2f(-lift);
     if (q < a.T) {
@@ -633,10 +651,10 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, hi = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int sink_blocks = (a.sinks + 31) / 32;
-    const int per_head = a.tiles + sink_blocks * a.far_blocks;
-    const int item = w % per_head, b = w / per_head % a.B, hk = w / per_head / a.B, bh = b * a.Hk + hk;
+    const unsigned wt = a.by_item.of(w), hk = a.by_batch.of(wt), b = wt - hk * a.B, bh = b * a.Hk + hk;
+    const int item = w - wt * a.by_item.d;
     const int len = frames_of(a, b);
-    const int grp = a.Hq / a.Hk;
+    const int grp = a.by_group.d;
     const bool far = item >= a.tiles;
     int k0w, qa, qb;   // this wave's keys; queries qa .. qb
     int block = 0, chunk = 0;
@@ -657,7 +675,7 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
     const int key = k0w + col;
     u16x8 kf[NS], vf[NS];
     {
-        const int row = min(key, max(len - 1, 0));
+        const int row = min(key, a.T - 1);
         const bf16_t* kr = a.k.p + b * a.k.b + hk * a.k.h + (long)row * a.k.r + hi * 8;
         const bf16_t* vr = a.v.p + b * a.v.b + hk * a.v.h + (long)row * a.v.r + hi * 8;
 #pragma unroll
@@ -702,10 +720,7 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
         if (tid < 2 * BQ) reinterpret_cast<float*>(buf + 2 * TILE)[tid] = stat;
         tiles_landed();
     };
-    if (total > 0) {
-        request(lds);
-        landed(lds);
-    }
+    if (total > 0) request(lds);
     const QueryVis vis(k0w, len, a.left, a.right, a.sinks);
     int qt = t0;
     for (int it = 0; it < total; ++it) {
@@ -714,9 +729,8 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
         char* const Ds = Qs + TILE;
         const float* const st_l = reinterpret_cast<const float*>(Qs + 2 * TILE) + 4 * hi;
         const float* const st_d = st_l + BQ;
-        const bool more = it + 1 < total;
-        char* const next = lds + ((it + 1) & 1) * BUF;
-        if (more) request(next);
+        landed(Qs);
+        if (it + 1 < total) request(lds + ((it + 1) & 1) * BUF);
         if (++qt == t0 + nt) qt = t0;
         const auto block = [&](auto uc) {
             constexpr int u = decltype(uc)::value, Q_AT = 64 * D * u;
@@ -773,10 +787,7 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
         };
         block(Const<0>{});
         if constexpr (BQ == 64) block(Const<1>{});
-        if (more) {
-            at.turn(it & 1 ? -BUF : BUF);
-            landed(next);
-        }
+        at.turn(it & 1 ? -BUF : BUF);
     }
     const float vfin = __builtin_amdgcn_exp2f(-p_lift), kfin = a.scale * __builtin_amdgcn_exp2f(-ds_lift);
     if (far || (k0w < a.sinks && a.far_blocks > 0)) {
@@ -815,6 +826,11 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
 template <int FMT, int D, bool SPLIT>
 __global__ __launch_bounds__(256, bwd_waves(D)) void window_bwd_kernel(WinArgs a, unsigned key_side, unsigned key_blocks) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
+    want(a.q);
+    want(a.k);
+    want(a.v);
+    want(a.d);
+    asm volatile("" ::"s"(a.lse), "s"(a.delta), "s"(a.nframes), "s"(a.T), "s"(a.left), "s"(a.right), "s"(a.sinks), "s"(a.scale));
     if (blockIdx.x < key_blocks) {
         if (blockIdx.x < key_side) window_dkv<FMT, D, SPLIT>(a, xcd_order(blockIdx.x, key_side), lds);
     } else {
@@ -891,6 +907,11 @@ bool window_args(const WindowParams& p, WinArgs& a) {
     a.scale = p.scale;
     a.nframes = p.nframes;
     a.tiles = (p.T + 127) / 128;
+    if (p.B > 0 && p.T > 0) {
+        a.by_tiles = a.by_item = Div(a.tiles);
+        a.by_batch = Div(p.B);
+        a.by_group = Div(p.Hq / p.Hk);
+    }
     return true;
 }
 
@@ -976,6 +997,7 @@ hipError_t launch_window_attention_bwd(const WindowParams& p, const float* lse, 
     if (heads * (a.tiles + sb * a.far_blocks) + 8 + (long)p.B * p.Hq * a.tiles > WG_MAX ||
         (a.far_blocks > 0 && heads * sb * (p.D / 16) > WG_MAX / 4))
         return hipErrorInvalidValue;
+    a.by_item = Div((unsigned)(a.tiles + sb * a.far_blocks));
     hipError_t rc = hipSuccess;
     SLSMI_FMT_DISPATCH(p.fmt, rc = p.D == 64 ? (launch_bwd<F, 64>(a, s)) : (launch_bwd<F, 128>(a, s)));
     return rc;
