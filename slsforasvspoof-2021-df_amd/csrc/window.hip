@@ -310,7 +310,11 @@ __device__ __forceinline__ float halves_sum(float v) {
 __device__ __forceinline__ void want(const HeadPtr& x) { asm volatile("" ::"s"(x.p), "s"(x.b), "s"(x.r), "s"(x.h)); }
 __device__ __forceinline__ void want(const HeadOut& x) { asm volatile("" ::"s"(x.p), "s"(x.b), "s"(x.r), "s"(x.h)); }
 
-__device__ __forceinline__ int frames_of(const WinArgs& a, int b) { return a.nframes ? min(max(a.nframes[b], 0), a.T) : a.T; }
+// (read through the scalar cache: a wait for it is no wait for the vector loads under way)
+__device__ __forceinline__ int frames_of(const WinArgs& a, int b) {
+    if (!a.nframes) return a.T;
+    return min(max(*reinterpret_cast<const __attribute__((address_space(4))) int*>((uintptr_t)(a.nframes + b)), 0), a.T);
+}
 
 // Bounds of a query's keys relative to itself, for the masked blocks: key - q in [-left, right] and below len.
 struct KeyRange {
