@@ -574,7 +574,7 @@ def _window_shape(q: torch.Tensor, k: torch.Tensor, left, right, sinks: int, sca
     return qs, (B, T, kv, D), _SHAPE.pack(B, T, H, kv, D, _window_side(left, "left"), _window_side(right, "right"), sinks, fmt, scale)
 
 
-def _rows_arg(t: torch.Tensor, name: str, width: int, dtype: torch.dtype, index: int, lead=None, written: bool = False) -> int:
+def _rows_arg(t: torch.Tensor, name: str, width: int, dtype: torch.dtype, index: int, lead=None) -> int:
     """Row stride of [rows, >= width] or [batch, frames, >= width] whose rows lie at one distance."""
     shape = t.shape
     if t.dtype != dtype or len(shape) not in (2, 3) or shape[-1] < width or t.get_device() != index or \
@@ -695,10 +695,13 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, left: Op
     index = _device_of(q)
     qs, ks, shape = _window_shape(q, k, left, right, sinks, scale)
     dtype = q.dtype
-    if out is None:
-        out = q.new_empty(qs)
     aq, ak, av = _heads_arg(q, "q", qs, dtype, index), _heads_arg(k, "k", ks, dtype, index), _heads_arg(v, "v", ks, dtype, index)
-    ao = _heads_arg(out, "out", qs, dtype, index, True)
+    if out is None:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        _, T, H, D = qs
+        ao = _HEADS.pack(out.data_ptr(), T * H * D, H * D, D)
+    else:
+        ao = _heads_arg(out, "out", qs, dtype, index, True)
     lse = torch.empty(qs[0], qs[2], qs[1], dtype=torch.float32, device=q.device) if return_lse else None
     _on_device(index, _lib.load().slsmi_window_attention, shape, aq, ak, av, ao, lse.data_ptr() if return_lse else None,
                _vector(nframes, "nframes", torch.int32, qs[:1], index))
@@ -716,9 +719,10 @@ def window_attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tens
     index = _device_of(q)
     qs, ks, shape = _window_shape(q, k, left, right, sinks, scale)
     dtype = q.dtype
-    dq = q.new_empty(qs) if dq is None else dq
-    dk = q.new_empty(ks) if dk is None else dk
-    dv = q.new_empty(ks) if dv is None else dv
+    fresh = torch.contiguous_format
+    dq = torch.empty_like(q, memory_format=fresh) if dq is None else dq
+    dk = torch.empty_like(k, memory_format=fresh) if dk is None else dk
+    dv = torch.empty_like(k, memory_format=fresh) if dv is None else dv
     args = [_heads_arg(t, n, s, dtype, index) for t, n, s in ((dout, "dout", qs), (q, "q", qs), (k, "k", ks), (v, "v", ks),
                                                              (out, "out", qs))]
     outs = [_heads_arg(t, n, s, dtype, index, True) for t, n, s in ((dq, "dq", qs), (dk, "dk", ks), (dv, "dv", ks))]
