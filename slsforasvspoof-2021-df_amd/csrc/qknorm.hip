@@ -44,18 +44,6 @@ __device__ __forceinline__ long long row_position(const QkNormArgs& a, long row)
     return a.positions ? a.positions[i] : (long long)i;
 }
 
-template <int D>
-__device__ __forceinline__ void lane_weights(const QkNormArgs& a, int c, int pc, float (&wq)[8], float (&wk)[8],
-                                             float (&pwq)[8], float (&pwk)[8]) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        wq[e] = a.wq[c * 8 + e];
-        wk[e] = a.wk[c * 8 + e];
-        pwq[e] = a.wq[pc * 8 + e];
-        pwk[e] = a.wk[pc * 8 + e];
-    }
-}
-
 template <int FMT, int D>
 __global__ __launch_bounds__(QN_WAVES * 64) void qk_norm_rope_kernel(QkNormArgs a) {
     constexpr int GL = D / 8, HW = 64 / GL;   // lanes per head, heads a wave holds at once
@@ -75,10 +63,15 @@ __global__ __launch_bounds__(QN_WAVES * 64) void qk_norm_rope_kernel(QkNormArgs 
 #pragma unroll
         for (int u = 0; u < U; ++u) v[u] = *reinterpret_cast<const u16x8*>(x + (long)min(h + u * HW, H - 1) * D);
     };
-    request(h0 + g);   // (on their way while the angles are computed)
-    const NormLane t = norm_lane<D>(lane, row_position(a, row), a.freqs, a.half, a.interleaved, tab[wave]);
+    request(h0 + g);   // (on their way while the angles are computed, as are the weights)
+    const double freq = norm_freq(lane, a.freqs, a.half);
+    const int pc = norm_partner<D>(lane, a.half, a.interleaved) & (GL - 1);
     float wq[8], wk[8], pwq[8], pwk[8];
-    lane_weights<D>(a, c, t.partner & (GL - 1), wq, wk, pwq, pwk);
+    load8(a.wq + c * 8, wq);
+    load8(a.wk + c * 8, wk);
+    load8(a.wq + pc * 8, pwq);
+    load8(a.wk + pc * 8, pwk);
+    const NormLane t = norm_lane<D>(lane, row_position(a, row), freq, a.half, a.interleaved, tab[wave]);
     for (int h = h0 + g; h - g < h1; h += U * HW) {
         if (h - g > h0) request(h);
 #pragma unroll
@@ -124,11 +117,10 @@ __global__ __launch_bounds__(QN_WAVES * 64) void qk_norm_rope_bwd_kernel(QkNormA
     const int H = a.Hq + a.Hk;
     float gq[8], gk[8], wq[8], wk[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        gq[e] = gk[e] = 0.f;
-        wq[e] = a.wq[c * 8 + e];
-        wk[e] = a.wk[c * 8 + e];
-    }
+    for (int e = 0; e < 8; ++e) gq[e] = gk[e] = 0.f;
+    load8(a.wq + c * 8, wq);
+    load8(a.wk + c * 8, wk);
+    const double freq = norm_freq(lane, a.freqs, a.half);
     for (long row = (long)blockIdx.x * QN_WAVES + wave; row < a.rows; row += (long)gridDim.x * QN_WAVES) {
         const bf16_t* x = a.x + row * a.ldx + c * 8;
         const bf16_t* dy = a.dy + row * a.lddy + c * 8;
@@ -145,7 +137,7 @@ __global__ __launch_bounds__(QN_WAVES * 64) void qk_norm_rope_bwd_kernel(QkNormA
             }
         };
         request(g);
-        const NormLane t = norm_lane<D>(lane, row_position(a, row), a.freqs, a.half, a.interleaved, tab[wave]);
+        const NormLane t = norm_lane<D>(lane, row_position(a, row), freq, a.half, a.interleaved, tab[wave]);
         for (int h = g; h - g < H; h += U * HW) {
             if (h > g) request(h);
 #pragma unroll

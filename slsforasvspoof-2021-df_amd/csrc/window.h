@@ -78,6 +78,17 @@ __device__ __forceinline__ u16x8 lane_exchange(u16x8 x, int src) {
     return __builtin_bit_cast(u16x8, r);
 }
 
+// eight weights, wherever fp32 values may lie
+__device__ __forceinline__ void load8(const float* __restrict__ p, float (&w)[8]) {
+    typedef float any4 __attribute__((ext_vector_type(4), aligned(4)));
+    const any4 a = *reinterpret_cast<const any4*>(p), b = *reinterpret_cast<const any4*>(p + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        w[e] = a[e];
+        w[4 + e] = b[e];
+    }
+}
+
 template <int FMT, int D>
 __device__ __forceinline__ void norm_rope_lane(u16x8 x, const float* w, const float* pw, const NormLane& t, float eps,
                                                float* y) {
@@ -109,16 +120,26 @@ __device__ __forceinline__ void angle_cos_sin(long long p, double freq, float& c
     sincospif(2.0f * t, &s, &c);
 }
 
+// Where a lane's other members are, and its frequency: known before the position is, so that what they lead to (weights,
+// the frequency itself) can be on its way early.
+template <int D>
+__device__ __forceinline__ int norm_partner(int lane, int half, int interleaved) {
+    const int c = lane & (D / 8 - 1), hc = half >> 3;   // hc: chunks of a half (half is a multiple of 8)
+    return interleaved || c >= 2 * hc ? lane : c < hc ? lane + hc : lane - hc;
+}
+__device__ __forceinline__ double norm_freq(int lane, const double* __restrict__ freqs, int half) {
+    return lane < half ? freqs[lane] : 0.0;
+}
+
 // What a lane of the norm has to know beside its data: which channels its pairs are and their angles.  tab: wave-private
 // LDS of 64 (cos, sin) pairs, written here (half = R / 2 <= 64 pairs).
 template <int D>
-__device__ __forceinline__ NormLane norm_lane(int lane, long long p, const double* __restrict__ freqs, int half,
-                                              int interleaved, float2* tab) {
+__device__ __forceinline__ NormLane norm_lane(int lane, long long p, double freq, int half, int interleaved, float2* tab) {
     constexpr int GL = D / 8;
     const int c = lane & (GL - 1);
     NormLane t;
     t.role = 0;
-    t.partner = lane;
+    t.partner = norm_partner<D>(lane, half, interleaved);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         t.cs[e] = 1.f;
@@ -127,13 +148,13 @@ __device__ __forceinline__ NormLane norm_lane(int lane, long long p, const doubl
     if (half <= 0) return t;
     if (lane < half) {
         float cc, ss;
-        angle_cos_sin(p, freqs[lane], cc, ss);
+        angle_cos_sin(p, freq, cc, ss);
         tab[lane] = float2{cc, ss};
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    const int hc = half >> 3;   // chunks of a half (half is a multiple of 8)
+    const int hc = half >> 3;
     if (c < 2 * hc) {
         if (interleaved) {
             t.role = 3;
@@ -146,7 +167,6 @@ __device__ __forceinline__ NormLane norm_lane(int lane, long long p, const doubl
         } else {
             const bool first = c < hc;
             t.role = first ? 1 : 2;
-            t.partner = first ? lane + hc : lane - hc;
             const int at = (first ? c : c - hc) * 8;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {

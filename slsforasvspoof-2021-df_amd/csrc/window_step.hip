@@ -81,7 +81,7 @@ __global__ __launch_bounds__(ST_WAVES * 64) void window_step_kernel(StepArgs a) 
         nv = *reinterpret_cast<const u16x8*>(row + (long)(a.Hq + a.Hk + hk) * D);
         const float sc = a.scale * LOG2E;
         if (a.wq) {
-            const NormLane t = norm_lane<D>(lane, pos, a.freqs, a.half, a.interleaved, tab[wave]);
+            const NormLane t = norm_lane<D>(lane, pos, norm_freq(lane, a.freqs, a.half), a.half, a.interleaved, tab[wave]);
             const int pc = t.partner & (GL - 1);
             float w[8], pw[8], y[8];
 #pragma unroll

@@ -655,3 +655,21 @@ def test_infinities_and_nan_reach_what_sees_them(dtype):
     cache[1][0, 1, 3, 5] = math.nan
     o = ops.window_attention_step(rnd(1, 6 * 64, seed=8, dtype=dtype), *cache, torch.tensor([100], device=DEV), 2, 0)
     assert bool(o[0, 1, 5].isnan()) and int(o.isnan().sum()) == 1
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_weights_and_frequencies_at_odd_addresses(dtype):
+    """fp32 weights one value past an aligned address and float64 frequencies one value past one: the same results."""
+    x, wq, wk, fr, _, _ = norm_case(35, 7, 5, 1, 128, 96, False, None, 128, dtype)
+    odd = [torch.cat((w[:1], w))[1:] for w in (wq, wk, fr)]
+    assert all(w.data_ptr() % 16 for w in odd)
+    dy = rnd(5, 7, 768, seed=5, dtype=dtype)
+    assert torch.equal(ops.qk_norm_rope(x, 5, 1, *odd), ops.qk_norm_rope(x, 5, 1, wq, wk, fr))
+    for a, b in zip(ops.qk_norm_rope_backward(dy, x, 5, 1, *odd), ops.qk_norm_rope_backward(dy, x, 5, 1, wq, wk, fr)):
+        assert torch.equal(a, b)
+    results = []
+    for w in ((wq, wk, fr), odd):
+        cache = [rnd(35, 1, 40, 128, seed=i, dtype=dtype) for i in (6, 7)]
+        p = torch.arange(35, device=DEV) * 3
+        results.append([ops.window_attention_step(x.view(35, 896)[:, :896], *cache, p, 5, 4, *w)] + cache)
+    assert all(torch.equal(a, b) for a, b in zip(*results))
