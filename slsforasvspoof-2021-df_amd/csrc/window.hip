@@ -11,6 +11,10 @@
 // and the packed probabilities ARE the B operand of O^T = V^T P^T when the 16 keys of a step are enumerated as
 // (half hi, j) -> 4 hi + j (j < 4), 8 + 4 hi + j - 4: P never leaves registers.  V^T comes from row-major LDS by
 // ds_read_b64_tr_b16.  The key loop visits only the tiles of the sinks and of the window.
+//
+// What bounds these kernels: neither HBM (84 MB in the 95 us of 8192 frames, 16 heads of 128 channels on 4, 1024 keys a query) nor the
+// matrix units alone, but a wave's matrix and vector instructions, which overlap only in part.  Counters of the backward at
+// 8192 x 16 x 64, 512 keys: matrix units 30 % of all cycles, vector units 35 %, LDS 17 %, no bank conflicts.
 #include "kernels.h"
 #include "window.h"
 
@@ -26,7 +30,9 @@ template <int N>
 using Const = std::integral_constant<int, N>;
 constexpr float LN2 = 0.6931471805599453f;
 
-// Waves per SIMD the kernels are built for: the most that registers allow without spilling (128 / 168 / 256 per wave).
+// Waves per SIMD the kernels are built for, 128, 168 or 256 registers a wave.  The backward keeps a few words of its
+// prologue in scratch for it (nothing inside the loops); one wave fewer is slower (2 for 3 at 64 channels: 100 -> 114 us at
+// 8192 frames, 512 keys).
 constexpr int fwd_waves(int D) { return D == 64 ? 4 : 3; }
 constexpr int bwd_waves(int D) { return D == 64 ? 3 : 2; }
 
@@ -340,7 +346,12 @@ __device__ __forceinline__ void hide_keys(f32x16& s, int k0, int kb, int q, int 
     }
 }
 
-// ---- forward: 128 queries per workgroup, 32 per wave; key tiles in two LDS buffers (one barrier per tile).
+// ---- forward: 128 queries per workgroup, 32 per wave; key tiles in two LDS buffers (one barrier per tile): the next
+// tile is asked for when every wave has left the one it replaces.  Times (kernel, 16 heads of 64): one second 4.1 us, of
+// which 1900 cycles are the way to the first load; 4 x 1001 frames, 201 keys, 14.8 us; 8192 frames, 512 keys, 32 us (540
+// TFLOP/s); 8192 frames, 16 heads of 128 on 4, 1024 keys, 95 us (680 TFLOP/s).  Measured against it and slower: 64 queries a wave, 8 waves a
+// workgroup, both blocks of a tile in one softmax, three or four buffers, 2 waves a workgroup where the CUs are full (32 -> 42
+// us; 8 to 15 % faster where at most two workgroups meet on a CU, not worth a second kernel).
 //
 // The running maximum `m` of a query is only a reference for the exponent: it is moved (and the sums rescaled) when a
 // score of its wave passes it by more than 2^RISE, so almost never after the first block; probabilities stay below 2^RISE
@@ -464,7 +475,8 @@ __global__ __launch_bounds__(256, fwd_waves(D)) void window_fwd_kernel(WinArgs a
 }
 
 // ---- backward, first launch: delta = rowsum(dO o O) of DELTA_ROWS rows of a head per workgroup, and (half precision) the
-// largest |dO| and |delta| among them.  D / 8 lanes hold a row, 16 bytes of both each.
+// largest |dO| and |delta| among them.  D / 8 lanes hold a row, 16 bytes of both each.  Bound by reading both once (8192 x
+// 16 x 64: 34 MB in 6.4 us, 5.2 TB/s).
 constexpr int DELTA_ROWS = 128;
 
 template <int FMT, int D>
@@ -542,7 +554,8 @@ __device__ __forceinline__ float row_size(const u16x8 (&d)[NS]) {
 }
 
 // ---- backward, queries: dQ; the forward's loop with P recomputed from lse.  The product dO V^T starts from -delta, so
-// dP - delta leaves the matrix units.
+// dP - delta leaves the matrix units.  dQ and dK / dV each recompute P (7 products instead of 5): one pass for all three
+// would add partial dQ to memory once per key tile, 340 MB at 8192 x 16 x 64 and 512 keys, more time than the products take.
 template <int FMT, int D>
 __device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* lds) {
     constexpr int BN = tile_rows(D), NS = D / 16, DT = D / 32, TILE = BN * D * 2;
@@ -640,8 +653,8 @@ __device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* ld
     }
 }
 
-// ---- backward, keys: dK and dV.  A workgroup owns 128 keys (32 per wave) and goes through the 64-query tiles of every
-// query head of the group that see them; S = Q K^T this time (queries on the row index), so P and dS are the B operands
+// ---- backward, keys: dK and dV.  A workgroup owns 128 keys (32 per wave) and goes through the tiles of queries, of every
+// query head of the group, that see them; S = Q K^T this time (queries on the row index), so P and dS are the B operands
 // of dV^T = dO^T P and dK^T = Q^T dS.  The products start from -lse / scale and -delta of their rows (LDS), which also
 // takes rows out: a row with lse = +inf has P = 0.
 //
@@ -826,7 +839,9 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
 }
 
 // Both sides of the backward in one launch: the key-side workgroups (the longer ones) first, the query-side ones behind
-// them fill the CUs that these leave.  The key side's count is rounded up to the XCDs, so that both have their order.
+// them fill the CUs that these leave (4 x 1001 frames: 49 -> 44 us against two launches).  The key side's count is rounded
+// up to the XCDs, so that both have their order.  Times, both sides: 4 x 1001 x 16 x 64, 201 keys, 35 us; 8192 x 16 x 64, 512
+// keys, 95 us (440 TFLOP/s of the 5 products a gradient needs, 700 of the 8 that run); 128 channels, 8 heads, 1024 keys, 160 us.
 template <int FMT, int D, bool SPLIT>
 __global__ __launch_bounds__(256, bwd_waves(D)) void window_bwd_kernel(WinArgs a, unsigned key_side, unsigned key_blocks) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -843,7 +858,8 @@ __global__ __launch_bounds__(256, bwd_waves(D)) void window_bwd_kernel(WinArgs a
 }
 
 // The partial sums of a sink block (32 keys) -> its rows of dK and dV.  A workgroup takes one of dK, dV for 1024 / D keys;
-// four threads share a sum, each every fourth slot in ascending order, and are added in their order.
+// four threads share a sum, each every fourth slot in ascending order, and are added in their order (one thread a sum: 12
+// instead of 4.3 us at 8192 frames).
 template <int FMT, int D>
 __global__ __launch_bounds__(1024) void window_sink_kernel(WinArgs a) {
     constexpr int KEYS = 1024 / D, PARTS = 32 / KEYS;
@@ -871,7 +887,7 @@ __global__ __launch_bounds__(1024) void window_sink_kernel(WinArgs a) {
         u32x2_t{result2<FMT>(s[0], s[1]), result2<FMT>(s[2], s[3])};
 }
 
-constexpr int FAR_CHUNK = 1024;
+constexpr int FAR_CHUNK = 1024;   // 8 workgroups a sink block at 8192 frames; their loops are as long as the near ones'
 constexpr long WG_MAX = 0xffffffffL / 256;   // workgroups of 256 in a launch, whose work-items a 32-bit number counts
 
 // queries past the near ones of the first sink block, in chunks (0: none)

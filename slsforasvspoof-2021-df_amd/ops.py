@@ -1,7 +1,8 @@
 """Thin torch-tensor wrappers over libslsmi's single-kernel entry points.
 
-Used by the parity tests (one kernel at a time against an fp32 reference) and
-by AutoEncoderTopK's stand-alone encode/decode.  Every function takes ROCm
+Used by the parity tests (one kernel at a time against an fp32 reference), by
+AutoEncoderTopK's stand-alone encode/decode and, from qk_norm_rope on, by callers
+with models of their own (training.windowed_attention).  Every function takes ROCm
 tensors, enqueues on torch's current stream and returns torch tensors; nothing
 here computes on the host.
 """
