@@ -656,7 +656,8 @@ typedef struct slsmi_window_shape {
  * out rows of padded frames are written as zeros; what q, k, v hold there is never used.  lse: NULL or fp32
  * [batch][heads][frames], the log of the sum of exponentials per row (-inf at padded frames): what the backward needs.
  * out may be q, but shares no memory with k and v.  What a recording's own frames hold is finite: an infinity or NaN
- * there reaches the rows that see it and may reach others up to a tile away.  batch * heads * (frames / 128, rounded up)
+ * there reaches the rows that see it and may reach others up to a tile away.  Scores (scale q k) stay below 2^23 in
+ * magnitude, lse being 32 bits.  batch * heads * (frames / 128, rounded up)
  * stays below 2^24, in the backward both sides together. */
 int slsmi_window_attention(const slsmi_window_shape* shape, const slsmi_heads* q, const slsmi_heads* k, const slsmi_heads* v,
                            const slsmi_heads* out, float* lse, const int32_t* nframes, void* stream);

@@ -30,11 +30,14 @@ template <int N>
 using Const = std::integral_constant<int, N>;
 constexpr float LN2 = 0.6931471805599453f;
 
-// Waves per SIMD the kernels are built for, 128, 168 or 256 registers a wave.  The backward keeps a few words of its
-// prologue in scratch for it (nothing inside the loops); one wave fewer is slower (2 for 3 at 64 channels: 100 -> 114 us at
-// 8192 frames, 512 keys).
+// Waves per SIMD the kernels are built for, 128, 168 or 256 registers a wave (backward at 64 channels, two waves instead of
+// three: 8192 frames, 512 keys 94 -> 98 us, 8 x 4096 frames, 201 keys 250 -> 277 us).
 constexpr int fwd_waves(int D) { return D == 64 ? 4 : 3; }
 constexpr int bwd_waves(int D) { return D == 64 ? 3 : 2; }
+// Fragments of 16 bytes a lane that the key side keeps in LDS for want of registers: as many as it takes for no kernel to
+// spill, few enough for the waves above (44 to 108 bytes spilled, partly inside the loops, cost 9 to 20 %: 128 channels at 8192
+// frames 163 -> 148 us, the split form at 8 x 4096 frames 288 -> 245 us).
+constexpr int frags_in_lds(int fmt, int D, bool split) { return D == 128 ? 6 : !split ? 0 : fmt == FMT_F16 ? 5 : 3; }
 
 struct HeadPtr {
     const bf16_t* p;
@@ -73,7 +76,7 @@ struct WinArgs {
     int left, right, sinks;  // left, right in [0, T]; sinks in [0, SINK_MAX]
     int tiles;               // tiles of a head in this launch
     int far_blocks, far_chunk;   // dkv: workgroups per sink block beyond the near tiles, queries per workgroup
-    float scale;
+    float scale, scale2, inv_scale;   // scale2: scale / ln 2
 };
 
 constexpr int SINK_MAX = 128;
@@ -312,7 +315,7 @@ __device__ __forceinline__ float halves_sum(float v) {
 }
 
 // A kernel's arguments are wanted together: where each is loaded just before its first use, a workgroup begins with five
-// round trips to the scalar cache one after the other (2500 cycles before the first tile arrives became 1600).
+// round trips to the scalar cache one after the other (2500 to 3300 cycles to the first load became 1900).
 __device__ __forceinline__ void want(const HeadPtr& x) { asm volatile("" ::"s"(x.p), "s"(x.b), "s"(x.r), "s"(x.h)); }
 __device__ __forceinline__ void want(const HeadOut& x) { asm volatile("" ::"s"(x.p), "s"(x.b), "s"(x.r), "s"(x.h)); }
 
@@ -397,7 +400,7 @@ __global__ __launch_bounds__(256, fwd_waves(D)) void window_fwd_kernel(WinArgs a
     const TileLoad<D, BN> lk(a.k.r, lane, wave), lv(a.v.r, lane, wave);
     lk.issue(kh, a.k.r, kt.tile(0) * BN, len, lds, wave);
     lv.issue(vh, a.v.r, kt.tile(0) * BN, len, lds + TILE, wave);
-    const float sc = a.scale * LOG2E;
+    const float sc = a.scale2;
     float m = -INFINITY, ref = 0.f, most = -INFINITY, l = 0.f;   // most: the score that moves the reference
     f32x16 o[DT];
 #pragma unroll
@@ -576,11 +579,12 @@ __device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* ld
         }
     }
     const int len = frames_of(a, b);
-    bf16_t* const dqrow = a.dq.p + b * a.dq.b + h * a.dq.h + (long)q * a.dq.r;
+    // (formed where it is used: held through the loop it would cost registers that the kernel does not have)
+    const auto dqrow = [&]() { return a.dq.p + b * a.dq.b + h * a.dq.h + (long)q * a.dq.r; };
     if (q0 >= len) {
         if (q < a.T) {
 #pragma unroll
-            for (int dt = 0; dt < DT; ++dt) store_column<FMT>(dqrow, dt, zero16(), hi);
+            for (int dt = 0; dt < DT; ++dt) store_column<FMT>(dqrow(), dt, zero16(), hi);
         }
         return;
     }
@@ -592,7 +596,7 @@ __device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* ld
     lk.issue(kh, a.k.r, kt.tile(0) * BN, len, lds, wave);
     lv.issue(vh, a.v.r, kt.tile(0) * BN, len, lds + TILE, wave);
     const bool live = q < len;
-    const float sc = a.scale * LOG2E;
+    const float sc = a.scale2;
     const long stat = (long)bh * a.T + min(q, len - 1);
     const float lift = FMT == FMT_F16 ? lift_of(row_size<FMT>(df), 0) : 0.f;
     const float ls = a.lse[stat] * LOG2E - lift, delta = a.delta[stat];
@@ -643,12 +647,17 @@ __device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* ld
         if constexpr (BN == 64) block(Const<1>{});
         at.turn(it & 1 ? -2 * TILE : 2 * TILE);
     }
-    const float fin = a.scale * __builtin_amdgcn_exp2f(-lift);
+    float fin = a.scale;
+    if constexpr (FMT == FMT_F16) {   // (the row's lift, a whole number, once more: through the loop there is no register for it)
+        int row = min(q, len - 1);
+        asm volatile("" : "+v"(row));
+        fin *= __builtin_amdgcn_exp2f(rintf(fmaf(-a.lse[(long)bh * a.T + row], LOG2E, ls)));
+    }
     if (q < a.T) {
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
             const f32x16 v = live ? acc[dt] * fin : zero16();
-            store_column<FMT>(dqrow, dt, v, hi);
+            store_column<FMT>(dqrow(), dt, v, hi);
         }
     }
 }
@@ -690,6 +699,10 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
         qb = min(first + (chunk + 1) * a.far_chunk, len) - 1;
     }
     const int key = k0w + col;
+    // the last VL of a wave's value fragments and KL of its key fragments wait in LDS
+    constexpr int LF = frags_in_lds(FMT, D, SPLIT), VL = LF < NS ? LF : NS, KL = LF - VL, VR = NS - VL, KR = NS - KL;
+    char* const own = lds + 2 * BUF + (wave * LF * 64 + lane) * 16;
+    const auto parked = [&](int i) { return *reinterpret_cast<const u16x8*>(own + i * 1024); };
     u16x8 kf[NS], vf[NS];
     {
         const int row = min(key, a.T - 1);
@@ -701,17 +714,20 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
             vf[s] = *reinterpret_cast<const u16x8*>(vr + s * 16);
         }
     }
+#pragma unroll
+    for (int e = VR; e < NS; ++e) *reinterpret_cast<u16x8*>(own + (e - VR) * 1024) = vf[e];
+#pragma unroll
+    for (int e = KR; e < NS; ++e) *reinterpret_cast<u16x8*>(own + (VL + e - KR) * 1024) = kf[e];
     f32x16 ak[DT], av[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) ak[dt] = av[dt] = zero16();
-    const float sc = a.scale * LOG2E, lsc = 1.0f / a.scale;
-    const float p_lift = FMT == FMT_F16 ? P_LIFT : 0.f, lift_sc = p_lift / sc;
-    float ds_lift = 0.f;
+    const float sc = a.scale2;
+    constexpr float p_lift = FMT == FMT_F16 ? P_LIFT * LN2 : 0.f;
+    float turn = 1.f;   // 2^(lift of dS - lift of P), of this lane's key
     if constexpr (FMT == FMT_F16) {
         const f32x2 top = grad_size(a, (long)b * a.Hq + hk * grp, grp, qa, qb);
-        ds_lift = lift_of(fmaf(top[0] * (D == 64 ? 8.f : 11.f), row_size<FMT>(vf), top[1]), 8);
+        turn = __builtin_amdgcn_exp2f(lift_of(fmaf(top[0] * (D == 64 ? 8.f : 11.f), row_size<FMT>(vf), top[1]), 8) - P_LIFT);
     }
-    const float turn = __builtin_amdgcn_exp2f(ds_lift - p_lift);
     const int t0 = qa / BQ, nt = qb < qa ? 0 : qb / BQ - t0 + 1;
     const int total = nt * grp;
     LaneAt<D> at(lane, lds);
@@ -726,7 +742,7 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
             const int q = q0 + (tid & (BQ - 1));
             const long at = ((long)b * a.Hq + rh) * a.T + min(q, len - 1);
             const bool in = q >= qa && q <= qb;
-            stat = tid < BQ ? (in ? fmaf(-a.lse[at], lsc, lift_sc) : -INFINITY) : (in ? -a.delta[at] : 0.f);
+            stat = tid < BQ ? (in ? (p_lift - a.lse[at]) * a.inv_scale : -INFINITY) : (in ? -a.delta[at] : 0.f);
         }
         if (++rt == t0 + nt) {
             rt = t0;
@@ -767,8 +783,8 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
             }
 #pragma unroll
             for (int e = 0; e < NS; ++e) {
-                s = mfma32<FMT>(row_frag<D>(Qs, 32 * u, at, e), kf[e], s);
-                dp = mfma32<FMT>(row_frag<D>(Ds, 32 * u, at, e), vf[e], dp);
+                s = mfma32<FMT>(row_frag<D>(Qs, 32 * u, at, e), e < KR ? kf[e] : parked(VL + e - KR), s);
+                dp = mfma32<FMT>(row_frag<D>(Ds, 32 * u, at, e), e < VR ? vf[e] : parked(e - VR), dp);
             }
             if (!vis.all(qs)) {
                 // q - key of register r is base + 8 (r / 4) + r % 4: seen from -right to left, and any later query by a sink
@@ -806,11 +822,16 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
         if constexpr (BQ == 64) block(Const<1>{});
         at.turn(it & 1 ? -BUF : BUF);
     }
-    const float vfin = __builtin_amdgcn_exp2f(-p_lift), kfin = a.scale * __builtin_amdgcn_exp2f(-ds_lift);
+    // (1 / turn by its exponent)
+    const float vfin = FMT == FMT_F16 ? 0x1p-15f : 1.f,
+                kfin = a.scale * vfin * (FMT == FMT_F16 ? __builtin_bit_cast(float, 0x7f000000u - __builtin_bit_cast(uint32_t, turn)) : 1.f);
+    int half = tid;   // (hi, but not the register that held it before the loop)
+    asm volatile("" : "+v"(half));
+    half = (half >> 5) & 1;
     if (far || (k0w < a.sinks && a.far_blocks > 0)) {
         const int blk = far ? block : k0w / 32, slot = far ? 1 + chunk * 4 + wave : 0;
         if (far && key >= a.sinks) return;
-        float* dst = a.part + ((((long)bh * sink_blocks + blk) * (1 + 4 * a.far_blocks) + slot) * 2 * 32 + col) * D + 4 * hi;
+        float* dst = a.part + ((((long)bh * sink_blocks + blk) * (1 + 4 * a.far_blocks) + slot) * 2 * 32 + col) * D + 4 * half;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -832,8 +853,8 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
         const bool live = key < len;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-            store_column<FMT>(dk, dt, live ? ak[dt] * kfin : zero16(), hi);
-            store_column<FMT>(dv, dt, live ? av[dt] * vfin : zero16(), hi);
+            store_column<FMT>(dk, dt, live ? ak[dt] * kfin : zero16(), half);
+            store_column<FMT>(dv, dt, live ? av[dt] * vfin : zero16(), half);
         }
     }
 }
@@ -841,7 +862,7 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
 // Both sides of the backward in one launch: the key-side workgroups (the longer ones) first, the query-side ones behind
 // them fill the CUs that these leave (4 x 1001 frames: 49 -> 44 us against two launches).  The key side's count is rounded
 // up to the XCDs, so that both have their order.  Times, both sides: 4 x 1001 x 16 x 64, 201 keys, 35 us; 8192 x 16 x 64, 512
-// keys, 95 us (440 TFLOP/s of the 5 products a gradient needs, 700 of the 8 that run); 128 channels, 8 heads, 1024 keys, 160 us.
+// keys, 90 us (470 TFLOP/s of the 5 products a gradient needs, 750 of the 8 that run); 128 channels, 8 heads, 1024 keys, 142 us.
 template <int FMT, int D, bool SPLIT>
 __global__ __launch_bounds__(256, bwd_waves(D)) void window_bwd_kernel(WinArgs a, unsigned key_side, unsigned key_blocks) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -925,6 +946,8 @@ bool window_args(const WindowParams& p, WinArgs& a) {
     a.right = p.right < 0 || p.right > p.T ? p.T : p.right;
     a.sinks = a.left >= p.T ? 0 : (p.sinks < p.T ? p.sinks : p.T);
     a.scale = p.scale;
+    a.scale2 = p.scale * LOG2E;
+    a.inv_scale = 1.0f / p.scale;
     a.nframes = p.nframes;
     a.tiles = (p.T + 127) / 128;
     if (p.B > 0 && p.T > 0) {
@@ -964,9 +987,9 @@ hipError_t launch_bwd(const WinArgs& a, hipStream_t s) {
     const int sb = (a.sinks + 31) / 32;
     const unsigned ks = a.B * a.Hk * (a.tiles + sb * a.far_blocks), kb = (ks + 7) & ~7u, qs = a.B * a.Hq * a.tiles;
     hipLaunchKernelGGL((window_delta_kernel<FMT, D>), dim3((a.T + DELTA_ROWS - 1) / DELTA_ROWS, a.Hq, a.B), dim3(256), 0, s, a);
-    constexpr int LDS = 2 * (2 * 8192 + 2 * tile_rows(D) * 4);
-    if (few_keys(a)) hipLaunchKernelGGL((window_bwd_kernel<FMT, D, true>), dim3(kb + qs), dim3(256), LDS, s, a, ks, kb);
-    else hipLaunchKernelGGL((window_bwd_kernel<FMT, D, false>), dim3(kb + qs), dim3(256), LDS, s, a, ks, kb);
+    const auto lds = [](bool split) { return 2 * (2 * 8192 + 2 * tile_rows(D) * 4) + frags_in_lds(FMT, D, split) * 4096; };
+    if (few_keys(a)) hipLaunchKernelGGL((window_bwd_kernel<FMT, D, true>), dim3(kb + qs), dim3(256), lds(true), s, a, ks, kb);
+    else hipLaunchKernelGGL((window_bwd_kernel<FMT, D, false>), dim3(kb + qs), dim3(256), lds(false), s, a, ks, kb);
     if (a.far_blocks > 0) hipLaunchKernelGGL((window_sink_kernel<FMT, D>), dim3(a.B * a.Hk * sb * (D / 16)), dim3(1024), 0, s, a);
     return hipGetLastError();
 }
