@@ -325,28 +325,24 @@ __device__ __forceinline__ int frames_of(const WinArgs& a, int b) {
     return min(max(*reinterpret_cast<const __attribute__((address_space(4))) int*>((uintptr_t)(a.nframes + b)), 0), a.T);
 }
 
-// Bounds of a query's keys relative to itself, for the masked blocks: key - q in [-left, right] and below len.
-struct KeyRange {
-    int left;
-    unsigned span;   // left + min(right, len - 1 - q)
-    __device__ __forceinline__ KeyRange(int q, int len, int l, int right) : left(l), span((unsigned)(l + min(right, len - 1 - q))) {}
-    __device__ __forceinline__ bool has(int rel) const { return (unsigned)(rel + left) <= span; }
-};
-
-// Scores of the 32 keys kb' .. of one lane's query that it does not see become -inf.  kb: key of register 0 of this lane.
-__device__ __forceinline__ void hide_keys(f32x16& s, int k0, int kb, int q, int len, int left, int right, int sinks) {
-    const KeyRange in(q, len, left, right);
-    if (k0 < sinks) {
-        const int last = min(min(sinks, len) - 1, q + right);
+// A masked block: bit i of a lane's mask tells whether entry i (of 28 rows or keys that the lane holds 16 of) is visible, and
+// an entry costs two instructions (a sign-extended bit and a bitwise choice; compared with its bounds it would be three).
+__device__ __forceinline__ uint32_t bits_below(int n) { return (1u << min(max(n, 0), 28)) - 1; }
+__device__ __forceinline__ void hide(f32x16& s, uint32_t seen) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int key = kb + 8 * (r >> 2) + (r & 3);
-            s[r] = (in.has(key - q) | (key <= last)) ? s[r] : -INFINITY;
-        }
-    } else {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = in.has(kb - q + 8 * (r >> 2) + (r & 3)) ? s[r] : -INFINITY;
+    for (int r = 0; r < 16; ++r) {
+        const uint32_t keep = (uint32_t)((int32_t)(seen << (31 - 8 * (r >> 2) - (r & 3))) >> 31);
+        const float v = s[r];   // (a bit cast of the element itself reads element 0)
+        s[r] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, v) & keep) | (0xff800000u & ~keep));
     }
+}
+
+// Scores of the 32 keys k0 .. of one lane's query that it does not see become -inf.  kb: key of register 0 of this lane.
+__device__ __forceinline__ void hide_keys(f32x16& s, int k0, int kb, int q, int len, int left, int right, int sinks) {
+    const int end = min(q + right, len - 1) + 1;   // keys below it, from q - left on
+    uint32_t seen = bits_below(end - kb) & ~bits_below(q - left - kb);
+    if (k0 < sinks) seen |= bits_below(min(sinks, end) - kb);
+    hide(s, seen);
 }
 
 // ---- forward: 128 queries per workgroup, 32 per wave; key tiles in two LDS buffers (one barrier per tile): the next
@@ -787,11 +783,9 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
                 dp = mfma32<FMT>(row_frag<D>(Ds, 32 * u, at, e), e < VR ? vf[e] : parked(e - VR), dp);
             }
             if (!vis.all(qs)) {
-                // q - key of register r is base + 8 (r / 4) + r % 4: seen from -right to left, and any later query by a sink
-                const int base = qs + 4 * hi - key;
-                const unsigned span = (unsigned)(a.right + (key < a.sinks ? 2 * a.T : a.left));
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s[r] = (unsigned)(base + 8 * (r >> 2) + (r & 3) + a.right) <= span ? s[r] : -INFINITY;
+                // rows from key - right to key + left, or any later one where the key is a sink's
+                const int from = qs + 4 * hi;
+                hide(s, (key < a.sinks ? ~0u : bits_below(key + a.left + 1 - from)) & ~bits_below(key - a.right - from));
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) {

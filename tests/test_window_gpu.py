@@ -673,3 +673,13 @@ def test_weights_and_frequencies_at_odd_addresses(dtype):
         p = torch.arange(35, device=DEV) * 3
         results.append([ops.window_attention_step(x.view(35, 896)[:, :896], *cache, p, 5, 4, *w)] + cache)
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", [(1, 1300, 2, 1, 64, None, 0, 0, None), (2, 1100, 2, 2, 64, 300, 300, 4, [1100, 700]),
+                                  (1, 1700, 2, 1, 64, 200, 0, 128, None), (3, 500, 2, 1, 128, 90, 90, 0, [500, 0, 411]),
+                                  (1, 1600, 1, 1, 128, 180, 3, 40, [1500])])
+def test_window_attention_of_many_keys(case, dtype):
+    """Rows that see hundreds of keys, some through far sinks: forward and gradients."""
+    test_window_attention(case, dtype)
+    test_window_attention_backward(case, dtype)
