@@ -181,4 +181,27 @@ __device__ __forceinline__ NormLane norm_lane(int lane, long long p, double freq
     return t;
 }
 
+// LDS image of a tile of rows of D 16-bit values, without padding: 16-byte chunks of a row permuted by its row number so
+// that 16 consecutive rows read at one chunk (ds_read_b128 of the row operand) and four consecutive rows read at four
+// neighbouring chunks (ds_read_b64_tr_b16 of the transposed operand) both touch every bank once (no conflict cycles
+// measured).  The permutation repeats every 16 rows.
+template <int D>
+__device__ __forceinline__ int chunk_turn(int row) {
+    return D == 64 ? (((row >> 1) & 1) << 2) | ((row >> 2) & 3) : ((row & 3) << 2) | ((row >> 2) & 3);
+}
+template <int D>
+__device__ __forceinline__ int tile_at(int row, int chunk) {
+    return row * D * 2 + ((chunk ^ chunk_turn<D>(row)) << 4);
+}
+
+__device__ __forceinline__ uint32_t lds_offset(const char* p) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
+}
+
+typedef __attribute__((address_space(3))) void* lds_ptr;
+
+__device__ __forceinline__ u16x8 tr_pair(s16x4 lo, s16x4 hi) {
+    return __builtin_bit_cast(u16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
 }  // namespace slsmi

@@ -85,23 +85,6 @@ constexpr long ROW_MAX = 1L << 23;   // row stride: 64 rows of a tile are reache
 // rows of a staged tile: 8 KiB either way, so that the two buffers of two tiles of several workgroups fit a CU
 constexpr int tile_rows(int D) { return D == 64 ? 64 : 32; }
 
-// LDS image of a tile of rows of D 16-bit values, without padding: 16-byte chunks of a row permuted by its row number so
-// that 16 consecutive rows read at one chunk (ds_read_b128 of the row operand) and four consecutive rows read at four
-// neighbouring chunks (ds_read_b64_tr_b16 of the transposed operand) both touch every bank once (no conflict cycles
-// measured).  The permutation repeats every 16 rows.
-template <int D>
-__device__ __forceinline__ int chunk_turn(int row) {
-    return D == 64 ? (((row >> 1) & 1) << 2) | ((row >> 2) & 3) : ((row & 3) << 2) | ((row >> 2) & 3);
-}
-template <int D>
-__device__ __forceinline__ int tile_at(int row, int chunk) {
-    return row * D * 2 + ((chunk ^ chunk_turn<D>(row)) << 4);
-}
-
-__device__ __forceinline__ uint32_t lds_offset(const char* p) {
-    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
-}
-
 // What a lane reads of a tile: the row operand of rows 0 .. 31 per 16 columns, as byte offsets, and the transposed operand
 // (rows as columns' neighbours) of rows 0 .. 15 per 32 columns, as LDS addresses in the current one of two buffers; other
 // rows and tiles lie a constant further, which the instruction holds.
@@ -134,10 +117,6 @@ template <int D>
 __device__ __forceinline__ u16x8 row_frag(const char* tile, int row0, const LaneAt<D>& at, int e) {
     return *reinterpret_cast<const u16x8*>(tile + row0 * D * 2 + at.row[e]);
 }
-__device__ __forceinline__ u16x8 tr_pair(s16x4 lo, s16x4 hi) {
-    return __builtin_bit_cast(u16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-}
-
 // A operands of a transposed product for all column blocks (32 columns each) of the 16 rows that lie `OFF` bytes past the
 // buffer's begin, rows enumerated as above.  The transposed read's builtin makes the compiler wait for every load into LDS that is
 // under way (the next tile's), so the reads are written out, with their wait in the same block.
@@ -183,8 +162,6 @@ __device__ __forceinline__ void tr_frags2(const LaneAt<D>& at, u16x8 (&f)[2][D /
         f[1][d + 1] = tr_pair(r6, r7);
     }
 }
-
-typedef __attribute__((address_space(3))) void* lds_ptr;
 
 // Rows row0 .. row0 + ROWS - 1 of a head straight into an LDS tile (16 bytes per lane; a wave fills 1 KiB pieces; the
 // permutation is applied to the source addresses).  The buffer descriptor ends behind row len - 1: later rows arrive as

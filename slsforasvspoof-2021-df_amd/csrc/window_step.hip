@@ -5,10 +5,13 @@
 // 0 .. min(p + 1, slots) - 1 are exactly the frames that position p sees (the sinks and the last `window` ones).
 // Softmax does not care about their order, so the kernel needs no mask beyond a count.
 //
-// Bound by reading the cache once (4 D bytes per slot and key head).  A wave reads 64 / (D / 8) slots at a time, 16 bytes
-// per lane; the D / 8 lanes of a slot sum the products of their channels by lane moves inside a row of 16, every slot
-// group keeps its own running maximum and sum, and groups, waves and the workgroups that share a long axis are joined at
-// the end.  Queries stay in 32 bits (normalised and turned here, never rounded).
+// Bound by reading the cache once (4 D bytes per slot and key head); a single short stream by latency.  Up to two query heads
+// a key head (window_step_kernel): a wave reads 64 / (D / 8) slots at a time, 16 bytes per lane; the D / 8 lanes of a slot sum
+// the products of their channels by lane moves inside a row of 16, every slot group keeps its own running maximum and sum,
+// and groups, waves and the workgroups that share a long axis are joined at the end.  Queries stay in 32 bits (normalised
+// and turned here, never rounded).  Measured: 64 streams of 1027 slots, 16 heads of 64, 270 MB in 50 us (5.4 TB/s); one
+// stream of 260 slots 4.0 us.  Measured and slower: weights and first slots asked for before the position is known, the next
+// slots while these are used (64 streams 3 % faster, one stream 8 % slower).
 #include "kernels.h"
 #include "window.h"
 
@@ -40,6 +43,45 @@ struct StepArgs {
     int splits, per_split; // slots per workgroup
 };
 
+// A share without slots: zeros as the result, or no weight.
+template <int D, int GP>
+__device__ __forceinline__ void step_nothing(const StepArgs& a, long share, long out, int live) {
+    const int tid = threadIdx.x;
+    if (a.splits == 1) {
+        for (int i = tid; i < GP * D; i += ST_WAVES * 64)
+            if (i / D < live) a.out[out + i] = 0;
+    } else if (tid < GP && tid < live) {
+        *reinterpret_cast<f32x2*>(a.ml + (share + (long)tid * a.splits) * 2) = f32x2{-INFINITY, 0.f};
+    }
+}
+
+// The waves' maxima, sums and values -> the result, or this workgroup's share of it.  live: query heads there are.
+template <int FMT, int D, int GP>
+__device__ __forceinline__ void step_join_waves(const StepArgs& a, const float (&red_m)[ST_WAVES][GP], const float (&red_l)[ST_WAVES][GP],
+                                                const float (*red_o)[GP][D], long share, long out, int live) {
+    for (int t = threadIdx.x; t < GP * D; t += ST_WAVES * 64) {
+        const int i = t / D, d = t % D;
+        if (i >= live) break;
+        float mx = red_m[0][i];
+#pragma unroll
+        for (int w = 1; w < ST_WAVES; ++w) mx = fmaxf(mx, red_m[w][i]);
+        const float ref = mx == -INFINITY ? 0.f : mx;
+        float sum = 0.f, acc = 0.f;
+#pragma unroll
+        for (int w = 0; w < ST_WAVES; ++w) {
+            const float corr = __builtin_amdgcn_exp2f(red_m[w][i] - ref);
+            sum = fmaf(red_l[w][i], corr, sum);
+            acc = fmaf(red_o[w][i][d], corr, acc);
+        }
+        if (a.splits == 1) {
+            a.out[out + t] = (bf16_t)result2<FMT>(acc / sum, 0.f);
+        } else {
+            a.acc[(share + (long)i * a.splits) * D + d] = acc;
+            if (d == 0) *reinterpret_cast<f32x2*>(a.ml + (share + (long)i * a.splits) * 2) = f32x2{mx, sum};
+        }
+    }
+}
+
 template <int FMT, int D, int GP>
 __global__ __launch_bounds__(ST_WAVES * 64) void window_step_kernel(StepArgs a) {
     constexpr int GL = D / 8, KG = 64 / GL, U = 4;
@@ -57,12 +99,7 @@ __global__ __launch_bounds__(ST_WAVES * 64) void window_step_kernel(StepArgs a) 
     const int n = pos < 0 ? 0 : (int)min(pos + 1, (long long)a.slots);
     const long share = ((long)b * a.Hq + hk * grp + g0) * a.splits + split;
     if (s0 >= n) {   // nothing here (also: no frame for this stream)
-        if (a.splits == 1) {
-            for (int i = tid; i < GP * D; i += ST_WAVES * 64)
-                if (g0 + i / D < grp) a.out[((long)b * a.Hq + hk * grp + g0) * D + i] = 0;
-        } else if (tid < GP && g0 + tid < grp) {
-            *reinterpret_cast<f32x2*>(a.ml + (share + (long)tid * a.splits) * 2) = f32x2{-INFINITY, 0.f};
-        }
+        step_nothing<D, GP>(a, share, ((long)b * a.Hq + hk * grp + g0) * D, grp - g0);
         return;
     }
     const int slot = pos < a.sinks ? (int)pos : a.sinks + (int)((pos - a.sinks) % (a.slots - a.sinks));
@@ -215,47 +252,231 @@ __global__ __launch_bounds__(ST_WAVES * 64) void window_step_kernel(StepArgs a) 
         }
     }
     __syncthreads();
-    for (int t = tid; t < GP * D; t += ST_WAVES * 64) {
-        const int i = t / D, d = t % D;
-        if (g0 + i >= grp) break;
-        float mx = red_m[0][i];
-#pragma unroll
-        for (int w = 1; w < ST_WAVES; ++w) mx = fmaxf(mx, red_m[w][i]);
-        const float ref = mx == -INFINITY ? 0.f : mx;
-        float sum = 0.f, acc = 0.f;
-#pragma unroll
-        for (int w = 0; w < ST_WAVES; ++w) {
-            const float corr = __builtin_amdgcn_exp2f(red_m[w][i] - ref);
-            sum = fmaf(red_l[w][i], corr, sum);
-            acc = fmaf(red_o[w][i][d], corr, acc);
-        }
-        if (a.splits == 1) {
-            a.out[((long)b * a.Hq + hk * grp + g0 + i) * D + d] = (bf16_t)result2<FMT>(acc / sum, 0.f);
-        } else {
-            a.acc[(share + (long)i * a.splits) * D + d] = acc;
-            if (d == 0) *reinterpret_cast<f32x2*>(a.ml + (share + (long)i * a.splits) * 2) = f32x2{mx, sum};
-        }
-    }
+    step_join_waves<FMT, D, GP>(a, red_m, red_l, red_o, share, ((long)b * a.Hq + hk * grp + g0) * D, grp - g0);
 }
 
-// Joins the shares of one query head: a wave forms the shares' weights, then D / 4 threads times 1024 / D groups of shares
-// (every (1024 / D)th, in order) sum the values, and the groups are added in their order.
+// The same for three or more query heads a key head: on vector instructions their products take as long as the bytes (16 heads
+// on 4 of 128 channels, 32768 slots, 67 MB: 23.4 us with the join, 17.9 here; 32 heads on 4: 32.3 and 19.1, at 256 slots 14.7
+// and 7.2), so both products run on
+// the 16 x 16 x 32 MFMA, 16 columns for eight heads: a head's query as the sum of two 16-bit operands in columns i and i + 8,
+// and its probabilities likewise, so that neither is rounded to 16 bits.  A wave takes 32 slots at a time; keys go from the
+// cache to the A operand's registers, values to a tile of the wave's own (zeros past the last slot) and from there by
+// transposed reads.  Scores arrive with four consecutive slots per lane and 16-slot group, which is the order the value
+// operand's slots are enumerated in.
 template <int FMT, int D>
-__global__ __launch_bounds__(256) void window_step_join_kernel(const float* __restrict__ ml, const float* __restrict__ acc,
-                                                               bf16_t* __restrict__ out, int splits) {
-    constexpr int G = 1024 / D, C = D / 4;
+__global__ __launch_bounds__(ST_WAVES * 64) void window_step_group_kernel(StepArgs a) {
+    constexpr int GP = 8, GL = D / 8, KG = 64 / GL, KS = D / 32, CT = D / 16, TILE = 32 * D * 2, STEP = ST_WAVES * 32;
+    constexpr float RISE = 8.f;   // how far (powers of two) scores may pass the reference before it moves
+    __shared__ __attribute__((aligned(1024))) char tiles[ST_WAVES * TILE];
+    __shared__ __attribute__((aligned(16))) bf16_t qs[2][GP][D];
+    __shared__ __attribute__((aligned(16))) bf16_t nks[D];
+    __shared__ float2 tab[ST_WAVES][64];
+    __shared__ float red_m[ST_WAVES][GP], red_l[ST_WAVES][GP];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int split = blockIdx.x, hk = blockIdx.y / a.qblocks, qb = blockIdx.y % a.qblocks, b = blockIdx.z;
+    const int grp = a.Hq / a.Hk;
+    const int g0 = qb * GP;
+    const long long pos = a.positions[b];
+    const int s0 = split * a.per_split, s1 = min(s0 + a.per_split, a.slots);
+    const int n = pos < 0 ? 0 : (int)min(pos + 1, (long long)a.slots);
+    const long share = ((long)b * a.Hq + hk * grp + g0) * a.splits + split;
+    const long out = ((long)b * a.Hq + hk * grp + g0) * D;
+    if (s0 >= n) {   // nothing here (also: no frame for this stream)
+        step_nothing<D, GP>(a, share, out, grp - g0);
+        return;
+    }
+    const int slot = pos < a.sinks ? (int)pos : a.sinks + (int)((pos - a.sinks) % (a.slots - a.sinks));
+    const bool own = slot >= s0 && slot < s1;
+    const int end = min(s1, n);
+    const long head = ((long)b * a.Hk + hk) * a.slots;
+    const bf16_t* const kc = a.kc + head * D;
+    const bf16_t* const row = a.qkv + (long)b * a.ld;
+    const bf16_t* const nv = row + (long)(a.Hq + a.Hk + hk) * D;
+
+    // ---- the wave's first slots
+    const int fr = lane & 15, fg = lane >> 4;
+    u16x8 kf[2][KS];
+    const auto ask_keys = [&](int k0) {
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+                kf[g][s] = *reinterpret_cast<const u16x8*>(kc + (long)min(k0 + 16 * g + fr, end - 1) * D + 32 * s + 8 * fg);
+    };
+    char* const tile = tiles + wave * TILE;
+    const auto ask_values = [&](int k0) {
+#ifdef __HIP_DEVICE_COMPILE__   // (the descriptor type does not exist in the host pass)
+        const auto r = __builtin_amdgcn_make_buffer_rsrc((void*)(a.vc + (head + k0) * D), 0, min(end - k0, 32) * D * 2, 0x00027000);
+#pragma unroll
+        for (int i = 0; i < 32 / KG; ++i) {
+            const int at = i * KG + lane / GL;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(tile + i * 1024), 16, at * D * 2 + (((lane & (GL - 1)) ^ chunk_turn<D>(at)) << 4),
+                                                     0, 0, 0);
+        }
+#endif
+    };
+    int k0 = s0 + wave * 32;
+    if (k0 < end) {
+        ask_keys(k0);
+        ask_values(k0);
+    }
+
+    // ---- queries and the new key, a head to D / 8 lanes: heads 0 .. 7 of this workgroup, then the key
+    const int c = lane & (GL - 1), item = wave * KG + lane / GL;
+    if (wave * KG <= GP) {
+        const bool isq = item < GP;
+        const u16x8 x = *reinterpret_cast<const u16x8*>(row + (long)(isq ? hk * grp + min(g0 + item, grp - 1) : a.Hq + hk) * D + c * 8);
+        u16x8 hi = x, lo = 0;
+        if (a.wq) {
+            const NormLane t = norm_lane<D>(lane, pos, norm_freq(lane, a.freqs, a.half), a.half, a.interleaved, tab[wave]);
+            float w[8], pw[8], y[8];
+            load8((isq ? a.wq : a.wk) + c * 8, w);
+            load8((isq ? a.wq : a.wk) + (t.partner & (GL - 1)) * 8, pw);
+            norm_rope_lane<FMT, D>(x, w, pw, t, a.eps, y);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                hi[e] = (bf16_t)result2<FMT>(y[e], 0.f);
+                lo[e] = (bf16_t)result2<FMT>(y[e] - Op<FMT>::unpack(hi[e]), 0.f);
+            }
+        }
+        if (isq) {
+            *reinterpret_cast<u16x8*>(&qs[0][item][c * 8]) = hi;
+            *reinterpret_cast<u16x8*>(&qs[1][item][c * 8]) = lo;
+        } else if (item == GP) {
+            *reinterpret_cast<u16x8*>(&nks[c * 8]) = hi;
+            if (own && qb == 0) {
+                *reinterpret_cast<u16x8*>(a.kc + (head + slot) * D + c * 8) = hi;
+                *reinterpret_cast<u16x8*>(a.vc + (head + slot) * D + c * 8) = *reinterpret_cast<const u16x8*>(nv + c * 8);
+            }
+        }
+    }
+    __syncthreads();
+    const int part = fr >> 3;   // this lane's column: head fr & 7, first or second operand
+    u16x8 q[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) q[s] = *reinterpret_cast<const u16x8*>(&qs[part][fr & 7][32 * s + 8 * fg]);
+    uint32_t va[CT];   // the lane's place in the wave's tile per 16 channels
+    {
+        const int r = 4 * fg + (fr >> 2), cc = 4 * (fr & 3);
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) va[ct] = lds_offset(tile) + tile_at<D>(r, (16 * ct + cc) >> 3) + (cc & 4) * 2;
+    }
+
+    const float sc = a.scale * LOG2E;
+    float m = -INFINITY, ref = 0.f, most = -INFINITY, l = 0.f;
+    f32x4 o[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) o[ct] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (; k0 < end; k0 += STEP) {
+        const int next = k0 + STEP;
+        __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): this wave's keys and values are here
+        if (own && slot >= k0 && slot < k0 + 32) {
+            // the slot just written is taken from where it came from: the store need not have landed when it was read
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+                if (k0 + 16 * g + fr == slot) {
+#pragma unroll
+                    for (int s = 0; s < KS; ++s) kf[g][s] = *reinterpret_cast<const u16x8*>(&nks[32 * s + 8 * fg]);
+                }
+            if (lane < GL) *reinterpret_cast<u16x8*>(tile + tile_at<D>(slot - k0, lane)) = *reinterpret_cast<const u16x8*>(nv + lane * 8);
+        }
+        f32x4 s[2];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+            s[g] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < KS; ++e) s[g] = Op<FMT>::mfma(kf[g][e], q[e], s[g]);
+        }
+        if (next < end) ask_keys(next);
+        float p[8];
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float v = s[j >> 2][j & 3];
+            p[j] = k0 + 16 * (j >> 2) + 4 * fg + (j & 3) < end ? v + dpp_move<0x128>(v) : -INFINITY;   // row_ror 8: the other operand's column
+            mx = fmaxf(mx, p[j]);
+        }
+        if (__builtin_amdgcn_ballot_w64(mx > most) != 0) {
+            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            const float mn = fmaxf(m, mx * sc);
+            ref = mn == -INFINITY ? 0.f : mn;
+            const float corr = __builtin_amdgcn_exp2f(m - ref);   // (0 where nothing was seen yet)
+            m = mn;
+            most = (m + RISE) / sc;
+            l *= corr;
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) o[ct] *= corr;
+        }
+        u16x8 pf;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            p[j] = __builtin_amdgcn_exp2f(fmaf(p[j], sc, -ref));
+            l += p[j];
+            const bf16_t first = (bf16_t)Op<FMT>::pack2_unit(p[j], 0.f);
+            pf[j] = part ? (bf16_t)Op<FMT>::pack2_unit(p[j] - Op<FMT>::unpack(first), 0.f) : first;
+        }
+#pragma unroll
+        for (int ct = 0; ct < CT; ct += 2) {
+            s16x4 r0, r1, r2, r3;
+            asm volatile("ds_read_b64_tr_b16 %0, %4\n\t"
+                         "ds_read_b64_tr_b16 %1, %4 offset:%6\n\t"
+                         "ds_read_b64_tr_b16 %2, %5\n\t"
+                         "ds_read_b64_tr_b16 %3, %5 offset:%6\n\t"
+                         "s_waitcnt lgkmcnt(0)"
+                         : "=&v"(r0), "=&v"(r1), "=&v"(r2), "=&v"(r3)
+                         : "v"(va[ct]), "v"(va[ct + 1]), "n"(16 * D * 2)
+                         : "memory");
+            o[ct] = Op<FMT>::mfma(tr_pair(r0, r1), pf, o[ct]);
+            o[ct + 1] = Op<FMT>::mfma(tr_pair(r2, r3), pf, o[ct + 1]);
+        }
+        if (next < end) ask_values(next);
+    }
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    __syncthreads();   // (the tiles are free)
+    float (*const red_o)[GP][D] = reinterpret_cast<float (*)[GP][D]>(tiles);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float v = o[ct][i];
+            o[ct][i] = v + dpp_move<0x128>(v);
+        }
+        if (!part) *reinterpret_cast<f32x4*>(&red_o[wave][fr][16 * ct + 4 * fg]) = o[ct];
+    }
+    if (!part && fg == 0) {
+        red_m[wave][fr] = m;
+        red_l[wave][fr] = l;
+    }
+    __syncthreads();
+    step_join_waves<FMT, D, GP>(a, red_m, red_l, red_o, share, out, grp - g0);
+}
+
+// Joins the shares of one query head: D / 4 threads times G groups of shares (every G-th, in order) ask for the values, a wave
+// forms the shares' weights meanwhile, and the groups' sums are added in their order.  256 threads as long as each has four
+// shares at most, then 1024 (16 heads of 64: 1.2 us more at 8 shares; 16 heads of 128: 3 us less at 128).
+template <int FMT, int D, int THREADS>
+__global__ __launch_bounds__(THREADS) void window_step_join_kernel(const float* __restrict__ ml, const float* __restrict__ acc,
+                                                                bf16_t* __restrict__ out, int splits) {
+    constexpr int C = D / 4, G = THREADS / C, N = MAX_SPLITS / G < 4 ? MAX_SPLITS / G : 4;
     __shared__ float wt[MAX_SPLITS];
     __shared__ float total;
     __shared__ f32x4 red[G][C];
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, c = tid % C, g = tid / C;
+    f32x4 v[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+        v[j] = *reinterpret_cast<const f32x4*>(acc + ((long)blockIdx.x * splits + min(g + j * G, splits - 1)) * D + c * 4);
     if (tid < 64) {
         float mx = -INFINITY, m[MAX_SPLITS / 64], l[MAX_SPLITS / 64];
 #pragma unroll
         for (int i = 0; i < MAX_SPLITS / 64; ++i) {
             const int s = tid + 64 * i;
-            const f32x2 v = s < splits ? *reinterpret_cast<const f32x2*>(ml + ((long)blockIdx.x * splits + s) * 2) : f32x2{-INFINITY, 0.f};
-            m[i] = v[0];
-            l[i] = v[1];
+            const f32x2 p = s < splits ? *reinterpret_cast<const f32x2*>(ml + ((long)blockIdx.x * splits + s) * 2) : f32x2{-INFINITY, 0.f};
+            m[i] = p[0];
+            l[i] = p[1];
             mx = fmaxf(mx, m[i]);
         }
         mx = wave_max(mx);
@@ -270,17 +491,16 @@ __global__ __launch_bounds__(256) void window_step_join_kernel(const float* __re
         if (tid == 0) total = sum;
     }
     __syncthreads();
-    const int c = tid % C, g = tid / C;
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int i = g; i < splits; i += G) {
-        const float w = wt[i];
-        if (w != 0.f) s += w * *reinterpret_cast<const f32x4*>(acc + ((long)blockIdx.x * splits + i) * D + c * 4);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const float w = wt[g + j * G];   // (0 past the last share)
+        if (w != 0.f) s += w * v[j];
     }
     red[g][c] = s;
     __syncthreads();
     if (g) return;
-#pragma unroll
+#pragma unroll 8
     for (int i = 1; i < G; ++i) s += red[i][c];
     const float inv = total == 0.f ? 0.f : 1.0f / total;
     typedef __attribute__((ext_vector_type(2))) uint32_t u32x2_t;
@@ -327,7 +547,7 @@ int step_splits(int B, int heads, int slots, int D) {
 }
 
 // query heads a workgroup serves at once
-int step_heads(int grp) { return grp >= 8 ? 8 : grp >= 4 ? (grp > 4 ? 8 : 4) : grp > 2 ? 4 : grp; }
+int step_heads(int grp) { return grp > 2 ? 8 : grp; }
 
 bool step_ok(const WindowStepParams& p) {
     if (p.B < 0 || p.B > 65535 || p.Hk < 1 || p.Hq < p.Hk || p.Hq % p.Hk || p.Hq > 4096) return false;
@@ -347,9 +567,14 @@ void launch_step_one(int gp, dim3 grid, hipStream_t s, const StepArgs& a) {
     switch (gp) {
         case 1: hipLaunchKernelGGL((window_step_kernel<FMT, D, 1>), grid, dim3(ST_WAVES * 64), 0, s, a); break;
         case 2: hipLaunchKernelGGL((window_step_kernel<FMT, D, 2>), grid, dim3(ST_WAVES * 64), 0, s, a); break;
-        case 4: hipLaunchKernelGGL((window_step_kernel<FMT, D, 4>), grid, dim3(ST_WAVES * 64), 0, s, a); break;
-        default: hipLaunchKernelGGL((window_step_kernel<FMT, D, 8>), grid, dim3(ST_WAVES * 64), 0, s, a); break;
+        default: hipLaunchKernelGGL((window_step_group_kernel<FMT, D>), grid, dim3(ST_WAVES * 64), 0, s, a); break;
     }
+}
+
+template <int FMT, int D>
+void launch_step_join(int heads, hipStream_t s, const StepArgs& a) {
+    if (a.splits <= 4 * (1024 / D)) hipLaunchKernelGGL((window_step_join_kernel<FMT, D, 256>), dim3(heads), dim3(256), 0, s, a.ml, a.acc, a.out, a.splits);
+    else hipLaunchKernelGGL((window_step_join_kernel<FMT, D, 1024>), dim3(heads), dim3(1024), 0, s, a.ml, a.acc, a.out, a.splits);
 }
 
 }  // namespace
@@ -388,8 +613,8 @@ hipError_t launch_window_step(const WindowStepParams& p, void* ws, size_t ws_byt
         if (p.D == 64) launch_step_one<F, 64>(gp, grid, s, a);
         else launch_step_one<F, 128>(gp, grid, s, a);
         if (a.splits > 1) {
-            if (p.D == 64) hipLaunchKernelGGL((window_step_join_kernel<F, 64>), dim3(p.B * p.Hq), dim3(256), 0, s, a.ml, a.acc, a.out, a.splits);
-            else hipLaunchKernelGGL((window_step_join_kernel<F, 128>), dim3(p.B * p.Hq), dim3(256), 0, s, a.ml, a.acc, a.out, a.splits);
+            if (p.D == 64) launch_step_join<F, 64>(p.B * p.Hq, s, a);
+            else launch_step_join<F, 128>(p.B * p.Hq, s, a);
         }
     });
     return hipGetLastError();

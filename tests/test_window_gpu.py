@@ -683,3 +683,13 @@ def test_window_attention_of_many_keys(case, dtype):
     """Rows that see hundreds of keys, some through far sinks: forward and gradients."""
     test_window_attention(case, dtype)
     test_window_attention_backward(case, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", [(16, 4, 128, 0, False, False, 16, 20000, [25000]), (1, 1, 64, 64, False, True, 4, 20000, [19990, -1]),
+                                  (24, 3, 64, 32, False, True, 0, 12000, [11999]), (7, 1, 128, 128, True, True, 3, 9000, [40, -3, 9003]),
+                                  (5, 1, 64, 64, False, True, 1, 31, [0, 31, 32, 63])])
+def test_window_attention_step_of_long_and_of_grouped_caches(case, dtype):
+    """Shares joined by both forms of the join, groups of three to eight heads and not a multiple of them, shares without a
+    slot and streams without a frame."""
+    test_window_attention_step(case, dtype)
