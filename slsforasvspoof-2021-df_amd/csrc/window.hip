@@ -879,14 +879,19 @@ __global__ __launch_bounds__(1024) void window_sink_kernel(WinArgs a) {
         u32x2_t{result2<FMT>(s[0], s[1]), result2<FMT>(s[2], s[3])};
 }
 
-constexpr int FAR_CHUNK = 1024;   // 8 workgroups a sink block at 8192 frames; their loops are as long as the near ones'
+// Queries of a workgroup of far ones: 1024 rows over the heads of a group (8 workgroups a sink block at 8192 frames and one
+// head a group), in multiples of the 128 that its waves take in turn.  Their loops are about as long as the near ones'.
+int far_chunk_of(int grp) {
+    const int n = 1024 / grp / 128 * 128;
+    return n < 128 ? 128 : n;
+}
 constexpr long WG_MAX = 0xffffffffL / 256;   // workgroups of 256 in a launch, whose work-items a 32-bit number counts
 
 // queries past the near ones of the first sink block, in chunks (0: none)
-int far_blocks_of(int T, int left, int sinks) {
-    if (sinks <= 0) return 0;
-    const long first = 127L + left + 1;
-    return first >= T ? 0 : (int)((T - first + FAR_CHUNK - 1) / FAR_CHUNK);
+int far_blocks_of(const WinArgs& a) {
+    if (a.sinks <= 0) return 0;
+    const long first = 127L + a.left + 1, chunk = far_chunk_of(a.Hq / a.Hk);
+    return first >= a.T ? 0 : (int)((a.T - first + chunk - 1) / chunk);
 }
 
 bool head_ok(const WindowHeads& x, int heads, int T, int D) {
@@ -982,7 +987,7 @@ hipError_t launch_window_attention(const WindowParams& p, float* lse, hipStream_
 size_t window_attention_bwd_workspace(const WindowParams& p) {
     WinArgs a{};
     if (!window_args(p, a) || p.B == 0 || p.T == 0) return 0;
-    const size_t fb = far_blocks_of(p.T, a.left, a.sinks), sb = (a.sinks + 31) / 32;
+    const size_t fb = far_blocks_of(a), sb = (a.sinks + 31) / 32;
     return delta_bytes(a) + dmax_bytes(a) + (fb ? (size_t)p.B * p.Hk * sb * (1 + 4 * fb) * 2 * 32 * p.D * sizeof(float) : 0);
 }
 
@@ -1005,8 +1010,8 @@ hipError_t launch_window_attention_bwd(const WindowParams& p, const float* lse, 
     a.delta = reinterpret_cast<float*>(ws);
     a.dmax = reinterpret_cast<f32x2*>(reinterpret_cast<char*>(ws) + delta_bytes(a));
     a.part = reinterpret_cast<float*>(reinterpret_cast<char*>(a.dmax) + dmax_bytes(a));
-    a.far_chunk = FAR_CHUNK;
-    a.far_blocks = far_blocks_of(p.T, a.left, a.sinks);
+    a.far_chunk = far_chunk_of(a.Hq / a.Hk);
+    a.far_blocks = far_blocks_of(a);
     const long sb = (a.sinks + 31) / 32, heads = (long)p.B * p.Hk;
     if (heads * (a.tiles + sb * a.far_blocks) + 8 + (long)p.B * p.Hq * a.tiles > WG_MAX ||
         (a.far_blocks > 0 && heads * sb * (p.D / 16) > WG_MAX / 4))

@@ -255,14 +255,13 @@ __global__ __launch_bounds__(ST_WAVES * 64) void window_step_kernel(StepArgs a) 
     step_join_waves<FMT, D, GP>(a, red_m, red_l, red_o, share, ((long)b * a.Hq + hk * grp + g0) * D, grp - g0);
 }
 
-// The same for three or more query heads a key head: on vector instructions their products take as long as the bytes (16 heads
-// on 4 of 128 channels, 32768 slots, 67 MB: 23.4 us with the join, 17.9 here; 32 heads on 4: 32.3 and 19.1, at 256 slots 14.7
-// and 7.2), so both products run on
-// the 16 x 16 x 32 MFMA, 16 columns for eight heads: a head's query as the sum of two 16-bit operands in columns i and i + 8,
-// and its probabilities likewise, so that neither is rounded to 16 bits.  A wave takes 32 slots at a time; keys go from the
-// cache to the A operand's registers, values to a tile of the wave's own (zeros past the last slot) and from there by
-// transposed reads.  Scores arrive with four consecutive slots per lane and 16-slot group, which is the order the value
-// operand's slots are enumerated in.
+// The same for three or more query heads a key head.  On vector instructions their products take as long as the bytes (16
+// heads on 4 of 128 channels, 32768 slots, 67 MB: 23.4 us with the join, 17.9 here; 32 heads on 4: 32.3 and 19.1, at 256
+// slots 14.7 and 7.2), so both run on the 16 x 16 x 32 MFMA, 16 columns for eight heads: a head's query as the sum of two
+// 16-bit operands in columns i and i + 8, and its probabilities likewise, which leaves rounding errors of 2^-17 (bfloat16)
+// and 2^-22 of each.  A wave takes 32 slots at a time; keys go from the cache to the A operand's registers, values to a tile
+// of the wave's own (zeros past the last slot) and from there by transposed reads.  Scores arrive with four consecutive
+// slots per lane in each half of the 32, which is the order the value operand's slots are enumerated in.
 template <int FMT, int D>
 __global__ __launch_bounds__(ST_WAVES * 64) void window_step_group_kernel(StepArgs a) {
     constexpr int GP = 8, GL = D / 8, KG = 64 / GL, KS = D / 32, CT = D / 16, TILE = 32 * D * 2, STEP = ST_WAVES * 32;
