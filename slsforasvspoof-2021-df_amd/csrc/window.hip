@@ -66,16 +66,18 @@ struct Div {
 struct WinArgs {
     HeadPtr q, k, v, o, d;   // o, d (dO): backward
     HeadOut out, dq, dk, dv;
-    Div by_tiles, by_item, by_batch, by_group;   // tiles, workgroups of a key head, B, Hq / Hk
+    Div by_tiles, by_near, by_far, by_batch, by_group;   // tiles, a key head's near and far workgroups, B, Hq / Hk
     float* lse;              // [B][Hq][T]
     float* delta;            // [B][Hq][T]: rowsum(dO o O)
     f32x2* dmax;             // [B][Hq][T / DELTA_ROWS]: largest |dO|, |delta| (half precision)
     float* part;             // sink keys' partial sums (see window_dkv)
+    float* near;             // all keys', where a key head's queries are shared by heads
     const int* nframes;
     int B, T, Hq, Hk;
     int left, right, sinks;  // left, right in [0, T]; sinks in [0, SINK_MAX]
     int tiles;               // tiles of a head in this launch
     int far_blocks, far_chunk;   // dkv: workgroups per sink block beyond the near tiles, queries per workgroup
+    int shares, share_heads;     // dkv: workgroups that share the queries of a key tile, query heads of each
     float scale, scale2, inv_scale;   // scale2: scale / ln 2
 };
 
@@ -642,29 +644,33 @@ __device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* ld
 //
 // The sinks' keys are seen by every later query: the queries past the near ones of a sink block (32 keys) are cut into
 // chunks of far_chunk, one workgroup each, whose four waves share the block's keys and take 32 of 128 queries in turn.
-// Their sums for the sinks' rows, and the near workgroup's for all rows of the block, go as fp32 to `part`
-// [B][Hk][sink block][1 + 4 far_blocks][dK, dV][32 keys][D] and are added in that order by window_sink_kernel.
+// Their sums for the sinks' rows, and the near workgroups' for all rows of the block, go as fp32 to `part`
+// [B][Hk][sink block][shares + 4 far_blocks][dK, dV][32 keys][D] and are added in that order by window_join_kernel.
+//
+// With few key tiles and several query heads to a key head, the heads are shared out among `shares` workgroups, whose sums
+// go to `near` [B][Hk][block of 32 keys][shares][dK, dV][32 keys][D] (to `part` for the sinks' blocks) and are added likewise.
 template <int FMT, int D, bool SPLIT>
-__device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* lds) {
+__device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, bool far, char* lds) {
     constexpr int NS = D / 16, DT = D / 32, BQ = tile_rows(D), TILE = BQ * D * 2, BUF = 2 * TILE + 2 * BQ * 4;   // Q, dO, -lse / scale, -delta
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, hi = lane >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int sink_blocks = (a.sinks + 31) / 32;
-    const unsigned wt = a.by_item.of(w), hk = a.by_batch.of(wt), b = wt - hk * a.B, bh = b * a.Hk + hk;
-    const int item = w - wt * a.by_item.d;
+    const Div& per_head = far ? a.by_far : a.by_near;
+    const unsigned wt = per_head.of(w), hk = a.by_batch.of(wt), b = wt - hk * a.B, bh = b * a.Hk + hk;
+    const int item = w - wt * per_head.d;
     const int len = frames_of(a, b);
     const int grp = a.by_group.d;
-    const bool far = item >= a.tiles;
+    const int sp = far ? 0 : (int)a.by_tiles.of(item), heads = far ? grp : a.share_heads, h0 = hk * grp + sp * a.share_heads;
     int k0w, qa, qb;   // this wave's keys; queries qa .. qb
     int block = 0, chunk = 0;
     if (!far) {
-        const int k0 = item * 128;
+        const int k0 = (item - sp * a.tiles) * 128;
         k0w = k0 + wave * 32;
         qa = max(k0 - a.right, 0);
         qb = k0 < len ? min(k0 + 127 + a.left, len - 1) : -1;
     } else {
-        block = (item - a.tiles) / a.far_blocks;
-        chunk = (item - a.tiles) % a.far_blocks;
+        block = item / a.far_blocks;
+        chunk = item % a.far_blocks;
         k0w = block * 32;
         // the near workgroup of these keys ended at this query
         const int first = (k0w / 128) * 128 + 127 + a.left + 1;
@@ -698,15 +704,15 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
     constexpr float p_lift = FMT == FMT_F16 ? P_LIFT * LN2 : 0.f;
     float turn = 1.f;   // 2^(lift of dS - lift of P), of this lane's key
     if constexpr (FMT == FMT_F16) {
-        const f32x2 top = grad_size(a, (long)b * a.Hq + hk * grp, grp, qa, qb);
+        const f32x2 top = grad_size(a, (long)b * a.Hq + h0, heads, qa, qb);
         turn = __builtin_amdgcn_exp2f(lift_of(fmaf(top[0] * (D == 64 ? 8.f : 11.f), row_size<FMT>(vf), top[1]), 8) - P_LIFT);
     }
     const int t0 = qa / BQ, nt = qb < qa ? 0 : qb / BQ - t0 + 1;
-    const int total = nt * grp;
+    const int total = nt * heads;
     LaneAt<D> at(lane, lds);
     const TileLoad<D, BQ> lq(a.q.r, lane, wave), ld(a.d.r, lane, wave);
     float stat = 0.f;   // thread t: -lse / scale of row t of the tile for t < BQ, then -delta of row t - BQ
-    int rt = t0, rh = hk * grp;   // tile and head of the next request
+    int rt = t0, rh = h0;   // tile and head of the next request
     auto request = [&](char* buf) {
         const int q0 = rt * BQ;
         lq.issue(a.q.p + b * a.q.b + rh * a.q.h, a.q.r, q0, len, buf, wave);
@@ -799,10 +805,13 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
     int half = tid;   // (hi, but not the register that held it before the loop)
     asm volatile("" : "+v"(half));
     half = (half >> 5) & 1;
-    if (far || (k0w < a.sinks && a.far_blocks > 0)) {
-        const int blk = far ? block : k0w / 32, slot = far ? 1 + chunk * 4 + wave : 0;
+    const bool sink_block = far || (k0w < a.sinks && a.far_blocks > 0);
+    if (sink_block || a.shares > 1) {
         if (far && key >= a.sinks) return;
-        float* dst = a.part + ((((long)bh * sink_blocks + blk) * (1 + 4 * a.far_blocks) + slot) * 2 * 32 + col) * D + 4 * half;
+        const int blk = far ? block : k0w / 32, slot = far ? a.shares + chunk * 4 + wave : sp;
+        const long n = sink_block ? (long)bh * sink_blocks + blk : (long)bh * 4 * a.tiles + blk;
+        float* dst = (sink_block ? a.part : a.near) +
+                     ((n * (sink_block ? a.shares + 4 * a.far_blocks : a.shares) + slot) * 2 * 32 + col) * D + 4 * half;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
@@ -831,38 +840,43 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, char* l
 }
 
 // Both sides of the backward in one launch: the key-side workgroups (the longer ones) first, the query-side ones behind
-// them fill the CUs that these leave (4 x 1001 frames: 49 -> 44 us against two launches).  The key side's count is rounded
-// up to the XCDs, so that both have their order.  Times, both sides: 4 x 1001 x 16 x 64, 201 keys, 35 us; 8192 x 16 x 64, 512
-// keys, 90 us (470 TFLOP/s of the 5 products a gradient needs, 750 of the 8 that run); 128 channels, 8 heads, 1024 keys, 142 us.
+// them fill the CUs that these leave (4 x 1001 frames: 49 -> 44 us against two launches).  The key side's near and far
+// workgroups are counted apart, each rounded up to the XCDs, so that each kind is spread over all of them.  Times, both
+// sides: 4 x 1001 x 16 x 64, 201 keys, 35 us; 8192 x 16 x 64, 512 keys, 90 us (470 TFLOP/s of the 5 products a gradient
+// needs, 750 of the 8 that run); 128 channels, 8 heads, 1024 keys, 142 us.
 template <int FMT, int D, bool SPLIT>
-__global__ __launch_bounds__(256, bwd_waves(D)) void window_bwd_kernel(WinArgs a, unsigned key_side, unsigned key_blocks) {
+__global__ __launch_bounds__(256, bwd_waves(D)) void window_bwd_kernel(WinArgs a, unsigned near, unsigned far) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     want(a.q);
     want(a.k);
     want(a.v);
     want(a.d);
     asm volatile("" ::"s"(a.lse), "s"(a.delta), "s"(a.nframes), "s"(a.T), "s"(a.left), "s"(a.right), "s"(a.sinks), "s"(a.scale));
-    if (blockIdx.x < key_blocks) {
-        if (blockIdx.x < key_side) window_dkv<FMT, D, SPLIT>(a, xcd_order(blockIdx.x, key_side), lds);
+    const unsigned near8 = (near + 7) & ~7u, keys = near8 + ((far + 7) & ~7u);
+    if (blockIdx.x < keys) {
+        const bool is_far = blockIdx.x >= near8;
+        const unsigned n = is_far ? blockIdx.x - near8 : blockIdx.x, of = is_far ? far : near;
+        if (n < of) window_dkv<FMT, D, SPLIT>(a, xcd_order(n, of), is_far, lds);
     } else {
-        window_dq<FMT, D>(a, xcd_order(blockIdx.x - key_blocks, gridDim.x - key_blocks), lds);
+        window_dq<FMT, D>(a, xcd_order(blockIdx.x - keys, gridDim.x - keys), lds);
     }
 }
 
-// The partial sums of a sink block (32 keys) -> its rows of dK and dV.  A workgroup takes one of dK, dV for 1024 / D keys;
-// four threads share a sum, each every fourth slot in ascending order, and are added in their order (one thread a sum: 12
-// instead of 4.3 us at 8192 frames).
+// The partial sums of blocks of 32 keys -> their rows of dK and dV: blocks first .. first + count - 1 of every key head, whose
+// sums lie in `sums` [B][Hk][stride blocks][slots][dK, dV][32][D], for keys that are not sinks in the first a.shares slots
+// alone.  A workgroup takes one of dK, dV for 1024 / D keys; four threads share a sum, each every fourth slot in ascending
+// order, and are added in their order (one thread a sum: 12 instead of 4.3 us for the sinks at 8192 frames).
 template <int FMT, int D>
-__global__ __launch_bounds__(1024) void window_sink_kernel(WinArgs a) {
+__global__ __launch_bounds__(1024) void window_join_kernel(WinArgs a, const float* __restrict__ sums, int slots, int stride, int first,
+                                                           int count) {
     constexpr int KEYS = 1024 / D, PARTS = 32 / KEYS;
     __shared__ f32x4 red[3][256];
-    const int sink_blocks = (a.sinks + 31) / 32, slots = 1 + 4 * a.far_blocks;
-    const int which = blockIdx.x & 1, part = (blockIdx.x >> 1) % PARTS, n = (blockIdx.x >> 1) / PARTS, blk = n % sink_blocks,
-              bh = n / sink_blocks, b = bh / a.Hk, hk = bh % a.Hk;
+    const int which = blockIdx.x & 1, part = (blockIdx.x >> 1) % PARTS, n = (blockIdx.x >> 1) / PARTS, blk = first + n % count,
+              bh = n / count, b = bh / a.Hk, hk = bh % a.Hk;
     const int len = frames_of(a, b);
     const int at = threadIdx.x & 255, sg = threadIdx.x >> 8, kl = part * KEYS + at / (D / 4), c = (at % (D / 4)) * 4;
-    const int key = blk * 32 + kl, mine = key < a.sinks ? slots : 1;
-    const float* src = a.part + (((long)n * slots * 2 + which) * 32 + kl) * D + c;
+    const int key = blk * 32 + kl, mine = key < a.sinks ? slots : a.shares;
+    const float* src = sums + ((((long)bh * stride + blk) * slots * 2 + which) * 32 + kl) * D + c;
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
     if (key < len) {
 #pragma unroll 8
@@ -885,6 +899,18 @@ int far_chunk_of(int grp) {
     const int n = 1024 / grp / 128 * 128;
     return n < 128 ? 128 : n;
 }
+// Workgroups that share a key tile's query heads: as few (a divisor of the group) as give the key side one per CU.  Their sums
+// cost 64 or 128 KiB of traffic each way a workgroup, the loop over all heads more where CUs are idle (8 heads on one, 963
+// frames 56 -> 18 us; 32 on 4 of 128 channels, 2000 frames 191 -> 93, with two per CU 120).
+constexpr long SHARE_WG = 256;
+
+int shares_of(const WinArgs& a) {
+    const long have = (long)a.B * a.Hk * a.tiles, grp = a.Hq / a.Hk;
+    long n = 1;
+    while (n < grp && (have * n < SHARE_WG || grp % n)) ++n;
+    return (int)n;
+}
+
 constexpr long WG_MAX = 0xffffffffL / 256;   // workgroups of 256 in a launch, whose work-items a 32-bit number counts
 
 // queries past the near ones of the first sink block, in chunks (0: none)
@@ -927,7 +953,7 @@ bool window_args(const WindowParams& p, WinArgs& a) {
     a.nframes = p.nframes;
     a.tiles = (p.T + 127) / 128;
     if (p.B > 0 && p.T > 0) {
-        a.by_tiles = a.by_item = Div(a.tiles);
+        a.by_tiles = Div(a.tiles);
         a.by_batch = Div(p.B);
         a.by_group = Div(p.Hq / p.Hk);
     }
@@ -939,6 +965,14 @@ HeadOut out_head(const WindowHeads& x) { return {const_cast<bf16_t*>(x.p), x.bat
 
 size_t dmax_bytes(const WinArgs& a) {
     return ((size_t)a.B * a.Hq * ((a.T + DELTA_ROWS - 1) / DELTA_ROWS) * sizeof(f32x2) + 255) & ~(size_t)255;
+}
+size_t part_bytes(const WinArgs& a, int D) {
+    const size_t fb = far_blocks_of(a), sb = (a.sinks + 31) / 32;
+    return fb ? (size_t)a.B * a.Hk * sb * (shares_of(a) + 4 * fb) * 2 * 32 * D * sizeof(float) : 0;
+}
+size_t near_bytes(const WinArgs& a, int D) {
+    const size_t n = shares_of(a);
+    return n > 1 ? (size_t)a.B * a.Hk * a.tiles * 4 * n * 2 * 32 * D * sizeof(float) : 0;
 }
 size_t delta_bytes(const WinArgs& a) { return ((size_t)a.B * a.Hq * a.T * sizeof(float) + 255) & ~(size_t)255; }
 
@@ -960,13 +994,19 @@ bool few_keys(const WinArgs& a) {
 
 template <int FMT, int D>
 hipError_t launch_bwd(const WinArgs& a, hipStream_t s) {
-    const int sb = (a.sinks + 31) / 32;
-    const unsigned ks = a.B * a.Hk * (a.tiles + sb * a.far_blocks), kb = (ks + 7) & ~7u, qs = a.B * a.Hq * a.tiles;
+    const int sb = (a.sinks + 31) / 32, blocks = (a.T + 31) / 32, first = a.far_blocks > 0 ? min(sb, blocks) : 0;
+    const unsigned near = a.B * a.Hk * a.tiles * a.shares, far = a.B * a.Hk * sb * a.far_blocks;
+    const dim3 grid(((near + 7) & ~7u) + ((far + 7) & ~7u) + a.B * a.Hq * a.tiles);
     hipLaunchKernelGGL((window_delta_kernel<FMT, D>), dim3((a.T + DELTA_ROWS - 1) / DELTA_ROWS, a.Hq, a.B), dim3(256), 0, s, a);
     const auto lds = [](bool split) { return 2 * (2 * 8192 + 2 * tile_rows(D) * 4) + frags_in_lds(FMT, D, split) * 4096; };
-    if (few_keys(a)) hipLaunchKernelGGL((window_bwd_kernel<FMT, D, true>), dim3(kb + qs), dim3(256), lds(true), s, a, ks, kb);
-    else hipLaunchKernelGGL((window_bwd_kernel<FMT, D, false>), dim3(kb + qs), dim3(256), lds(false), s, a, ks, kb);
-    if (a.far_blocks > 0) hipLaunchKernelGGL((window_sink_kernel<FMT, D>), dim3(a.B * a.Hk * sb * (D / 16)), dim3(1024), 0, s, a);
+    if (few_keys(a)) hipLaunchKernelGGL((window_bwd_kernel<FMT, D, true>), grid, dim3(256), lds(true), s, a, near, far);
+    else hipLaunchKernelGGL((window_bwd_kernel<FMT, D, false>), grid, dim3(256), lds(false), s, a, near, far);
+    if (a.far_blocks > 0)
+        hipLaunchKernelGGL((window_join_kernel<FMT, D>), dim3(a.B * a.Hk * sb * (D / 16)), dim3(1024), 0, s, a, a.part,
+                           a.shares + 4 * a.far_blocks, sb, 0, sb);
+    if (a.shares > 1 && blocks > first)
+        hipLaunchKernelGGL((window_join_kernel<FMT, D>), dim3(a.B * a.Hk * (blocks - first) * (D / 16)), dim3(1024), 0, s, a, a.near,
+                           a.shares, 4 * a.tiles, first, blocks - first);
     return hipGetLastError();
 }
 
@@ -987,8 +1027,7 @@ hipError_t launch_window_attention(const WindowParams& p, float* lse, hipStream_
 size_t window_attention_bwd_workspace(const WindowParams& p) {
     WinArgs a{};
     if (!window_args(p, a) || p.B == 0 || p.T == 0) return 0;
-    const size_t fb = far_blocks_of(a), sb = (a.sinks + 31) / 32;
-    return delta_bytes(a) + dmax_bytes(a) + (fb ? (size_t)p.B * p.Hk * sb * (1 + 4 * fb) * 2 * 32 * p.D * sizeof(float) : 0);
+    return delta_bytes(a) + dmax_bytes(a) + part_bytes(a, p.D) + near_bytes(a, p.D);
 }
 
 hipError_t launch_window_attention_bwd(const WindowParams& p, const float* lse, const WindowHeads& dout, const WindowHeads& dq,
@@ -1012,11 +1051,16 @@ hipError_t launch_window_attention_bwd(const WindowParams& p, const float* lse, 
     a.part = reinterpret_cast<float*>(reinterpret_cast<char*>(a.dmax) + dmax_bytes(a));
     a.far_chunk = far_chunk_of(a.Hq / a.Hk);
     a.far_blocks = far_blocks_of(a);
+    a.shares = shares_of(a);
+    a.share_heads = p.Hq / p.Hk / a.shares;
+    a.near = reinterpret_cast<float*>(reinterpret_cast<char*>(a.part) + part_bytes(a, p.D));
     const long sb = (a.sinks + 31) / 32, heads = (long)p.B * p.Hk;
-    if (heads * (a.tiles + sb * a.far_blocks) + 8 + (long)p.B * p.Hq * a.tiles > WG_MAX ||
+    const long items = (long)a.tiles * a.shares + sb * a.far_blocks;
+    if (heads * items + 16 + (long)p.B * p.Hq * a.tiles > WG_MAX ||   // (shared tiles are few: 4 * 512 blocks at most)
         (a.far_blocks > 0 && heads * sb * (p.D / 16) > WG_MAX / 4))
         return hipErrorInvalidValue;
-    a.by_item = Div((unsigned)(a.tiles + sb * a.far_blocks));
+    a.by_near = Div((unsigned)(a.tiles * a.shares));
+    if (a.far_blocks > 0) a.by_far = Div((unsigned)(sb * a.far_blocks));
     hipError_t rc = hipSuccess;
     SLSMI_FMT_DISPATCH(p.fmt, rc = p.D == 64 ? (launch_bwd<F, 64>(a, s)) : (launch_bwd<F, 128>(a, s)));
     return rc;

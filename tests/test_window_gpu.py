@@ -693,3 +693,12 @@ def test_window_attention_step_of_long_and_of_grouped_caches(case, dtype):
     """Shares joined by both forms of the join, groups of three to eight heads and not a multiple of them, shares without a
     slot and streams without a frame."""
     test_window_attention_step(case, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", [(2, 330, 8, 1, 64, 28, 28, 1, [330, 100]), (1, 500, 6, 2, 128, None, 0, 0, None), (1, 700, 12, 2, 64, 60, 0, 70, [650]),
+                                  (2, 260, 10, 1, 64, None, None, 0, [260, 0]), (1, 33, 4, 1, 128, 5, 5, 33, None), (1, 1200, 16, 2, 64, 250, 250, 40, None)])
+def test_window_attention_with_shared_heads(case, dtype):
+    """Several query heads to a key head and few key tiles: the heads' sums for a key come from several workgroups."""
+    test_window_attention(case, dtype)
+    test_window_attention_backward(case, dtype)
