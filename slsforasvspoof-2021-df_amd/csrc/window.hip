@@ -452,12 +452,42 @@ __global__ __launch_bounds__(256, fwd_waves(D)) void window_fwd_kernel(WinArgs a
     }
 }
 
+// sum_j P_ij dP_ij of row q, whose channels c .. c + 7 of dO this lane holds (D / 8 lanes a row, the same total in all)
+template <int FMT, int D>
+__device__ __forceinline__ float exact_delta(const WinArgs& a, int b, int h, int q, int len, int c, u16x8 dout) {
+    const int hk = a.by_group.of(h);
+    const bf16_t* const kr = a.k.p + b * a.k.b + hk * a.k.h + c;
+    const bf16_t* const vr = a.v.p + b * a.v.b + hk * a.v.h + c;
+    const u16x8 qx = *reinterpret_cast<const u16x8*>(a.q.p + b * a.q.b + h * a.q.h + (long)q * a.q.r + c);
+    const float ls = a.lse[((long)b * a.Hq + h) * a.T + q] * LOG2E;
+    const int lo = max(q - a.left, 0), hi = min(q + a.right, len - 1), first = min(a.sinks, lo);   // sinks before the window
+    float sum = 0.f;
+    for (int i = 0; i < first + hi - lo + 1; ++i) {
+        const int j = i < first ? i : lo + i - first;
+        const u16x8 k = *reinterpret_cast<const u16x8*>(kr + (long)j * a.k.r), v = *reinterpret_cast<const u16x8*>(vr + (long)j * a.v.r);
+        float s = 0.f, dp = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            s = fmaf(Op<FMT>::unpack(qx[e]), Op<FMT>::unpack(k[e]), s);
+            dp = fmaf(Op<FMT>::unpack(dout[e]), Op<FMT>::unpack(v[e]), dp);
+        }
+        s = lane_group_sum<D / 8>(s);
+        dp = lane_group_sum<D / 8>(dp);
+        sum = fmaf(__builtin_amdgcn_exp2f(fmaf(s, a.scale2, -ls)), dp, sum);
+    }
+    return sum;
+}
+
 // ---- backward, first launch: delta = rowsum(dO o O) of DELTA_ROWS rows of a head per workgroup, and (half precision) the
 // largest |dO| and |delta| among them.  D / 8 lanes hold a row, 16 bytes of both each.  Bound by reading both once (8192 x
 // 16 x 64: 34 MB in 6.4 us, 5.2 TB/s).
+//
+// FEW: rows that see a handful of keys feel the rounding of O through delta more than everything else (error of dQ and dK
+// against rounding once at the end, dS in two operands: 2.5 times with 2 keys, 1.7 with 5, 1.5 with up to 29, 1.33 with 17);
+// there delta = sum_j P_ij dP_ij over the row's keys, in 32 bits throughout (1.00 times).
 constexpr int DELTA_ROWS = 128;
 
-template <int FMT, int D>
+template <int FMT, int D, bool FEW>
 __global__ __launch_bounds__(256) void window_delta_kernel(WinArgs a) {
     constexpr int GL = D / 8, PER = 256 / GL;
     __shared__ f32x2 red[4];
@@ -469,15 +499,19 @@ __global__ __launch_bounds__(256) void window_delta_kernel(WinArgs a) {
     for (int i = 0; i < DELTA_ROWS / PER; ++i) {
         const int q = blockIdx.x * DELTA_ROWS + i * PER + threadIdx.x / GL, row = min(q, max(len - 1, 0));   // (a batch has a row 0)
         const u16x8 x = *reinterpret_cast<const u16x8*>(a.d.p + b * a.d.b + h * a.d.h + (long)row * a.d.r + c);
-        const u16x8 y = *reinterpret_cast<const u16x8*>(a.o.p + b * a.o.b + h * a.o.h + (long)row * a.o.r + c);
+        u16x8 y = x;
+        if constexpr (!FEW) y = *reinterpret_cast<const u16x8*>(a.o.p + b * a.o.b + h * a.o.h + (long)row * a.o.r + c);
         float s = 0.f, m = 0.f;
+        if constexpr (FEW) {
+            if (q < len) s = exact_delta<FMT, D>(a, b, h, q, len, c, x);
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const float d = Op<FMT>::unpack(x[e]);
-            s = fmaf(d, Op<FMT>::unpack(y[e]), s);
+            if constexpr (!FEW) s = fmaf(d, Op<FMT>::unpack(y[e]), s);
             m = fmaxf(m, fabsf(d) < INFINITY ? fabsf(d) : 0.f);   // (infinite rows say nothing about the others')
         }
-        s = lane_group_sum<GL>(s);
+        if constexpr (!FEW) s = lane_group_sum<GL>(s);
         if (q < len) {
             top = f32x2{fmaxf(top[0], m), fmaxf(top[1], fabsf(s) < INFINITY ? fabsf(s) : 0.f)};
             if (c == 0) a.delta[bh * a.T + q] = s;
@@ -987,9 +1021,12 @@ hipError_t launch_fwd(const WinArgs& a, hipStream_t s) {
 // Whether dK's dS is split in two operands as well.  Against rounding everything once at the end, dK's error is 1.6 to 1.7
 // times larger with dS rounded once where rows see few keys (52 to 268 frames, or one side only: the early rows), 1.44 to
 // 1.49 from about 160 keys on both sides or 1024 on one; split it is 1.02 to 1.4, for 25 % of the key side's time.
+int row_keys(const WinArgs& a) {   // the most a row sees
+    const int span = a.left + a.right + 1 + a.sinks;
+    return span < a.T ? span : a.T;
+}
 bool few_keys(const WinArgs& a) {
-    const int span = a.left + a.right + 1 + a.sinks, keys = span < a.T ? span : a.T;
-    return keys <= 160 || (a.right < a.left && a.T <= 1024);
+    return row_keys(a) <= 160 || (a.right < a.left && a.T <= 1024);
 }
 
 template <int FMT, int D>
@@ -997,7 +1034,9 @@ hipError_t launch_bwd(const WinArgs& a, hipStream_t s) {
     const int sb = (a.sinks + 31) / 32, blocks = (a.T + 31) / 32, first = a.far_blocks > 0 ? min(sb, blocks) : 0;
     const unsigned near = a.B * a.Hk * a.tiles * a.shares, far = a.B * a.Hk * sb * a.far_blocks;
     const dim3 grid(((near + 7) & ~7u) + ((far + 7) & ~7u) + a.B * a.Hq * a.tiles);
-    hipLaunchKernelGGL((window_delta_kernel<FMT, D>), dim3((a.T + DELTA_ROWS - 1) / DELTA_ROWS, a.Hq, a.B), dim3(256), 0, s, a);
+    const dim3 rows((a.T + DELTA_ROWS - 1) / DELTA_ROWS, a.Hq, a.B);
+    if (a.T <= 48 || row_keys(a) <= 16) hipLaunchKernelGGL((window_delta_kernel<FMT, D, true>), rows, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((window_delta_kernel<FMT, D, false>), rows, dim3(256), 0, s, a);
     const auto lds = [](bool split) { return 2 * (2 * 8192 + 2 * tile_rows(D) * 4) + frags_in_lds(FMT, D, split) * 4096; };
     if (few_keys(a)) hipLaunchKernelGGL((window_bwd_kernel<FMT, D, true>), grid, dim3(256), lds(true), s, a, near, far);
     else hipLaunchKernelGGL((window_bwd_kernel<FMT, D, false>), grid, dim3(256), lds(false), s, a, near, far);

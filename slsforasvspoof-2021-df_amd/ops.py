@@ -672,8 +672,7 @@ def qk_norm_rope_backward(dout: torch.Tensor, qkv: torch.Tensor, heads: int, kv_
         out, lddx = qkv.new_empty(lead + (width,)), width
     else:
         lddx = _rows_arg(out, "out", width, dtype, index, lead)
-    dw = torch.empty(2, D, dtype=torch.float32, device=qkv.device)
-    dwq, dwk = dw[0], dw[1]
+    dwq, dwk = torch.empty(2, D, dtype=torch.float32, device=qkv.device).unbind(0)
     lib = _lib.load()
     n = lib.slsmi_qk_norm_rope_backward_workspace_bytes(rows, D)
     ws = torch.empty(n, dtype=torch.uint8, device=qkv.device)

@@ -702,3 +702,20 @@ def test_window_attention_with_shared_heads(case, dtype):
     """Several query heads to a key head and few key tiles: the heads' sums for a key come from several workgroups."""
     test_window_attention(case, dtype)
     test_window_attention_backward(case, dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", [(2, 200, 4, 4, 64, 1, 0, 0, [200, 77]), (2, 150, 4, 2, 128, 2, 2, 0, None), (1, 300, 2, 1, 64, 4, 0, 1, None),
+                                  (3, 29, 4, 1, 64, None, 0, 0, [29, 1, 0]), (1, 400, 2, 2, 64, 5, 0, 10, [390]), (2, 48, 6, 2, 128, None, None, 0, None)])
+def test_gradients_of_rows_that_see_a_handful_of_keys(case, dtype):
+    """Neither the rounding of the saved output nor that of dS shows: dq and dk are off by their own rounding and what two
+    16-bit operands leave of dS (2^-17 or 2^-22 of each term; u 2^-7 is more) and 32-bit arithmetic."""
+    B, T, H, Hk, D, left, right, sinks, lens = case
+    q, k, v, nf = win_case(*case, dtype)
+    do = rnd(B, T, H, D, seed=9, dtype=dtype)
+    out, lse = ops.window_attention(q, k, v, left, right, sinks, nframes=nf, return_lse=True)
+    dq, dk, _ = ops.window_attention_backward(do, q, k, v, out, lse, left, right, sinks, nframes=nf)
+    r = attention64(q, k, v, lens, left, right, sinks, D ** -0.5, do)
+    u = unit(dtype)
+    for g, n, m in ((dq, "dq", "Mq"), (dk, "dk", "Mk")):
+        close(g, r[n], u * (r[n].abs() + r[m] * 2 ** -7) + 3 * SLACK * r[m] + 2 ** -24, n)
