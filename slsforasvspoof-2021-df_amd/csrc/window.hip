@@ -452,42 +452,24 @@ __global__ __launch_bounds__(256, fwd_waves(D)) void window_fwd_kernel(WinArgs a
     }
 }
 
-// sum_j P_ij dP_ij of row q, whose channels c .. c + 7 of dO this lane holds (D / 8 lanes a row, the same total in all)
-template <int FMT, int D>
-__device__ __forceinline__ float exact_delta(const WinArgs& a, int b, int h, int q, int len, int c, u16x8 dout) {
-    const int hk = a.by_group.of(h);
-    const bf16_t* const kr = a.k.p + b * a.k.b + hk * a.k.h + c;
-    const bf16_t* const vr = a.v.p + b * a.v.b + hk * a.v.h + c;
-    const u16x8 qx = *reinterpret_cast<const u16x8*>(a.q.p + b * a.q.b + h * a.q.h + (long)q * a.q.r + c);
-    const float ls = a.lse[((long)b * a.Hq + h) * a.T + q] * LOG2E;
-    const int lo = max(q - a.left, 0), hi = min(q + a.right, len - 1), first = min(a.sinks, lo);   // sinks before the window
-    float sum = 0.f;
-    for (int i = 0; i < first + hi - lo + 1; ++i) {
-        const int j = i < first ? i : lo + i - first;
-        const u16x8 k = *reinterpret_cast<const u16x8*>(kr + (long)j * a.k.r), v = *reinterpret_cast<const u16x8*>(vr + (long)j * a.v.r);
-        float s = 0.f, dp = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            s = fmaf(Op<FMT>::unpack(qx[e]), Op<FMT>::unpack(k[e]), s);
-            dp = fmaf(Op<FMT>::unpack(dout[e]), Op<FMT>::unpack(v[e]), dp);
-        }
-        s = lane_group_sum<D / 8>(s);
-        dp = lane_group_sum<D / 8>(dp);
-        sum = fmaf(__builtin_amdgcn_exp2f(fmaf(s, a.scale2, -ls)), dp, sum);
-    }
-    return sum;
-}
-
 // ---- backward, first launch: delta = rowsum(dO o O) of DELTA_ROWS rows of a head per workgroup, and (half precision) the
 // largest |dO| and |delta| among them.  D / 8 lanes hold a row, 16 bytes of both each.  Bound by reading both once (8192 x
 // 16 x 64: 34 MB in 6.4 us, 5.2 TB/s).
-//
-// FEW: rows that see a handful of keys feel the rounding of O through delta more than everything else (error of dQ and dK
-// against rounding once at the end, dS in two operands: 2.5 times with 2 keys, 1.7 with 5, 1.5 with up to 29, 1.33 with 17);
-// there delta = sum_j P_ij dP_ij over the row's keys, in 32 bits throughout (1.00 times).
-constexpr int DELTA_ROWS = 128;
+constexpr int DELTA_ROWS = 128;   // (a query tile: the exact form below counts them alike)
 
-template <int FMT, int D, bool FEW>
+// the largest of a workgroup's values (infinite ones were left out: they say nothing about the others')
+__device__ __forceinline__ void put_sizes(f32x2 top, f32x2* red, f32x2* to) {
+    top = f32x2{wave_max(top[0]), wave_max(top[1])};
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+#pragma unroll
+        for (int w = 1; w < 4; ++w) top = f32x2{fmaxf(top[0], red[w][0]), fmaxf(top[1], red[w][1])};
+        *to = top;
+    }
+}
+
+template <int FMT, int D>
 __global__ __launch_bounds__(256) void window_delta_kernel(WinArgs a) {
     constexpr int GL = D / 8, PER = 256 / GL;
     __shared__ f32x2 red[4];
@@ -499,34 +481,21 @@ __global__ __launch_bounds__(256) void window_delta_kernel(WinArgs a) {
     for (int i = 0; i < DELTA_ROWS / PER; ++i) {
         const int q = blockIdx.x * DELTA_ROWS + i * PER + threadIdx.x / GL, row = min(q, max(len - 1, 0));   // (a batch has a row 0)
         const u16x8 x = *reinterpret_cast<const u16x8*>(a.d.p + b * a.d.b + h * a.d.h + (long)row * a.d.r + c);
-        u16x8 y = x;
-        if constexpr (!FEW) y = *reinterpret_cast<const u16x8*>(a.o.p + b * a.o.b + h * a.o.h + (long)row * a.o.r + c);
+        const u16x8 y = *reinterpret_cast<const u16x8*>(a.o.p + b * a.o.b + h * a.o.h + (long)row * a.o.r + c);
         float s = 0.f, m = 0.f;
-        if constexpr (FEW) {
-            if (q < len) s = exact_delta<FMT, D>(a, b, h, q, len, c, x);
-        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const float d = Op<FMT>::unpack(x[e]);
-            if constexpr (!FEW) s = fmaf(d, Op<FMT>::unpack(y[e]), s);
-            m = fmaxf(m, fabsf(d) < INFINITY ? fabsf(d) : 0.f);   // (infinite rows say nothing about the others')
+            s = fmaf(d, Op<FMT>::unpack(y[e]), s);
+            m = fmaxf(m, fabsf(d) < INFINITY ? fabsf(d) : 0.f);
         }
-        if constexpr (!FEW) s = lane_group_sum<GL>(s);
+        s = lane_group_sum<GL>(s);
         if (q < len) {
             top = f32x2{fmaxf(top[0], m), fmaxf(top[1], fabsf(s) < INFINITY ? fabsf(s) : 0.f)};
             if (c == 0) a.delta[bh * a.T + q] = s;
         }
     }
-    if constexpr (FMT == FMT_F16) {
-        top = f32x2{wave_max(top[0]), wave_max(top[1])};
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = top;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-#pragma unroll
-            for (int w = 1; w < 4; ++w) top = f32x2{fmaxf(top[0], red[w][0]), fmaxf(top[1], red[w][1])};
-            a.dmax[bh * gridDim.x + blockIdx.x] = top;
-        }
-    }
+    if constexpr (FMT == FMT_F16) put_sizes(top, red, a.dmax + bh * gridDim.x + blockIdx.x);
 }
 
 // Half precision holds dS as c dS, c a power of two (here its logarithm), so that gradients under a loss scale stay below
@@ -553,14 +522,17 @@ __device__ __forceinline__ f32x2 grad_size(const WinArgs& a, long first, int n, 
         }
     return f32x2{wave_max(top[0]), wave_max(top[1])};
 }
-// largest value of the row that a lane and the lane 32 further hold
-template <int FMT, int NS>
+// largest value of the row that a lane and the lane 32 further hold; FINITE: infinite ones left out
+template <int FMT, bool FINITE, int NS>
 __device__ __forceinline__ float row_size(const u16x8 (&d)[NS]) {
     float top = 0.f;
 #pragma unroll
     for (int s = 0; s < NS; ++s)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(Op<FMT>::unpack(d[s][e])));
+        for (int e = 0; e < 8; ++e) {
+            const float v = fabsf(Op<FMT>::unpack(d[s][e]));
+            top = fmaxf(top, !FINITE || v < INFINITY ? v : 0.f);
+        }
     const f32x2 two = both_halves(top);
     return fmaxf(two[0], two[1]);
 }
@@ -568,7 +540,12 @@ __device__ __forceinline__ float row_size(const u16x8 (&d)[NS]) {
 // ---- backward, queries: dQ; the forward's loop with P recomputed from lse.  The product dO V^T starts from -delta, so
 // dP - delta leaves the matrix units.  dQ and dK / dV each recompute P (7 products instead of 5): one pass for all three
 // would add partial dQ to memory once per key tile, 340 MB at 8192 x 16 x 64 and 512 keys, more time than the products take.
-template <int FMT, int D>
+//
+// DELTA: the same pass for delta alone, delta_i = sum_j P_ij dP_ij in 32 bits instead of rowsum(dO o O), for rows that see a
+// handful of keys.  They feel the rounding of O through delta more than everything else: error of dQ and dK against rounding
+// once at the end 2.5 times with 2 keys, 1.7 with 5, 1.5 with up to 29, 1.33 with 17; 1.00 this way (8 x 4096 frames, 16 keys:
+// 197 -> 231 us).
+template <int FMT, int D, bool DELTA>
 __device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* lds) {
     constexpr int BN = tile_rows(D), NS = D / 16, DT = D / 32, TILE = BN * D * 2;
     const int tid = threadIdx.x, lane = tid & 63, col = lane & 31, hi = lane >> 5;
@@ -590,6 +567,10 @@ __device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* ld
     const int len = frames_of(a, b);
     // (formed where it is used: held through the loop it would cost registers that the kernel does not have)
     const auto dqrow = [&]() { return a.dq.p + b * a.dq.b + h * a.dq.h + (long)q * a.dq.r; };
+    if (DELTA && q0 >= len) {
+        if (FMT == FMT_F16 && tid == 0) a.dmax[bh * a.tiles + tile] = f32x2{0.f, 0.f};
+        return;
+    }
     if (q0 >= len) {
         if (q < a.T) {
 #pragma unroll
@@ -607,8 +588,9 @@ __device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* ld
     const bool live = q < len;
     const float sc = a.scale2;
     const long stat = (long)bh * a.T + min(q, len - 1);
-    const float lift = FMT == FMT_F16 ? lift_of(row_size<FMT>(df), 0) : 0.f;
-    const float ls = a.lse[stat] * LOG2E - lift, delta = a.delta[stat];
+    const float lift = FMT == FMT_F16 && !DELTA ? lift_of(row_size<FMT, false>(df), 0) : 0.f;
+    const float ls = a.lse[stat] * LOG2E - lift, delta = DELTA ? 0.f : a.delta[stat];
+    float sum = 0.f;
     f32x16 acc[DT], start;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt] = zero16();
@@ -635,12 +617,19 @@ __device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* ld
                 s = mfma32<FMT>(row_frag<D>(Ks, 32 * u, at, e), qf[e], s);
                 dp = mfma32<FMT>(row_frag<D>(Vs, 32 * u, at, e), df[e], dp);
             }
-            __builtin_amdgcn_sched_barrier(0);
             u16x8 kt2[2][DT];
-            tr_frags2<D, 64 * D * u>(at, kt2);
+            if constexpr (!DELTA) {
+                __builtin_amdgcn_sched_barrier(0);
+                tr_frags2<D, 64 * D * u>(at, kt2);
+            }
             if (!vis.all(kb)) hide_keys(s, kb, kb + 4 * hi, q, len, a.left, a.right, a.sinks);
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(fmaf(s[r], sc, -ls)) * dp[r];
+            if constexpr (DELTA) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sum += s[r];
+                return;
+            }
 #pragma unroll
             for (int st = 0; st < 2; ++st) {
                 u16x8 e, rest;
@@ -655,6 +644,16 @@ __device__ __forceinline__ void window_dq(const WinArgs& a, unsigned w, char* ld
         block(Const<0>{});
         if constexpr (BN == 64) block(Const<1>{});
         at.turn(it & 1 ? -2 * TILE : 2 * TILE);
+    }
+    if constexpr (DELTA) {
+        sum = halves_sum(sum);
+        if (live && hi == 0) a.delta[stat] = sum;
+        if constexpr (FMT == FMT_F16) {
+            const float m = row_size<FMT, true>(df), d = fabsf(sum);
+            __syncthreads();   // (the tiles are free)
+            put_sizes(live ? f32x2{m, d < INFINITY ? d : 0.f} : f32x2{0.f, 0.f}, reinterpret_cast<f32x2*>(lds), a.dmax + bh * a.tiles + tile);
+        }
+        return;
     }
     float fin = a.scale;
     if constexpr (FMT == FMT_F16) {   // (the row's lift, a whole number, once more: through the loop there is no register for it)
@@ -739,7 +738,7 @@ __device__ __forceinline__ void window_dkv(const WinArgs& a, unsigned w, bool fa
     float turn = 1.f;   // 2^(lift of dS - lift of P), of this lane's key
     if constexpr (FMT == FMT_F16) {
         const f32x2 top = grad_size(a, (long)b * a.Hq + h0, heads, qa, qb);
-        turn = __builtin_amdgcn_exp2f(lift_of(fmaf(top[0] * (D == 64 ? 8.f : 11.f), row_size<FMT>(vf), top[1]), 8) - P_LIFT);
+        turn = __builtin_amdgcn_exp2f(lift_of(fmaf(top[0] * (D == 64 ? 8.f : 11.f), row_size<FMT, false>(vf), top[1]), 8) - P_LIFT);
     }
     const int t0 = qa / BQ, nt = qb < qa ? 0 : qb / BQ - t0 + 1;
     const int total = nt * heads;
@@ -892,8 +891,18 @@ __global__ __launch_bounds__(256, bwd_waves(D)) void window_bwd_kernel(WinArgs a
         const unsigned n = is_far ? blockIdx.x - near8 : blockIdx.x, of = is_far ? far : near;
         if (n < of) window_dkv<FMT, D, SPLIT>(a, xcd_order(n, of), is_far, lds);
     } else {
-        window_dq<FMT, D>(a, xcd_order(blockIdx.x - keys, gridDim.x - keys), lds);
+        window_dq<FMT, D, false>(a, xcd_order(blockIdx.x - keys, gridDim.x - keys), lds);
     }
+}
+
+template <int FMT, int D>
+__global__ __launch_bounds__(256, bwd_waves(D)) void window_exact_delta_kernel(WinArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    want(a.q);
+    want(a.k);
+    want(a.v);
+    want(a.d);
+    window_dq<FMT, D, true>(a, xcd_order(blockIdx.x, gridDim.x), lds);
 }
 
 // The partial sums of blocks of 32 keys -> their rows of dK and dV: blocks first .. first + count - 1 of every key head, whose
@@ -1034,9 +1043,10 @@ hipError_t launch_bwd(const WinArgs& a, hipStream_t s) {
     const int sb = (a.sinks + 31) / 32, blocks = (a.T + 31) / 32, first = a.far_blocks > 0 ? min(sb, blocks) : 0;
     const unsigned near = a.B * a.Hk * a.tiles * a.shares, far = a.B * a.Hk * sb * a.far_blocks;
     const dim3 grid(((near + 7) & ~7u) + ((far + 7) & ~7u) + a.B * a.Hq * a.tiles);
-    const dim3 rows((a.T + DELTA_ROWS - 1) / DELTA_ROWS, a.Hq, a.B);
-    if (a.T <= 48 || row_keys(a) <= 16) hipLaunchKernelGGL((window_delta_kernel<FMT, D, true>), rows, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((window_delta_kernel<FMT, D, false>), rows, dim3(256), 0, s, a);
+    if (a.T <= 48 || row_keys(a) <= 16)
+        hipLaunchKernelGGL((window_exact_delta_kernel<FMT, D>), dim3(a.B * a.Hq * a.tiles), dim3(256), 4 * 8192, s, a);
+    else
+        hipLaunchKernelGGL((window_delta_kernel<FMT, D>), dim3((a.T + DELTA_ROWS - 1) / DELTA_ROWS, a.Hq, a.B), dim3(256), 0, s, a);
     const auto lds = [](bool split) { return 2 * (2 * 8192 + 2 * tile_rows(D) * 4) + frags_in_lds(FMT, D, split) * 4096; };
     if (few_keys(a)) hipLaunchKernelGGL((window_bwd_kernel<FMT, D, true>), grid, dim3(256), lds(true), s, a, near, far);
     else hipLaunchKernelGGL((window_bwd_kernel<FMT, D, false>), grid, dim3(256), lds(false), s, a, near, far);
