@@ -56,9 +56,9 @@ __device__ __forceinline__ void step_nothing(const StepArgs& a, long share, long
 }
 
 // The waves' maxima, sums and values -> the result, or this workgroup's share of it.  live: query heads there are.
-template <int FMT, int D, int GP>
+template <int FMT, int D, int GP, int ROW>
 __device__ __forceinline__ void step_join_waves(const StepArgs& a, const float (&red_m)[ST_WAVES][GP], const float (&red_l)[ST_WAVES][GP],
-                                                const float (*red_o)[GP][D], long share, long out, int live) {
+                                                const float (*red_o)[GP][ROW], long share, long out, int live) {
     for (int t = threadIdx.x; t < GP * D; t += ST_WAVES * 64) {
         const int i = t / D, d = t % D;
         if (i >= live) break;
@@ -256,8 +256,8 @@ __global__ __launch_bounds__(ST_WAVES * 64) void window_step_kernel(StepArgs a) 
 }
 
 // The same for three or more query heads a key head.  On vector instructions their products take as long as the bytes (16
-// heads on 4 of 128 channels, 32768 slots, 67 MB: 23.4 us with the join, 17.9 here; 32 heads on 4: 32.3 and 19.1, at 256
-// slots 14.7 and 7.2), so both run on the 16 x 16 x 32 MFMA, 16 columns for eight heads: a head's query as the sum of two
+// heads on 4 of 128 channels, 32768 slots, 67 MB: 23.4 us with the join, 17.4 here; 32 heads on 4: 32.3 and 18.2, at 256
+// slots 14.7 and 6.9), so both run on the 16 x 16 x 32 MFMA, 16 columns for eight heads: a head's query as the sum of two
 // 16-bit operands in columns i and i + 8, and its probabilities likewise, which leaves rounding errors of 2^-17 (bfloat16)
 // and 2^-22 of each.  A wave takes 32 slots at a time; keys go from the cache to the A operand's registers, values to a tile
 // of the wave's own (zeros past the last slot) and from there by transposed reads.  Scores arrive with four consecutive
@@ -267,7 +267,7 @@ __global__ __launch_bounds__(ST_WAVES * 64) void window_step_group_kernel(StepAr
     constexpr int GP = 8, GL = D / 8, KG = 64 / GL, KS = D / 32, CT = D / 16, TILE = 32 * D * 2, STEP = ST_WAVES * 32;
     constexpr float RISE = 8.f;   // how far (powers of two) scores may pass the reference before it moves
     __shared__ __attribute__((aligned(1024))) char tiles[ST_WAVES * TILE];
-    __shared__ __attribute__((aligned(16))) bf16_t qs[2][GP][D];
+    __shared__ __attribute__((aligned(16))) bf16_t qs[2][GP][D + 8];   // (rows 16 bytes apart in the banks)
     __shared__ __attribute__((aligned(16))) bf16_t nks[D];
     __shared__ float2 tab[ST_WAVES][64];
     __shared__ float red_m[ST_WAVES][GP], red_l[ST_WAVES][GP];
@@ -435,7 +435,8 @@ __global__ __launch_bounds__(ST_WAVES * 64) void window_step_group_kernel(StepAr
     l += __shfl_xor(l, 16, 64);
     l += __shfl_xor(l, 32, 64);
     __syncthreads();   // (the tiles are free)
-    float (*const red_o)[GP][D] = reinterpret_cast<float (*)[GP][D]>(tiles);
+    constexpr int ROW = D + 4;
+    float (*const red_o)[GP][ROW] = reinterpret_cast<float (*)[GP][ROW]>(tiles);
 #pragma unroll
     for (int ct = 0; ct < CT; ++ct) {
 #pragma unroll

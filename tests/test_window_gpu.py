@@ -719,3 +719,40 @@ def test_gradients_of_rows_that_see_a_handful_of_keys(case, dtype):
     u = unit(dtype)
     for g, n, m in ((dq, "dq", "Mq"), (dk, "dk", "Mk")):
         close(g, r[n], u * (r[n].abs() + r[m] * 2 ** -7) + 3 * SLACK * r[m] + 2 ** -24, n)
+
+
+def test_grouped_heads_in_a_captured_graph():
+    """Shared key heads: forward, gradient (heads shared among workgroups, sums joined) and a step on the matrix units,
+    captured once and replayed on new inputs with eager work in between."""
+    q, k, v, nf = win_case(2, 330, 8, 1, 64, 28, 28, 1, [330, 100], torch.float16)
+    q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    do = rnd(2, 330, 8, 64, seed=9, dtype=torch.float16)
+    row = rnd(2, 10 * 64, seed=11, dtype=torch.float16)
+    cache = [rnd(2, 1, 600, 64, seed=i, dtype=torch.float16) for i in (6, 7)]
+    pos = torch.tensor([700, 20], device=DEV)
+
+    def run():
+        out, lse = ops.window_attention(q, k, v, 28, 28, 1, nframes=nf, return_lse=True)
+        grads = ops.window_attention_backward(do, q, k, v, out, lse, 28, 28, 1, nframes=nf)
+        return (out, lse) + grads + (ops.window_attention_step(row, *cache, pos, 8, 4),)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            held = run()
+    torch.cuda.current_stream().wait_stream(side)
+    for i in range(3):
+        for t, s in ((q, 20), (k, 30), (v, 40), (do, 50)):
+            t.copy_(rnd(*t.shape, seed=s + i, dtype=torch.float16))
+        pos += 1
+        before = [c.clone() for c in cache]
+        graph.replay()
+        torch.cuda.synchronize()
+        after = [c.clone() for c in cache]
+        for c, b in zip(cache, before):
+            c.copy_(b)
+        want = run()
+        assert all(torch.equal(a, b) for a, b in zip(held, want)) and all(torch.equal(a, b) for a, b in zip(after, cache))
