@@ -1028,14 +1028,15 @@ hipError_t launch_fwd(const WinArgs& a, hipStream_t s) {
 }
 
 // Whether dK's dS is split in two operands as well.  Against rounding everything once at the end, dK's error is 1.6 to 1.7
-// times larger with dS rounded once where rows see few keys (52 to 268 frames, or one side only: the early rows), 1.44 to
-// 1.49 from about 160 keys on both sides or 1024 on one; split it is 1.02 to 1.4, for 25 % of the key side's time.
+// times larger with dS rounded once where rows see few keys (52 to 268 frames); from about 160 keys on it is 1.43 to 1.48,
+// but where the window looks back further than ahead the early rows bring it to 1.47 to 1.52 up to 4000 frames (1.45 at
+// 8192).  Split it is 1.02 to 1.4, for 25 % of the key side's time.
 int row_keys(const WinArgs& a) {   // the most a row sees
     const int span = a.left + a.right + 1 + a.sinks;
     return span < a.T ? span : a.T;
 }
 bool few_keys(const WinArgs& a) {
-    return row_keys(a) <= 160 || (a.right < a.left && a.T <= 1024);
+    return row_keys(a) <= 160 || (a.right < a.left && a.T <= 4096);
 }
 
 template <int FMT, int D>
