@@ -756,3 +756,19 @@ def test_grouped_heads_in_a_captured_graph():
             c.copy_(b)
         want = run()
         assert all(torch.equal(a, b) for a, b in zip(held, want)) and all(torch.equal(a, b) for a, b in zip(after, cache))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_result_in_the_place_of_the_queries_and_refused_places(dtype):
+    q, k, v, nf = win_case(2, 300, 4, 4, 64, 40, 7, 3, [300, 129], dtype)
+    q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    want, lse = ops.window_attention(q, k, v, 40, 7, 3, nframes=nf, return_lse=True)
+    own = q.clone()
+    assert torch.equal(ops.window_attention(own, k, v, 40, 7, 3, nframes=nf, out=own), want) and torch.equal(own, want)
+    do = rnd(2, 300, 4, 64, seed=9, dtype=dtype)
+    for bad in (lambda: ops.window_attention(q, k, v, 40, 7, 3, out=k), lambda: ops.window_attention(q, k, v, 40, 7, 3, out=v),
+                lambda: ops.window_attention_backward(do, q, k, v, want, lse, 40, 7, 3, dq=do),
+                lambda: ops.window_attention_backward(do, q, k, v, want, lse, 40, 7, 3, dk=k),
+                lambda: ops.window_attention_backward(do, q, k, v, want, lse, 40, 7, 3, dq=own, dk=own)):
+        with pytest.raises(_lib.SlsmiError):
+            bad()
